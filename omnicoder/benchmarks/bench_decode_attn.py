@@ -26,7 +26,7 @@ def main(argv=None):
     ap.add_argument("--heads", type=int, default=16)
     ap.add_argument("--window", type=int, default=4096)
     ap.add_argument("--mem", type=int, default=64)
-    ap.add_argument("--kv", default="int8", choices=["int8", "bf16"])
+    ap.add_argument("--kv", default="int8", choices=["int8", "bf16", "int4"])
     ap.add_argument("--iters", type=int, default=20)
     ap.add_argument("--mha", type=int, default=0, metavar="KV_HEADS",
                     help="MHA / GQA cache with this many kv heads (head dim --head-dim) instead of the MLA latent")
@@ -35,6 +35,7 @@ def main(argv=None):
     from omnicoder.inference.kv_cache import quantize_int8
     from omnicoder.ops import _ext
     from omnicoder.ops.decode import decode_attention
+    from omnicoder.ops.kv4 import kv4_alloc, kv4_row_bytes, kv4_write
     dev = torch.device("cuda")
     B, Tn, H = a.batch, a.tn, a.heads
     DQ, DV = (a.head_dim, a.head_dim) if a.mha else (576, 512)
@@ -51,6 +52,17 @@ def main(argv=None):
         k, ks = quantize_int8(k, -1)
         if v is not None:
             v, vs = quantize_int8(v, -1)
+    elif a.kv == "int4":
+        rows = torch.arange(L, device=dev).expand(B, -1)
+        pairs = []
+        for x in (k, v):
+            if x is None:
+                pairs += [None, None]
+                continue
+            x = x if a.mha else x[:, :, None]
+            pairs += kv4_alloc(B, x.shape[2], L, DQ, 0 if a.mha else DV, dev)
+            kv4_write(rows, x, *pairs[-2:])
+        k, ks, v, vs = pairs
     kv_len = torch.full((B,), a.ctx + Tn, dtype=torch.int32, device=dev)
     q_pos = (kv_len[:, None] - Tn + torch.arange(Tn, device=dev)[None, :]).to(torch.int32)
     kw = dict(window=a.window, scale=1.0 / math.sqrt(DQ), k_scale=ks, v_scale=vs, latent_v_dim=0 if a.mha else DV,
@@ -70,7 +82,7 @@ def main(argv=None):
     times.sort()
     ms = times[len(times) // 2]
     rows = (min(a.ctx + Tn, a.window + Tn - 1) if a.window else a.ctx + Tn) + a.mem
-    row_bytes = (a.mha * (DQ + DV) if a.mha else DQ) * (1 if a.kv == "int8" else 2)
+    row_bytes = (2 * a.mha * kv4_row_bytes(DQ) if a.mha else kv4_row_bytes(DQ, DV)) if a.kv == "int4" else (a.mha * (DQ + DV) if a.mha else DQ) * (1 if a.kv == "int8" else 2)
     row_bytes += (4 * (2 * a.mha if a.mha else 1)) if a.kv == "int8" else 0
     nbytes = B * rows * row_bytes
     print(json.dumps({"kernel": f"decode attention ({'MHA/GQA %d kv heads x %d' % (a.mha, DQ) if a.mha else 'MLA latent'})", "batch": B, "tn": Tn, "heads": H, "ctx": a.ctx,

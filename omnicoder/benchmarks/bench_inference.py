@@ -169,7 +169,7 @@ def main(argv=None):
     ap.add_argument("--batch", type=int, default=64)
     ap.add_argument("--prompt", type=int, default=8192)
     ap.add_argument("--gen", type=int, default=512)
-    ap.add_argument("--kv", default="int8", choices=["int8", "bf16"])
+    ap.add_argument("--kv", default="int8", choices=["int8", "bf16", "int4"])
     ap.add_argument("--spec", type=int, default=0, help="draft tokens per step (0: plain decode)")
     ap.add_argument("--prefill_chunk", type=int, default=4, help="sequences per prefill call")
     ap.add_argument("--layers", type=int, default=0, help="override the layer count (quick runs only)")

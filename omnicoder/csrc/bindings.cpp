@@ -691,4 +691,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("epilogue"), py::arg("alpha") = 1.0, py::arg("block_n") = 256);
   omni::register_kernels(m);
   omni::register_ep(m);
+  omni::register_kv4(m);
 }

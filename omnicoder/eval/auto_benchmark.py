@@ -7,7 +7,7 @@ code (HumanEval-style pass@k), VQA / caption / ASR scoring from JSONL, a summary
 CSV).  Each part runs only when its input is given; nothing is downloaded.
 
   * throughput: greedy decode tokens/s of the model for each requested KV-cache format
-    (bf16 / int8 on GPU, the u8 / nf4 grouped formats through the decode-step runner);
+    (bf16 / int8 / int4 on GPU, the u8 / nf4 grouped formats through the decode-step runner);
     with --speculative a draft preset and its acceptance;
   * multiple choice (any of --mmlu_jsonl, --arc_jsonl, ...): rows {"question", "choices": [...],
     "answer": index or text}; the prediction is the choice with the highest mean token
@@ -74,8 +74,8 @@ def throughput(model, kv_formats: list[str], seq_len: int, gen: int, batch: int)
     out = {}
     dev = next(model.parameters()).device
     for kv in kv_formats:
-        if kv in ("none", "int8"):
-            if kv == "int8" and dev.type != "cuda":
+        if kv in ("none", "int8", "int4"):
+            if kv != "none" and dev.type != "cuda":
                 continue
             out[f"tokens_per_s_kv_{kv}"] = bench_tokens_per_second(model, seq_len=seq_len, gen_tokens=gen,
                                                                    batch=batch, kvq=kv)

@@ -14,7 +14,8 @@ Differences from the reference, by design:
     them by rejection sampling (exact-match when greedy), so the output distribution
     is the target's; the reference accepts by a verifier-probability threshold and
     re-feeds accepted tokens one at a time (generate.py:2925-3048);
-  * `kvq="int8"` stores the cache as int8 with per-token (MLA) / per-head-per-token
+  * `kvq="int4"` stores the cache in 4 bits with a scale and minimum per group of 64 (omnicoder.ops.kv4);
+    `kvq="int8"` stores the cache as int8 with per-token (MLA) / per-head-per-token
     (MHA/GQA) scales.
 """
 from __future__ import annotations
@@ -270,7 +271,7 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int, temperature: f
         cfg.attn.window = window_size
     if compress_kv_slots:
         cfg.attn.mem_slots = int(compress_kv_slots)
-    kv_dtype = "int8" if kvq in ("int8", "u8") else "bf16"
+    kv_dtype = {"int8": "int8", "u8": "int8", "int4": "int4"}.get(kvq, "bf16")
     P = 0 if prefix_embeds is None else int(prefix_embeds.shape[1])
     L = max_len or (P + S + max_new_tokens + max(0, speculative_draft_len) + 2)
     gen = None
@@ -674,7 +675,7 @@ def main(argv=None):
     ap.add_argument("--presence_penalty", type=float, default=0.0)
     ap.add_argument("--frequency_penalty", type=float, default=0.0)
     ap.add_argument("--logit_bias_file", default=None, help="JSON {token id: additive bias}")
-    ap.add_argument("--kvq", default="none", choices=["none", "int8", "u8"])
+    ap.add_argument("--kvq", default="none", choices=["none", "int8", "u8", "int4"])
     ap.add_argument("--window_size", type=int, default=0)
     ap.add_argument("--draft_preset", default=None)
     ap.add_argument("--draft_ckpt", default=None)

@@ -8,6 +8,9 @@ Per layer:
     per (sequence, position).  Decoding attends over this latent directly
     (absorbed up-projections, see OmniLM.prepare_inference).
 
+With kv_dtype "int4" both kinds are stored as 4-bit codes [B, Hk, L, W / 2] (MLA: Hk = 1) and bf16
+(scale, minimum) pairs per group of 64 dims, in `k` / `v` and `ks` / `vs`; see omnicoder.ops.kv4.
+
 `lengths[b]` counts the cached positions of sequence b; writes go to
 positions lengths[b] .. lengths[b]+T_new-1, stored at cache rows
 `sink + position`.  With `cfg.attn.mem_slots` = M > 0 the first M rows hold
@@ -25,6 +28,7 @@ from __future__ import annotations
 import torch
 
 from ..config import ModelConfig
+from ..ops.kv4 import kv4_alloc, kv4_read, kv4_write
 
 
 def quantize_int8(x: torch.Tensor, dim: int = -1) -> tuple[torch.Tensor, torch.Tensor]:
@@ -44,7 +48,7 @@ class KVCache:
         if dtype is None:
             dtype = torch.bfloat16 if str(device).startswith("cuda") else torch.float32
         self.cfg, self.batch, self.max_len, self.device, self.dtype = cfg, batch, max_len, torch.device(device), dtype
-        assert kv_dtype in ("bf16", "int8"), kv_dtype
+        assert kv_dtype in ("bf16", "int8", "int4"), kv_dtype
         self.kv_dtype = kv_dtype
         self.mla = cfg.attn.kind == "mla"
         self.sink = int(cfg.attn.mem_slots)          # rows reserved for compressed memory
@@ -54,7 +58,14 @@ class KVCache:
         store = torch.int8 if kv_dtype == "int8" else dtype
         max_len = max_len + self.sink
         for _ in range(cfg.n_layers):
-            if self.mla:
+            if kv_dtype == "int4":
+                r = cfg.attn.kv_lora_rank if self.mla else 0
+                heads, w = (1, r + cfg.attn.qk_rope_dim) if self.mla else (cfg.n_kv_heads, cfg.head_dim)
+                for codes, params in ((self.k, self.ks), (self.v, self.vs)):
+                    c, p = (None, None) if self.mla and codes is self.v else kv4_alloc(batch, heads, max_len, w, r, device)
+                    codes.append(c)
+                    params.append(p)
+            elif self.mla:
                 w = cfg.attn.kv_lora_rank + cfg.attn.qk_rope_dim
                 self.k.append(torch.zeros(batch, max_len, w, dtype=store, device=device))
                 self.v.append(None)
@@ -79,6 +90,10 @@ class KVCache:
     def write(self, layer: int, pos: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None = None):
         """Store new entries at positions pos [B, T]; k [B, T, ...] (MLA: latent [B, T, r+dr])."""
         B, T = pos.shape
+        if self.kv_dtype == "int4":
+            kv4_write(pos, k[:, :, None] if self.mla else k, self.k[layer], self.ks[layer], v, self.v[layer],
+                      self.vs[layer], self.sink)
+            return
         if k.is_cuda and self.k[layer].dtype in (torch.int8, torch.bfloat16):
             from ..ops import _ext
             C = _ext.load()
@@ -125,6 +140,12 @@ class KVCache:
                 t = store[layer]
                 if t is None:
                     continue
+                if self.kv_dtype == "int4":
+                    rows = torch.arange(M, M + n_old, device=self.device).expand(self.batch, -1)
+                    old = kv4_read(rows, t, scale[layer], dtype=torch.float32)
+                    segs = torch.stack([old[:, a:max(b, a + 1)].mean(1) for a, b in zip(bounds[:-1], bounds[1:])], 1)
+                    kv4_write(torch.arange(M, device=self.device).expand(self.batch, -1), segs, t, scale[layer])
+                    continue
                 rows = t[:, M:M + n_old].float()
                 if scale[layer] is not None:
                     rows = rows * scale[layer][:, M:M + n_old].unsqueeze(-1)
@@ -167,6 +188,11 @@ class KVCache:
     def layer_kv(self, layer: int, dtype=None):
         """Dequantised (k, v) of a layer (MLA: latent, None)."""
         dtype = dtype or self.dtype
+        if self.kv_dtype == "int4":          # head-major storage -> [B, L, Hk, D] (MLA: [B, L, r + dr])
+            rows = torch.arange(self.k[layer].shape[2], device=self.device).expand(self.batch, -1)
+            if self.mla:
+                return kv4_read(rows, self.k[layer], self.ks[layer], dtype=dtype)[:, :, 0], None
+            return kv4_read(rows, self.k[layer], self.ks[layer], self.v[layer], self.vs[layer], dtype=dtype)
         if self.kv_dtype == "int8":
             k = dequantize_int8(self.k[layer], self.ks[layer], -1, dtype)
             v = None if self.v[layer] is None else dequantize_int8(self.v[layer], self.vs[layer], -1, dtype)

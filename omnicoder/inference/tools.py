@@ -5,7 +5,7 @@ ToolRegistry: named tools; `run_calls(text)` finds `<tool>name(arg)</tool>`
 spans in generated text, executes them (python code in the sandboxed child
 process of the RL rewards, a safe arithmetic evaluator, user functions) and
 splices `<result>...</result>` back in.
-estimate_memory(cfg, ...): bytes of weights, KV cache (bf16 / int8 latent or
+estimate_memory(cfg, ...): bytes of weights, KV cache (bf16 / int8 / int4 latent or
 per-head), activations of a decode step, optimizer state for training.
 UnifiedRouter: dispatches a request to the text / image / audio handler by
 its declared modality (or by file extension of an attached path).
@@ -86,9 +86,14 @@ def estimate_memory(cfg, batch: int = 1, seq: int = 2048, kv_dtype: str = "bf16"
     m = cfg.moe
     ffn = (3 * D * m.ffn_dim * (m.n_experts + m.n_shared_experts) + m.n_experts * D) if m.enabled else 3 * D * cfg.ffn_dim
     n_params += L * (att + ffn + 2 * D)
-    kv_elem = 1 if kv_dtype == "int8" else 2
-    kv = L * batch * seq * kv_row * kv_elem + (L * batch * seq * 4 * (1 if a.kind == "mla" else 2 * cfg.n_kv_heads)
-                                                if kv_dtype == "int8" else 0)
+    if kv_dtype == "int4":
+        from ..ops.kv4 import kv4_row_bytes
+        kv = L * batch * seq * (kv4_row_bytes(kv_row, a.kv_lora_rank) if a.kind == "mla" else
+                                2 * cfg.n_kv_heads * kv4_row_bytes(cfg.head_dim))
+    else:
+        kv_elem = 1 if kv_dtype == "int8" else 2
+        kv = L * batch * seq * kv_row * kv_elem + (L * batch * seq * 4 * (1 if a.kind == "mla" else 2 * cfg.n_kv_heads)
+                                                    if kv_dtype == "int8" else 0)
     act = batch * D * 2 * 8 + batch * cfg.vocab_size * 4
     out = {"params": n_params, "weights_bytes": n_params * param_bytes, "kv_cache_bytes": kv,
            "decode_activation_bytes": act}

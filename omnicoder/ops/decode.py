@@ -15,8 +15,10 @@ absorbed output projection consumes.
 CUDA: MLA latent caches of the model sizes (576/512, 320/256) run a tcgen05
 kernel (keys on the MMA M side, query rows on N, any number of query rows);
 other layouts run the split-KV CUDA-core kernel (<= 64 query rows per call).
-Both take bf16 or int8 (per-token / per-head scaled) caches.  CPU: dense
-masked softmax (the oracle).
+Both take bf16 or int8 (per-token / per-head scaled) caches.  A uint8 cache is
+a 4-bit one (omnicoder.ops.kv4: codes [B, Hk, L, W / 2] with its bf16 parameters
+as k_scale / v_scale) and runs kernels of its own.  CPU: dense masked softmax
+(the oracle).
 """
 from __future__ import annotations
 
@@ -25,6 +27,7 @@ import math
 import torch
 
 from . import _ext
+from .kv4 import decode_attention_kv4
 
 
 def decode_attention_torch(q, k, v, q_pos, kv_len, *, window=0, scale=None, k_scale=None, v_scale=None,
@@ -62,6 +65,9 @@ def decode_attention_torch(q, k, v, q_pos, kv_len, *, window=0, scale=None, k_sc
 
 def decode_attention(q, k, v, q_pos, kv_len, *, window=0, scale=None, k_scale=None, v_scale=None,
                      latent_v_dim=0, sink_rows=0, n_sink=0):
+    if k.dtype == torch.uint8:
+        return decode_attention_kv4(q, k, v, q_pos, kv_len, window=window, scale=scale, k_params=k_scale,
+                                    v_params=v_scale, latent_v_dim=latent_v_dim, sink_rows=sink_rows, n_sink=n_sink)
     if not q.is_cuda:
         return decode_attention_torch(q, k, v, q_pos, kv_len, window=window, scale=scale, k_scale=k_scale,
                                       v_scale=v_scale, latent_v_dim=latent_v_dim, sink_rows=sink_rows,

@@ -248,7 +248,8 @@ def _cmd_kv_budget(a) -> int:
 
 def kv_bytes_at(cfg, ctx: int, kvq: str = "bf16", group: int = 64, batch: int = 1) -> int:
     """KV bytes of `batch` sequences of `ctx` tokens: bf16; int8 as this framework stores it (one
-    fp32 scale per latent row, or per head for GQA); u8 / nf4 with one fp32 scale per `group`."""
+    fp32 scale per latent row, or per head for GQA) and int4 (a bf16 pair per group of 64); u8 / nf4
+    with one fp32 scale per `group`."""
     a = cfg.attn
     if a.kind == "mla":
         per_tok, rows = a.kv_lora_rank + a.qk_rope_dim, 1
@@ -259,6 +260,9 @@ def kv_bytes_at(cfg, ctx: int, kvq: str = "bf16", group: int = 64, batch: int = 
         return n * per_tok * 2
     if kvq == "int8":
         return n * (per_tok + rows * 4)
+    if kvq == "int4":
+        from ..ops.kv4 import kv4_row_bytes
+        return n * rows * kv4_row_bytes(per_tok // rows, a.kv_lora_rank if a.kind == "mla" else 0)
     bits = {"u8": 8, "nf4": 4}[kvq]
     return n * (per_tok * bits // 8 + -(-per_tok // group) * 4)
 
@@ -1069,7 +1073,7 @@ def _parser() -> argparse.ArgumentParser:
     p.add_argument("--prompt_len", type=int, default=32)
     p.add_argument("--new_tokens", type=int, default=64)
     p.add_argument("--batch", type=int, default=1)
-    p.add_argument("--kv_dtype", default="bf16", choices=["bf16", "int8"])
+    p.add_argument("--kv_dtype", default="bf16", choices=["bf16", "int8", "int4"])
     p.add_argument("--out", default="weights/metrics_canaries.json")
     p.add_argument("--device", default=dev)
     p.set_defaults(fn=_cmd_metrics_canary)
@@ -1084,7 +1088,7 @@ def _parser() -> argparse.ArgumentParser:
     p = sub.add_parser("mobile-budget", help="resident bytes of a package at a target context")
     p.add_argument("--release_root", default="weights/phone")
     p.add_argument("--target_ctx", type=int, default=8192)
-    p.add_argument("--kvq", default="int8", choices=["bf16", "int8", "u8", "nf4"])
+    p.add_argument("--kvq", default="int8", choices=["bf16", "int8", "int4", "u8", "nf4"])
     p.add_argument("--budget_gb", type=float, default=4.0)
     p.add_argument("--preset", default=None, help="model config (default: the package's manifest)")
     p.add_argument("--bench_json", default="", help="metrics JSON whose tokens/s must reach --min_tps")
