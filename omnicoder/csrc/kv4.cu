@@ -11,8 +11,7 @@
 // p > q_pos[b, t] - window.
 #include <algorithm>
 
-#include "common.cuh"
-#include "kv4.h"
+#include "kv4_device.cuh"
 
 namespace omni {
 
@@ -20,12 +19,7 @@ namespace {
 
 using bf16 = __nv_bfloat16;
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kMinScale = 7.52316384526264e-37f;  // 2^-120
-
-__device__ __forceinline__ long long load_pos(const void* p, bool is64, long long i) {
-  return is64 ? reinterpret_cast<const long long*>(p)[i] : (long long)reinterpret_cast<const int*>(p)[i];
-}
 
 // ---------------------------------------------------------------------------
 // Eight consecutive values of one type <-> fp32
@@ -54,13 +48,6 @@ __device__ __forceinline__ void load8(const void* base, long long i, float* x) {
 }
 
 template <int TYPE>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if (TYPE == KV4_BF16) return pack_bf16x2(a, b);
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-template <int TYPE>
 __device__ __forceinline__ void store8(void* base, long long i, const float* x) {
   if (TYPE == KV4_F32) {
     float4* p = reinterpret_cast<float4*>(reinterpret_cast<float*>(base) + i);
@@ -68,15 +55,8 @@ __device__ __forceinline__ void store8(void* base, long long i, const float* x) 
     p[1] = make_float4(x[4], x[5], x[6], x[7]);
   } else {
     *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(base) + i) =
-        make_uint4(pack2<TYPE>(x[0], x[1]), pack2<TYPE>(x[2], x[3]), pack2<TYPE>(x[4], x[5]), pack2<TYPE>(x[6], x[7]));
+        make_uint4(kv4_pack2<TYPE>(x[0], x[1]), kv4_pack2<TYPE>(x[2], x[3]), kv4_pack2<TYPE>(x[4], x[5]), kv4_pack2<TYPE>(x[6], x[7]));
   }
-}
-
-template <int TYPE>
-__device__ __forceinline__ float load1(const void* base, long long i) {
-  if (TYPE == KV4_F32) return reinterpret_cast<const float*>(base)[i];
-  if (TYPE == KV4_BF16) return __bfloat162float(reinterpret_cast<const bf16*>(base)[i]);
-  return __half2float(reinterpret_cast<const __half*>(base)[i]);
 }
 
 template <int TYPE>
@@ -113,7 +93,7 @@ __device__ __forceinline__ IoIndex io_index(const Kv4IO& a) {
   const int r = k - x.h * per_head;
   x.t = r / pieces;
   x.piece = r - x.t * pieces;
-  x.row = a.row_offset + load_pos(a.pos, a.pos64, (long long)blockIdx.y * a.T + x.t);
+  x.row = a.row_offset + kv4_load_pos(a.pos, a.pos64, (long long)blockIdx.y * a.T + x.t);
   return x;
 }
 
@@ -214,22 +194,6 @@ dim3 io_grid(const Kv4IO& a) {
 // take 32-row tiles in turn; a lane owns a row for the scores and every 32nd
 // value dim for the output.  Statistics and sums in fp32.
 // ---------------------------------------------------------------------------
-// Rows that a query (or a block of them) sees: [0, sink) and [lo, hi).
-struct Seen {
-  int lo, hi;
-};
-
-__device__ __forceinline__ Seen seen_rows(const Kv4Attend& a, int b, int t) {
-  const long long len = load_pos(a.kv_len, a.len64, b), qp = load_pos(a.q_pos, a.pos64, (long long)b * a.Tn + t);
-  const long long end = min(min(len, qp + 1), (long long)(a.L - a.sink_rows));
-  const long long first = a.window > 0 ? max(qp - a.window + 1, 0ll) : 0ll;
-  Seen s;
-  s.lo = a.sink_rows + (int)min(first, (long long)(a.L - a.sink_rows));
-  s.hi = a.sink_rows + (int)max(end, 0ll);
-  s.hi = max(s.hi, s.lo);
-  return s;
-}
-
 constexpr int kRowWarps = 8;
 constexpr int kRowDims = 32;  // value dims of a lane: V <= 1024
 
@@ -242,9 +206,9 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv4_row_kernel(const Kv4Attend
   const int row = blockIdx.x, b = blockIdx.y, lane = lane_id(), warp = warp_id();
   const int t = row / a.H, h = row % a.H, hk = h / (a.H / a.Hk);
   const long long qi = ((long long)b * a.Tn * a.H + row) * a.W;
-  for (int i = threadIdx.x; i < a.W; i += kRowWarps * 32) sq[i] = load1<TYPE>(a.q, qi + i) * a.scale * kLog2e;
+  for (int i = threadIdx.x; i < a.W; i += kRowWarps * 32) sq[i] = kv4_load1<TYPE>(a.q, qi + i) * a.scale * kKv4Log2e;
   __syncthreads();
-  const Seen seen = seen_rows(a, b, t);
+  const Kv4Seen seen = kv4_seen(a, b, t);
   const uint8_t* kc = a.k.codes + b * a.k.c_b + hk * a.k.c_h;
   const uint8_t* kp = a.k.params + b * a.k.p_b + hk * a.k.p_h;
   const bool latent = a.v.codes == nullptr;
@@ -348,13 +312,14 @@ void kv4_read(const Kv4IO& a, cudaStream_t s) {
 
 Kv4Plan kv4_plan(const Kv4Attend& a) {
   Kv4Plan p{};
-  (void)a;
+  p.splits = 1;
+  if (a.v.codes != nullptr && a.group == 64 && (a.W == 64 || a.W == 128)) kv4_heads_plan(a, p);
   return p;
 }
 
 void kv4_attend(const Kv4Attend& a, const Kv4Plan& plan, cudaStream_t s) {
-  (void)plan;
-  if (a.type == KV4_F16) launch_rows<KV4_F16>(a, s);
+  if (plan.kernel == 1) kv4_heads_launch(a, plan, s);
+  else if (a.type == KV4_F16) launch_rows<KV4_F16>(a, s);
   else launch_rows<KV4_BF16>(a, s);
 }
 
