@@ -314,11 +314,13 @@ Kv4Plan kv4_plan(const Kv4Attend& a) {
   Kv4Plan p{};
   p.splits = 1;
   if (a.v.codes != nullptr && a.group == 64 && (a.W == 64 || a.W == 128)) kv4_heads_plan(a, p);
+  if (a.v.codes == nullptr && a.group == 64 && a.W == a.V + 64 && (a.V == 256 || a.V == 512)) kv4_latent_plan(a, p);
   return p;
 }
 
 void kv4_attend(const Kv4Attend& a, const Kv4Plan& plan, cudaStream_t s) {
   if (plan.kernel == 1) kv4_heads_launch(a, plan, s);
+  else if (plan.kernel == 2) kv4_latent_launch(a, plan, s);
   else if (a.type == KV4_F16) launch_rows<KV4_F16>(a, s);
   else launch_rows<KV4_BF16>(a, s);
 }

@@ -110,5 +110,7 @@ __device__ __forceinline__ float q_normaliser(float amax, float* unscale) {
 void kv4_combine(const Kv4Attend& a, int splits, cudaStream_t s);
 void kv4_heads_launch(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s);
 void kv4_heads_plan(const Kv4Attend& a, Kv4Plan& p);
+void kv4_latent_launch(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s);
+void kv4_latent_plan(const Kv4Attend& a, Kv4Plan& p);
 
 }  // namespace omni
