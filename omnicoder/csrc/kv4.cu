@@ -22,41 +22,43 @@ using bf16 = __nv_bfloat16;
 constexpr float kMinScale = 7.52316384526264e-37f;  // 2^-120
 
 // ---------------------------------------------------------------------------
-// Eight consecutive values of one type <-> fp32
+// Sixteen consecutive values of one type <-> fp32
 // ---------------------------------------------------------------------------
+constexpr int kPiece = 16;
+
 template <int TYPE>
-__device__ __forceinline__ void load8(const void* base, long long i, float* x) {
-  if (TYPE == KV4_F32) {
-    const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + i);
-    const float4 a = p[0], b = p[1];
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-  } else {
-    const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(base) + i);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+__device__ __forceinline__ void load_piece(const void* base, long long i, float* x, uint32_t* bits) {
+  constexpr int kWords = TYPE == KV4_F32 ? 16 : 8;
+  const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(base) + i * (TYPE == KV4_F32 ? 4 : 2));
+  uint32_t w[kWords];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (TYPE == KV4_BF16) {
-        x[2 * k] = bf16_lo(u[k]);
-        x[2 * k + 1] = bf16_hi(u[k]);
-      } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[k]));
-        x[2 * k] = f.x;
-        x[2 * k + 1] = f.y;
-      }
+  for (int k = 0; k < kWords / 4; ++k) *reinterpret_cast<uint4*>(w + 4 * k) = p[k];
+#pragma unroll
+  for (int k = 0; k < kWords; ++k) {
+    if (TYPE == KV4_F32) {
+      x[k] = __uint_as_float(w[k]);
+    } else if (TYPE == KV4_BF16) {
+      x[2 * k] = bf16_lo(w[k]);
+      x[2 * k + 1] = bf16_hi(w[k]);
+      bits[k] = w[k];
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+      x[2 * k] = f.x;
+      x[2 * k + 1] = f.y;
     }
   }
 }
 
 template <int TYPE>
-__device__ __forceinline__ void store8(void* base, long long i, const float* x) {
-  if (TYPE == KV4_F32) {
-    float4* p = reinterpret_cast<float4*>(reinterpret_cast<float*>(base) + i);
-    p[0] = make_float4(x[0], x[1], x[2], x[3]);
-    p[1] = make_float4(x[4], x[5], x[6], x[7]);
-  } else {
-    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(base) + i) =
-        make_uint4(kv4_pack2<TYPE>(x[0], x[1]), kv4_pack2<TYPE>(x[2], x[3]), kv4_pack2<TYPE>(x[4], x[5]), kv4_pack2<TYPE>(x[6], x[7]));
-  }
+__device__ __forceinline__ void store_piece(void* base, long long i, const float* x) {
+  constexpr int kWords = TYPE == KV4_F32 ? 16 : 8;
+  uint4* p = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(base) + i * (TYPE == KV4_F32 ? 4 : 2));
+  uint32_t w[kWords];
+#pragma unroll
+  for (int k = 0; k < kWords; ++k)
+    w[k] = TYPE == KV4_F32 ? __float_as_uint(x[k]) : kv4_pack2<TYPE>(x[2 * k], x[2 * k + 1]);
+#pragma unroll
+  for (int k = 0; k < kWords / 4; ++k) p[k] = *reinterpret_cast<uint4*>(w + 4 * k);
 }
 
 template <int TYPE>
@@ -68,125 +70,222 @@ __device__ __forceinline__ void store1(void* base, long long i, float x) {
 }
 
 // ---------------------------------------------------------------------------
-// Append and read back.  A thread owns eight dims (one 16-byte piece of a
-// 16-bit row, four bytes of codes); the threads of a group of g dims are
-// neighbours in a warp.  Threads run over (head, token, piece) of a sequence
-// with the token in the middle, so that a warp writes whole sectors of one
-// head's rows.  Both are bound by memory, single tokens by the launch.
+// Append and read back.  A thread owns sixteen dims of kPasses rows; the threads of
+// a group of g dims are neighbours in a warp, and a block's rows run over the
+// tokens of one head and then the next, so that a warp writes whole sectors of
+// the codes.
 // ---------------------------------------------------------------------------
 constexpr int kIoThreads = 256;
+constexpr int kPasses = 4;
 
-struct IoIndex {
-  int h, t, piece;
-  long long row;
-  bool active;
+struct IoGrid {
+  int pieces, rows_per_pass, passes;  // threads of a row, rows of a pass
+  uint32_t total, mul_t, shift_t;     // rows Hk * T of a sequence; n / T = (n * mul_t) >> 32 >> shift_t
 };
 
-__device__ __forceinline__ IoIndex io_index(const Kv4IO& a) {
-  const int pieces = a.W / 8, per_head = a.T * pieces;
-  const int total = per_head * a.Hk;
-  const long long i = (long long)blockIdx.x * kIoThreads + threadIdx.x;
-  IoIndex x;
-  x.active = i < total;
-  const int k = x.active ? (int)i : 0;
-  x.h = k / per_head;
-  const int r = k - x.h * per_head;
-  x.t = r / pieces;
-  x.piece = r - x.t * pieces;
+struct IoRow {
+  int h, t;
+  long long row;  // of the cache; -1: nothing to do
+};
+
+__device__ __forceinline__ IoRow io_row(const Kv4IO& a, const IoGrid& g, uint32_t r) {
+  IoRow x;
+  x.h = a.T == 1 ? (int)r : (int)(__umulhi(r, g.mul_t) >> g.shift_t);
+  x.t = (int)r - x.h * a.T;
   x.row = a.row_offset + kv4_load_pos(a.pos, a.pos64, (long long)blockIdx.y * a.T + x.t);
+  if (x.row < 0 || x.row >= a.L) x.row = -1;
   return x;
 }
 
-// Round (x - m) / s, decided as if the quotient were exact: d + e = x - m
-// exactly, r = d - n s exactly (n s has at most 12 significant bits and lies
-// within s of d), and r + e is compared with half a step.
-__device__ __forceinline__ int kv4_code(float x, float m, float s, float inv) {
-  const float d = x - m;
-  const float back = d - x;
-  const float e = (x - (d - back)) - (m + back);
-  float n = rintf(d * inv);
-  const float r = fmaf(-n, s, d), half = 0.5f * s;
-  const bool odd = ((int)n & 1) != 0;
-  if (r > half || (r == half && (e > 0.f || (e == 0.f && odd)))) n += 1.f;
-  else if (r < -half || (r == -half && (e < 0.f || (e == 0.f && odd)))) n -= 1.f;
-  return (int)fminf(fmaxf(n, 0.f), 15.f);
-}
-
-template <int TYPE>
-__global__ void __launch_bounds__(kIoThreads) kv4_write_kernel(const Kv4IO a) {
-  const IoIndex ix = io_index(a);
-  const int b = blockIdx.y;
-  const Kv4Cache& c = a.cache[blockIdx.z];
-  const Kv4Rows& src = a.rows[blockIdx.z];
-  float x[8];
-  load8<TYPE>(src.x, b * src.x_b + ix.t * src.x_t + ix.h * src.x_h + ix.piece * 8, x);
-  float lo = x[0], hi = x[0];
-  bool bad = false;
+// Round (x - m) / s, .. < 15.5, decided as if the quotient were exact: d + e = x - m exactly,
+// r = d - n s exactly for n next to it (n s has at most 12 significant bits), and r + e is compared
+// with half a step; ties to even.
+__device__ __forceinline__ uint32_t kv4_codes8_exact(const float* x, float m, float s, float inv) {
+  uint32_t code = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-    bad |= (__float_as_uint(x[i]) & 0x7f800000u) == 0x7f800000u;
+    const float d = x[i] - m, back = d - x[i], half = 0.5f * s;
+    const float e = (x[i] - (d - back)) - (m + back);
+    float n = rintf(d * inv);
+    const float r = fmaf(-n, s, d);
+    const bool odd = ((int)n & 1) != 0;
+    if (r > half || (r == half && (e > 0.f || (e == 0.f && odd)))) n += 1.f;
+    else if (r < -half || (r == -half && (e < 0.f || (e == 0.f && odd)))) n -= 1.f;
+    code |= (uint32_t)fminf(fmaxf(n, 0.f), 15.f) << (4 * i);
   }
-  const int lanes = a.group / 8;  // 2, 4 or 8 neighbouring threads hold a group
+  return code;
+}
+
+// Eight codes of bf16 rows whose values are 0 or at least 2^-16 of the range R.  Then x, m and s are
+// multiples of 2^-24 R: d = x - m is exact, and a quotient d / s that is not exactly halfway between
+// two codes is 2^-24 R / s > 2^-21 or more away, half a unit of the quotient's last place.  q' is the quotient rounded to fp32 (the residual
+// correction of Markstein, 1990), so adding 2^23
+// rounds it to the right code, ties to even.  Codes join by multiply-adds on the sums' bits.
+__device__ __forceinline__ uint32_t kv4_codes8(const float* x, float m, float s, float inv) {
+  uint32_t acc = 0;
 #pragma unroll
-  for (int o = 4; o > 0; o >>= 1) {
-    const float l2 = __shfl_xor_sync(0xffffffffu, lo, o), h2 = __shfl_xor_sync(0xffffffffu, hi, o);
-    const int b2 = __shfl_xor_sync(0xffffffffu, (int)bad, o);
-    if (o < lanes) {
-      lo = fminf(lo, l2);
-      hi = fmaxf(hi, h2);
-      bad |= b2 != 0;
+  for (int i = 7; i >= 0; --i) {
+    const float d = x[i] - m, q = d * inv, q1 = fmaf(fmaf(-q, s, d), inv, q);
+    acc = acc * 16u + __float_as_uint(q1 + 8388608.f);
+  }
+  return acc - 0xfb000000u;  // the sum of 0x4b000000 * 16^i, the bits of 2^23, modulo 2^32
+}
+
+template <int TYPE>
+__global__ void __launch_bounds__(kIoThreads) kv4_write_kernel(const Kv4IO a, const IoGrid g) {
+  const int b = blockIdx.y, r_in = threadIdx.x / g.pieces, piece = threadIdx.x - r_in * g.pieces;
+  const Kv4Cache& c = a.cache[blockIdx.z];
+  const Kv4Rows& src = a.rows[blockIdx.z];
+  const int lanes = a.group / kPiece;  // 1, 2 or 4 neighbouring threads hold a group
+  const uint32_t first = blockIdx.x * (uint32_t)(g.rows_per_pass * g.passes) + r_in;
+  const bool idle = r_in >= g.rows_per_pass;
+#pragma unroll 1
+  for (int k = 0; k < g.passes; ++k) {
+    const uint32_t r = first + k * g.rows_per_pass;
+    float x[kPiece] = {};
+    uint32_t bits[8] = {};
+    IoRow row;
+    row.row = -1;
+    if (!idle && r < g.total) {
+      row = io_row(a, g, r);
+      load_piece<TYPE>(src.x, b * src.x_b + row.t * src.x_t + row.h * src.x_h + piece * kPiece, x, bits);
     }
-  }
-  // m: exact for 16-bit rows whose type is bf16; the scale is taken from the rounded minimum
-  const bf16 mb = __float2bfloat16_rn(lo);
-  const float m = __bfloat162float(mb);
-  bf16 sb = __float2bfloat16_rn(__fdiv_rn(hi - m, 15.f));
-  float s = __bfloat162float(sb);
-  bad |= !(fabsf(m) <= 3.3895314e38f) || !(s <= 3.3895314e38f);
-  if (s < kMinScale) {
-    s = 0.f;
-    sb = __float2bfloat16_rn(0.f);
-  }
-  uint32_t code = 0;
-  if (!bad && s > 0.f) {
-    const float inv = 1.f / s;
+    float lo, hi, probe;  // probe: NaN behind a NaN or an infinity
+    if (TYPE == KV4_BF16) {
+      const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(bits);
+      const __nv_bfloat162 zero = __floats2bfloat162_rn(0.f, 0.f);
+      __nv_bfloat162 l = v[0], h = v[0], p = __hmul2(v[0], zero);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) code |= (uint32_t)kv4_code(x[i], m, s, inv) << (4 * i);
-  }
-  if (!ix.active || ix.row < 0 || ix.row >= a.L) return;
-  *reinterpret_cast<uint32_t*>(c.codes + b * c.c_b + ix.h * c.c_h + ix.row * (a.W / 2) + ix.piece * 4) = code;
-  if (ix.piece % lanes == 0) {
-    const uint32_t word = (uint32_t)__bfloat16_as_ushort(sb) | ((uint32_t)__bfloat16_as_ushort(mb) << 16);
-    *reinterpret_cast<uint32_t*>(c.params + b * c.p_b + ix.h * c.p_h + (ix.row * (a.W / a.group) + ix.piece / lanes) * 4) =
-        bad ? 0x7fc07fc0u : word;
+      for (int i = 1; i < 8; ++i) {
+        l = __hmin2(l, v[i]);
+        h = __hmax2(h, v[i]);
+        p = __hfma2(v[i], zero, p);
+      }
+      lo = fminf(__low2float(l), __high2float(l));
+      hi = fmaxf(__low2float(h), __high2float(h));
+      probe = __low2float(p) + __high2float(p);
+    } else {
+      lo = hi = x[0];
+      probe = 0.f;
+#pragma unroll
+      for (int i = 0; i < kPiece; ++i) {
+        lo = fminf(lo, x[i]);
+        hi = fmaxf(hi, x[i]);
+        probe = fmaf(x[i], 0.f, probe);
+      }
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      const float l2 = __shfl_xor_sync(0xffffffffu, lo, o), h2 = __shfl_xor_sync(0xffffffffu, hi, o);
+      const float p2 = __shfl_xor_sync(0xffffffffu, probe, o);
+      if (o < lanes) {
+        lo = fminf(lo, l2);
+        hi = fmaxf(hi, h2);
+        probe += p2;
+      }
+    }
+    // m is exact for bf16 rows; the scale is taken from the rounded minimum
+    const bf16 mb = __float2bfloat16_rn(lo);
+    const float m = __bfloat162float(mb);
+    const float range = hi - m;
+    bf16 sb = __float2bfloat16_rn(range * (1.f / 15.f));
+    float s = __bfloat162float(sb);
+    const bool bad = probe != 0.f || !(fabsf(m) <= 3.3895314e38f) || !(s <= 3.3895314e38f);
+    if (!(s >= kMinScale)) {
+      s = 0.f;
+      sb = __float2bfloat16_rn(0.f);
+    }
+    uint64_t code = 0;
+    if (!bad && s > 0.f) {
+      bool exact = TYPE != KV4_BF16;
+      if (TYPE == KV4_BF16) {
+        // the smallest |x| - 1 as bits; 0 becomes the largest
+        uint32_t least = 0xffffffffu;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) least = __viaddmin_u16x2(bits[i] & 0x7fff7fffu, 0xffffffffu, least);
+        const float smallest = __uint_as_float((min(least & 0xffffu, least >> 16) + 1u) << 16);
+        const float limit = range * 1.52587890625e-5f;
+        exact = smallest < limit || (m != 0.f && fabsf(m) < limit) || s < 1e-27f;
+      }
+      float inv;  // within 2^-23: candidates and residual corrections need no more
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+      if (exact) {
+        code = (uint64_t)kv4_codes8_exact(x, m, s, inv) | ((uint64_t)kv4_codes8_exact(x + 8, m, s, inv) << 32);
+      } else {
+        code = (uint64_t)kv4_codes8(x, m, s, inv) | ((uint64_t)kv4_codes8(x + 8, m, s, inv) << 32);
+      }
+    }
+    if (row.row < 0) continue;
+    *reinterpret_cast<uint64_t*>(c.codes + b * c.c_b + row.h * c.c_h + row.row * (a.W / 2) + piece * 8) = code;
+    if ((piece & (lanes - 1)) == 0) {
+      const uint32_t word = (uint32_t)__bfloat16_as_ushort(sb) | ((uint32_t)__bfloat16_as_ushort(mb) << 16);
+      *reinterpret_cast<uint32_t*>(c.params + b * c.p_b + row.h * c.p_h +
+                                   (row.row * (a.W / a.group) + piece / lanes) * 4) = bad ? 0x7fc07fc0u : word;
+    }
   }
 }
 
 template <int TYPE>
-__global__ void __launch_bounds__(kIoThreads) kv4_read_kernel(const Kv4IO a) {
-  const IoIndex ix = io_index(a);
-  if (!ix.active) return;
-  const int b = blockIdx.y;
+__global__ void __launch_bounds__(kIoThreads) kv4_read_kernel(const Kv4IO a, const IoGrid g) {
+  const int b = blockIdx.y, r_in = threadIdx.x / g.pieces, piece = threadIdx.x - r_in * g.pieces;
+  if (r_in >= g.rows_per_pass) return;
   const Kv4Cache& c = a.cache[blockIdx.z];
   const Kv4Rows& dst = a.rows[blockIdx.z];
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (ix.row >= 0 && ix.row < a.L) {
-    const uint32_t code =
-        *reinterpret_cast<const uint32_t*>(c.codes + b * c.c_b + ix.h * c.c_h + ix.row * (a.W / 2) + ix.piece * 4);
-    const uint32_t word = *reinterpret_cast<const uint32_t*>(
-        c.params + b * c.p_b + ix.h * c.p_h + (ix.row * (a.W / a.group) + ix.piece * 8 / a.group) * 4);
-    const float s = bf16_lo(word), m = bf16_hi(word);
+  const int lanes = a.group / kPiece;
+  const uint32_t first = blockIdx.x * (uint32_t)(g.rows_per_pass * g.passes) + r_in;
+  uint2 code[kPasses];
+  uint32_t word[kPasses];
+  IoRow row[kPasses];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = fmaf((float)((code >> (4 * i)) & 15u), s, m);
+  for (int k = 0; k < kPasses; ++k) {
+    const uint32_t r = first + k * g.rows_per_pass;
+    code[k] = make_uint2(0, 0);  // rows outside the cache read as zeros
+    word[k] = 0;
+    if (k < g.passes && r < g.total) {
+      row[k] = io_row(a, g, r);
+      if (row[k].row >= 0) {
+        code[k] = *reinterpret_cast<const uint2*>(c.codes + b * c.c_b + row[k].h * c.c_h + row[k].row * (a.W / 2) + piece * 8);
+        word[k] = *reinterpret_cast<const uint32_t*>(c.params + b * c.p_b + row[k].h * c.p_h +
+                                                     (row[k].row * (a.W / a.group) + piece / lanes) * 4);
+      }
+    }
   }
-  store8<TYPE>(dst.x, b * dst.x_b + ix.t * dst.x_t + ix.h * dst.x_h + ix.piece * 8, x);
+#pragma unroll
+  for (int k = 0; k < kPasses; ++k) {
+    if (k >= g.passes || first + k * g.rows_per_pass >= g.total) break;
+    const float s = bf16_lo(word[k]), m = bf16_hi(word[k]);
+    float x[kPiece];
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        // nibbles 2h and 4 + 2h as 1024 + n, 2h + 1 and 5 + 2h as 1024 + 16 n in fp16
+        const uint32_t u = (w ? code[k].y : code[k].x) >> (8 * h);
+        const uint32_t e = (u & 0x000f000fu) | 0x64006400u, o = (u & 0x00f000f0u) | 0x64006400u;
+        const __half2 ne = __hsub2(*reinterpret_cast<const __half2*>(&e), __float2half2_rn(1024.f));
+        const __half2 no = __hfma2(*reinterpret_cast<const __half2*>(&o), __float2half2_rn(0.0625f), __float2half2_rn(-64.f));
+        const float2 fe = __half22float2(ne), fo = __half22float2(no);
+        x[8 * w + 2 * h] = fmaf(fe.x, s, m);
+        x[8 * w + 2 * h + 4] = fmaf(fe.y, s, m);
+        x[8 * w + 2 * h + 1] = fmaf(fo.x, s, m);
+        x[8 * w + 2 * h + 5] = fmaf(fo.y, s, m);
+      }
+    store_piece<TYPE>(dst.x, b * dst.x_b + row[k].t * dst.x_t + row[k].h * dst.x_h + piece * kPiece, x);
+  }
 }
 
-dim3 io_grid(const Kv4IO& a) {
-  const long long n = (long long)a.T * a.Hk * (a.W / 8);
-  return dim3((unsigned)((n + kIoThreads - 1) / kIoThreads), (unsigned)a.B, (unsigned)a.count);
+// Enough blocks first, then several rows per thread.
+dim3 io_grid(const Kv4IO& a, IoGrid* g) {
+  g->pieces = a.W / kPiece;
+  g->rows_per_pass = kIoThreads / g->pieces;
+  g->total = (uint32_t)(a.T * a.Hk);
+  const long long blocks1 = (g->total + g->rows_per_pass - 1) / g->rows_per_pass;
+  g->passes = (int)std::min<long long>(kPasses, std::max<long long>(1, blocks1 * a.B * a.count / (148 * 4)));
+  g->shift_t = 0;  // n / T for n < 2^31: mul = ceil(2^(32 + shift) / T), shift = ceil(log2 T) - 1
+  while ((2ull << g->shift_t) < (unsigned long long)a.T) ++g->shift_t;
+  g->mul_t = a.T > 1 ? (uint32_t)(((1ull << (32 + g->shift_t)) + a.T - 1) / a.T) : 0;
+  const long long per_block = (long long)g->rows_per_pass * g->passes;
+  return dim3((unsigned)((g->total + per_block - 1) / per_block), (unsigned)a.B, (unsigned)a.count);
 }
 
 // ---------------------------------------------------------------------------
@@ -299,20 +398,23 @@ void launch_rows(const Kv4Attend& a, cudaStream_t s) {
 }  // namespace
 
 void kv4_write(const Kv4IO& a, cudaStream_t s) {
-  if (a.type == KV4_F32) kv4_write_kernel<KV4_F32><<<io_grid(a), kIoThreads, 0, s>>>(a);
-  else if (a.type == KV4_F16) kv4_write_kernel<KV4_F16><<<io_grid(a), kIoThreads, 0, s>>>(a);
-  else kv4_write_kernel<KV4_BF16><<<io_grid(a), kIoThreads, 0, s>>>(a);
+  IoGrid g;
+  const dim3 grid = io_grid(a, &g);
+  if (a.type == KV4_F32) kv4_write_kernel<KV4_F32><<<grid, kIoThreads, 0, s>>>(a, g);
+  else if (a.type == KV4_F16) kv4_write_kernel<KV4_F16><<<grid, kIoThreads, 0, s>>>(a, g);
+  else kv4_write_kernel<KV4_BF16><<<grid, kIoThreads, 0, s>>>(a, g);
 }
 
 void kv4_read(const Kv4IO& a, cudaStream_t s) {
-  if (a.type == KV4_F32) kv4_read_kernel<KV4_F32><<<io_grid(a), kIoThreads, 0, s>>>(a);
-  else if (a.type == KV4_F16) kv4_read_kernel<KV4_F16><<<io_grid(a), kIoThreads, 0, s>>>(a);
-  else kv4_read_kernel<KV4_BF16><<<io_grid(a), kIoThreads, 0, s>>>(a);
+  IoGrid g;
+  const dim3 grid = io_grid(a, &g);
+  if (a.type == KV4_F32) kv4_read_kernel<KV4_F32><<<grid, kIoThreads, 0, s>>>(a, g);
+  else if (a.type == KV4_F16) kv4_read_kernel<KV4_F16><<<grid, kIoThreads, 0, s>>>(a, g);
+  else kv4_read_kernel<KV4_BF16><<<grid, kIoThreads, 0, s>>>(a, g);
 }
 
 Kv4Plan kv4_plan(const Kv4Attend& a) {
   Kv4Plan p{};
-  p.splits = 1;
   if (a.v.codes != nullptr && a.group == 64 && (a.W == 64 || a.W == 128)) kv4_heads_plan(a, p);
   if (a.v.codes == nullptr && a.group == 64 && a.W == a.V + 64 && (a.V == 256 || a.V == 512)) kv4_latent_plan(a, p);
   return p;

@@ -53,7 +53,8 @@ struct Kv4Plan {
   int kernel;            // 0: one block per query row, 1: grouped heads, 2: latent
   int row_tiles;         // 8-row query tiles per block
   int row_blocks;        // blocks that share a key / value head's query rows
-  int splits;            // blocks that share the keys
+  int blocks;            // grid: blocks that share the key tiles of all of them
+  int min_steps;         // smallest share of a block, in steps of 128 keys; 0: a block per (sequence, head, rows)
   size_t floats;         // workspace
 };
 Kv4Plan kv4_plan(const Kv4Attend& a);

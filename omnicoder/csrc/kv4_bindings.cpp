@@ -162,7 +162,7 @@ at::Tensor kv4_attend_t(const at::Tensor& q_in, const at::Tensor& kc, const at::
               what, ": q_pos [B, Tn] and kv_len [B] on the cache's device");
   TORCH_CHECK(0 <= n_sink && n_sink <= sink_rows && sink_rows <= a.L && window >= 0, what,
               ": 0 <= n_sink <= sink_rows <= L, window >= 0");
-  TORCH_CHECK((int64_t)a.Tn * a.H < (1 << 24) && a.B <= 65535 && a.Hk <= 65535, what, ": too many query rows");
+  TORCH_CHECK((int64_t)a.B * a.Tn * a.H < (int64_t(1) << 31) && a.B <= 65535, what, ": too many query rows");
   a.q_pos = q_pos.data_ptr();
   a.kv_len = kv_len.data_ptr();
   a.window = (int)std::min<int64_t>(window, 1 << 30);

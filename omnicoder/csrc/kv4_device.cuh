@@ -54,6 +54,14 @@ __device__ __forceinline__ void mma_f16(float* d, uint32_t a0, uint32_t a1, uint
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// d = A B
+__device__ __forceinline__ void mma_f16_zero(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                             uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ void mma_bf16(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
   asm volatile(
@@ -68,12 +76,22 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
   return y;
 }
 
-// Nibble `mm` of both 16-bit halves as the bf16 pair (16 + n, 16 + n'): bits 3..6
-// of a bf16 mantissa at exponent 2^4 count in ones.
+// Nibble MM of both 16-bit halves as the bf16 pair (16 + n, 16 + n'): bits 3..6 of a
+// bf16 mantissa at exponent 2^4 count in ones.
 template <int MM>
 __device__ __forceinline__ uint32_t nibbles_bf16(uint32_t x) {
   const uint32_t y = MM == 0 ? x << 3 : x >> (MM == 0 ? 0 : 4 * MM - 3);
   return (y & 0x00780078u) | 0x41804180u;
+}
+
+// acc[nt] += value dims x keys (nibble MM: dims MM in the low, 4 + MM in the high halves of a
+// lane's eight) times the weights of row tile nt.
+template <int MM, int NT>
+__device__ __forceinline__ void mma_values(float (*acc)[4], uint32_t l0, uint32_t h0, uint32_t l8, uint32_t h8,
+                                           const uint32_t (*w)[2]) {
+  const uint32_t a0 = nibbles_bf16<MM>(l0), a1 = nibbles_bf16<MM>(h0), a2 = nibbles_bf16<MM>(l8), a3 = nibbles_bf16<MM>(h8);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) mma_bf16(acc[nt], a0, a1, a2, a3, w[nt][0], w[nt][1]);
 }
 
 __device__ __forceinline__ void kv4_cp16(uint32_t dst, const void* src) {
@@ -89,6 +107,12 @@ __device__ __forceinline__ uint2 lds64(uint32_t addr) {
   uint2 v;
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
   return v;
+}
+__device__ __forceinline__ void lds128(uint32_t addr, float* v) {
+  asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(addr));
+}
+__device__ __forceinline__ void sts128(uint32_t addr, const float* v) {
+  asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]) : "memory");
 }
 __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
   uint32_t v;
@@ -106,8 +130,142 @@ __device__ __forceinline__ float q_normaliser(float amax, float* unscale) {
   return __uint_as_float((268u - e) << 23);     // 2^(14 - (e - 127))
 }
 
-// Workspace of the splits: rows [B, Hk, R, splits] of V sums, then (max, sum) pairs.
-void kv4_combine(const Kv4Attend& a, int splits, cudaStream_t s);
+// ---- work of the blocks ---------------------------------------------------------
+// A segment is (sequence, key / value head, row block): its keys are walked in
+// steps of 128 rows.  Few short segments: a block each.  Otherwise the steps of
+// all segments form one line that the blocks share in equal consecutive pieces,
+// so that uneven lengths and segment counts that do not fill the GPU cost
+// nothing.  A block then holds at most two pieces that it shares with others,
+// the first (of a segment begun by an earlier block) and the last; those go to
+// slots 2 * block and 2 * block + 1 of the workspace, and the block that begins a
+// segment notes its first and last block for the kernel that joins them.
+constexpr int kKv4Step = 128;
+
+struct Kv4Line {
+  int segments;    // of one sequence: Hk * row_blocks
+  int tile;        // rows per tile: 32 (four warps a step) or 128
+  int min_steps;   // smallest share of a block; 0: a block per segment
+  int2* meta;      // [B * segments] first and last block
+};
+
+struct Kv4Piece {
+  int b, segment;                  // sequence, segment of it
+  long long begin;                 // its first step on the line
+  int steps;
+  int sink_tiles, first, tiles;    // tiles over the memory rows; first tile behind them; all
+};
+
+// Rows [lo, hi) that any of the queries t0, t0 + stride, .. < t1 sees.
+__device__ __forceinline__ Kv4Seen kv4_union(const Kv4Attend& a, int b, int t0, int t1, int stride) {
+  Kv4Seen u{a.L, 0};
+  for (int t = t0; t < t1; t += stride) {
+    const Kv4Seen s = kv4_seen(a, b, t);
+    if (s.hi > s.lo) {
+      u.lo = min(u.lo, s.lo);
+      u.hi = max(u.hi, s.hi);
+    }
+  }
+  return u;
+}
+
+__device__ __forceinline__ void kv4_tiles(const Kv4Attend& a, Kv4Seen u, int tile, Kv4Piece* p) {
+  p->sink_tiles = (a.n_sink + tile - 1) / tile;
+  p->first = max(u.lo / tile, p->sink_tiles);
+  p->tiles = p->sink_tiles + max(0, u.hi > u.lo ? (u.hi + tile - 1) / tile - p->first : 0);
+  const int per_step = kKv4Step / tile;
+  p->steps = max(1, (p->tiles + per_step - 1) / per_step);  // a sequence that sees nothing still writes zeros
+}
+
+// Whole warps: the segment that holds step `at` of the line, and the line's length.
+__device__ __forceinline__ Kv4Piece kv4_locate(const Kv4Attend& a, const Kv4Line& l, long long at, long long* total) {
+  Kv4Piece p{-1, 0, 0, 1, 0, 0, 0};
+  const int lane = lane_id();
+  long long base = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 32) {
+    Kv4Piece q{0, 0, 0, 0, 0, 0, 0};
+    if (b0 + lane < a.B) kv4_tiles(a, kv4_union(a, b0 + lane, 0, a.Tn, 1), l.tile, &q);
+    long long sum = q.steps;  // inclusive prefix of the sequences' steps
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
+    }
+    const long long end = base + sum * l.segments;
+    const uint32_t above = __ballot_sync(0xffffffffu, end > at);
+    if (p.b < 0 && above != 0) {
+      const int src = __ffs(above) - 1;
+      p.b = b0 + src;
+      p.steps = __shfl_sync(0xffffffffu, q.steps, src);
+      p.sink_tiles = __shfl_sync(0xffffffffu, q.sink_tiles, src);
+      p.first = __shfl_sync(0xffffffffu, q.first, src);
+      p.tiles = __shfl_sync(0xffffffffu, q.tiles, src);
+      const long long start = __shfl_sync(0xffffffffu, end, src) - (long long)p.steps * l.segments;
+      p.segment = (int)((at - start) / p.steps);
+      p.begin = start + (long long)p.segment * p.steps;
+    }
+    base = __shfl_sync(0xffffffffu, end, 31);
+  }
+  *total = base;
+  return p;
+}
+
+// The pieces of one block, in turn.
+struct Kv4Walk {
+  long long at, end;
+  int share;
+
+  __device__ __forceinline__ void begin(const Kv4Attend& a, const Kv4Line& l) {
+    if (l.min_steps == 0) {
+      at = 0;
+      end = 1;
+      share = 0;
+      return;
+    }
+    long long total;
+    kv4_locate(a, l, 0, &total);
+    share = max((int)((total + gridDim.x - 1) / gridDim.x), l.min_steps);
+    at = (long long)blockIdx.x * share;
+    end = min(total, at + share);
+  }
+  // Whole warps; rows_per_block query rows of a segment.  step0 .. step1: this block's steps of it.
+  __device__ __forceinline__ Kv4Piece next(const Kv4Attend& a, const Kv4Line& l, int rows_per_block, int* step0, int* step1) {
+    Kv4Piece p;
+    if (l.min_steps == 0) {
+      p.b = blockIdx.x / l.segments;
+      p.segment = blockIdx.x % l.segments;
+      p.begin = 0;
+      const int G = a.H / a.Hk, row0 = p.segment % (l.segments / a.Hk) * rows_per_block;
+      const int t0 = row0 / G, t1 = (min(row0 + rows_per_block, a.Tn * G) - 1) / G + 1;
+      Kv4Seen u = kv4_union(a, p.b, t0 + lane_id(), t1, 32);
+      u.lo = __reduce_min_sync(0xffffffffu, u.lo);
+      u.hi = __reduce_max_sync(0xffffffffu, u.hi);
+      kv4_tiles(a, u, l.tile, &p);
+      *step0 = 0;
+      *step1 = p.steps;
+      at = end;
+    } else {
+      long long total;
+      p = kv4_locate(a, l, at, &total);
+      *step0 = (int)(at - p.begin);
+      *step1 = (int)min((long long)p.steps, end - p.begin);
+      if (at == p.begin && threadIdx.x == 0)
+        l.meta[p.b * l.segments + p.segment] =
+            make_int2(blockIdx.x, (int)((p.begin + p.steps - 1) / share));
+      at = p.begin + p.steps;
+    }
+    return p;
+  }
+};
+
+// The kernel that joins the pieces may start its blocks early; they wait for this one's end.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous_grid() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Grid and workspace: slots blocks stay resident, shares of at least min_steps.
+void kv4_line_plan(const Kv4Attend& a, Kv4Plan& p, int slots, int min_steps);
+Kv4Line kv4_line(const Kv4Attend& a, const Kv4Plan& p, int tile);
+// Joins the pieces: 8 * row_tiles rows of V sums and then (max, sum) pairs per slot.
+void kv4_combine(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s);
 void kv4_heads_launch(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s);
 void kv4_heads_plan(const Kv4Attend& a, Kv4Plan& p);
 void kv4_latent_launch(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s);

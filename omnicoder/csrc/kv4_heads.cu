@@ -39,7 +39,7 @@ constexpr float kSlack = 8.f;   // log2 units a score may exceed the running max
 template <int D, int NT>
 struct HeadsCfg {
   static constexpr int NG = D / 64;
-  static constexpr int kStages = 3;
+  static constexpr int kStages = NT == 1 ? 3 : 3;
   static constexpr int kRow = D / 2;
   static constexpr int kCodes = kTile * kRow;
   static constexpr int kParams = kTile * NG * 4;
@@ -51,8 +51,15 @@ struct HeadsCfg {
   static constexpr int kSmem = kQ + kRows * D * 2 + kRows * (NG + 1) * 4;
 };
 
+__device__ __forceinline__ void load_params(uint32_t at, uint32_t (&p)[1]) { p[0] = lds32(at); }
+__device__ __forceinline__ void load_params(uint32_t at, uint32_t (&p)[2]) {
+  const uint2 v = lds64(at);
+  p[0] = v.x;
+  p[1] = v.y;
+}
+
 template <int D, int NT, int TYPE>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel(const Kv4Attend a, const int splits) {
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel(const Kv4Attend a, const Kv4Line line) {
   using C = HeadsCfg<D, NT>;
   constexpr int NG = C::NG;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -60,29 +67,31 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
   float* sqs = reinterpret_cast<float*>(smem + C::kQ + C::kRows * D * 2);   // [kRows][NG]: sum(q_g) 2^-24
   float* srs = sqs + C::kRows * NG;                                         // [kRows]: factor of the scores
   const int lane = lane_id(), warp = warp_id(), i = lane >> 2, j = lane & 3;
-  const int split = blockIdx.x % splits, row0 = (blockIdx.x / splits) * C::kRows, hk = blockIdx.y, b = blockIdx.z;
-  const int G = a.H / a.Hk, R = a.Tn * G, nrows = min(C::kRows, R - row0);
+  const int G = a.H / a.Hk, R = a.Tn * G, row_blocks = line.segments / a.Hk;
+  const uint32_t ring = smem_u32(smem) + warp * C::kStages * C::kStage;
+  if (line.min_steps > 0) launch_dependents();
+  Kv4Walk walk;
+  walk.begin(a, line);
+
+  while (walk.at < walk.end) {
+  int step0, step1;
+  const Kv4Piece piece = walk.next(a, line, C::kRows, &step0, &step1);
+  const int b = piece.b, hk = piece.segment / row_blocks, row0 = (piece.segment % row_blocks) * C::kRows;
+  const int nrows = min(C::kRows, R - row0);
+  const int sink_tiles = piece.sink_tiles, first = piece.first;
+  const int t0 = step0 * kWarps, t1 = min(piece.tiles, step1 * kWarps);
 
   // ---- the rows each query sees; lane r holds query row r --------------------
   Kv4Seen seen{0, 0};
   if (lane < nrows) seen = kv4_seen(a, b, (row0 + lane) / G);
-  const int lo_min = __reduce_min_sync(0xffffffffu, lane < nrows ? seen.lo : a.L);
-  const int hi_max = __reduce_max_sync(0xffffffffu, lane < nrows ? seen.hi : 0);
   const int lo_max = __reduce_max_sync(0xffffffffu, lane < nrows ? seen.lo : 0);
   const int hi_min = __reduce_min_sync(0xffffffffu, lane < nrows ? seen.hi : a.L);
-  const int sink_tiles = (a.n_sink + kTile - 1) / kTile;
-  const int first = max(lo_min / kTile, sink_tiles);
-  const int tiles = sink_tiles + max(0, hi_max > lo_min ? (hi_max + kTile - 1) / kTile - first : 0);
-  const int per = (tiles + splits - 1) / splits;
-  const int t0 = split * per, t1 = min(tiles, t0 + per);
   auto row_of = [&](int tile) { return (tile < sink_tiles ? tile : first + tile - sink_tiles) * kTile; };
 
   const uint8_t* kc = a.k.codes + b * a.k.c_b + hk * a.k.c_h;
   const uint8_t* vc = a.v.codes + b * a.v.c_b + hk * a.v.c_h;
   const uint8_t* kp = a.k.params + b * a.k.p_b + hk * a.k.p_h;
   const uint8_t* vp = a.v.params + b * a.v.p_b + hk * a.v.p_h;
-  const uint32_t ring = smem_u32(smem) + warp * C::kStages * C::kStage;
-
   // A tile is contiguous in memory.  In shared memory row t lies at t ^ bit2(t), and rows of 64
   // bytes have their halves swapped where bit1(t) is set: the 8 (scores) and 4 (output) rows that
   // one load touches then fall into different banks.
@@ -166,27 +175,32 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
     }
   }
 
-  float acc[NG][4][NT][4], accr[NG][NT][4], accm[NG][NT][2], lsum[NT][2], mx[NT][2];
+  float acc[NG][4][NT][4], accr[NT][4], accm[NG][NT][2], lsum[NT][2];
+  float limit[NT][2], ref[NT][2];  // running maximum + slack, running maximum (0 before any key)
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        accr[g][nt][c] = 0.f;
+      for (int c = 0; c < 4; ++c)
 #pragma unroll
         for (int mm = 0; mm < 4; ++mm) acc[g][mm][nt][c] = 0.f;
-      }
       accm[g][nt][0] = accm[g][nt][1] = 0.f;
     }
+    accr[nt][0] = accr[nt][1] = accr[nt][2] = accr[nt][3] = 0.f;
     lsum[nt][0] = lsum[nt][1] = 0.f;
-    mx[nt][0] = mx[nt][1] = -INFINITY;
+    limit[nt][0] = limit[nt][1] = -INFINITY;
+    ref[nt][0] = ref[nt][1] = 0.f;
   }
 
-  const uint32_t k_at = (i ^ ((i >> 2) & 1)) * C::kRow + j * 8, k_swap = D == 128 ? ((i >> 1) & 1) * 32 : 0;
-  const uint32_t v_at0 = C::kCodes + ((2 * j) ^ ((j >> 1) & 1)) * C::kRow + i * 4;
-  const uint32_t v_at1 = C::kCodes + ((2 * j + 1) ^ ((j >> 1) & 1)) * C::kRow + i * 4;
-  const uint32_t v_swap = D == 128 ? (j & 1) * 32 : 0;
+  uint32_t k_at[NG], v_at0[NG], v_at1[NG];
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    k_at[g] = (i ^ ((i >> 2) & 1)) * C::kRow + j * 8 + ((g ^ (D == 128 ? (i >> 1) & 1 : 0)) * 32);
+    const uint32_t at = C::kCodes + i * 4 + (g ^ (D == 128 ? j & 1 : 0)) * 32;
+    v_at0[g] = at + ((2 * j) ^ ((j >> 1) & 1)) * C::kRow;
+    v_at1[g] = at + ((2 * j + 1) ^ ((j >> 1) & 1)) * C::kRow;
+  }
 
   int stage = 0;
   for (int tile = t0 + warp; tile < t1; tile += kWarps, next += kWarps) {
@@ -194,146 +208,134 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
     __syncwarp();  // every lane's pieces have landed, and every lane has left the stage refilled below
     if (next < t1) issue(next, stage == 0 ? C::kStages - 1 : stage - 1);
     kv4_cp_commit();
-    const uint32_t st = ring + stage * C::kStage;
-    const uint32_t sp = st + 2 * C::kCodes;
     const int r0 = row_of(tile);
-
-    // ---- scores, in units of log2 ---------------------------------------------
-    float s[2][NT][4];
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) s[mt][nt][c] = 0.f;
+    const bool masked = !(r0 + kTile <= a.n_sink || (r0 >= lo_max && r0 + kTile <= hi_min));
+    uint32_t st = ring + stage * C::kStage, sp = st + 2 * C::kCodes + i * NG * 4;
+    // Rolled: the loop's code must stay in the instruction cache next to the scheduler.
+#pragma unroll 1
+    for (int r = r0 + i; r < r0 + kTile; r += 16, st += 16 * C::kRow, sp += 16 * NG * 4) {
+      // ---- scores of 16 keys (this lane: keys r and r + 8), in units of log2 ------------
+      uint32_t pa[NG], pb[NG];
+      load_params(sp, pa);
+      load_params(sp + 8 * NG * 4, pb);
+      float s[NT][4];
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        const uint2 wa = lds64(st + mt * 16 * C::kRow + k_at + ((g * 32) ^ k_swap));
-        const uint2 wb = lds64(st + (mt * 16 + 8) * C::kRow + k_at + ((g * 32) ^ k_swap));
-        const uint32_t pa = lds32(sp + ((mt * 16 + i) * NG + g) * 4), pb = lds32(sp + ((mt * 16 + i + 8) * NG + g) * 4);
+        const uint2 wa = lds64(st + k_at[g]), wb = lds64(st + k_at[g] + 8 * C::kRow);
         float d[NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) d[nt][c] = 0.f;
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
           const uint32_t xa = (ks < 2 ? wa.x : wa.y) >> ((ks & 1) * 8), xb = (ks < 2 ? wb.x : wb.y) >> ((ks & 1) * 8);
+          const uint32_t a0 = xa & 0x000f000fu, a1 = xb & 0x000f000fu, a2 = xa & 0x00f000f0u, a3 = xb & 0x00f000f0u;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            mma_f16(d[nt], xa & 0x000f000fu, xb & 0x000f000fu, xa & 0x00f000f0u, xb & 0x00f000f0u, qf[g][ks][nt][0],
-                    qf[g][ks][nt][1]);
+          for (int nt = 0; nt < NT; ++nt) {
+            if (ks == 0) mma_f16_zero(d[nt], a0, a1, a2, a3, qf[g][ks][nt][0], qf[g][ks][nt][1]);
+            else mma_f16(d[nt], a0, a1, a2, a3, qf[g][ks][nt][0], qf[g][ks][nt][1]);
+          }
         }
-        const float sa = bf16_lo(pa), ma = bf16_hi(pa), sb = bf16_lo(pb), mb = bf16_hi(pb);
+        const float sa = bf16_lo(pa[g]), ma = bf16_hi(pa[g]), sb = bf16_lo(pb[g]), mb = bf16_hi(pb[g]);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          s[mt][nt][0] = fmaf(d[nt][0], sa, fmaf(qs[g][nt][0], ma, s[mt][nt][0]));
-          s[mt][nt][1] = fmaf(d[nt][1], sa, fmaf(qs[g][nt][1], ma, s[mt][nt][1]));
-          s[mt][nt][2] = fmaf(d[nt][2], sb, fmaf(qs[g][nt][0], mb, s[mt][nt][2]));
-          s[mt][nt][3] = fmaf(d[nt][3], sb, fmaf(qs[g][nt][1], mb, s[mt][nt][3]));
-        }
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const float m = qs[g][nt][c & 1] * (c < 2 ? ma : mb);
+            s[nt][c] = fmaf(d[nt][c], c < 2 ? sa : sb, g == 0 ? m : m + s[nt][c]);
+          }
       }
-    }
-    const bool masked = !(r0 + kTile <= a.n_sink || (r0 >= lo_max && r0 + kTile <= hi_min));
-    bool above = false;
-    float top[NT][2];
+      bool above = false;
+      float top[NT][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
+        for (int c = 0; c < 4; ++c) s[nt][c] *= rs[nt][c & 1];
+      if (masked) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int r = r0 + mt * 16 + i + (c >> 1) * 8;
-          s[mt][nt][c] *= rs[nt][c & 1];
-          if (masked && !(r < a.n_sink || (r >= lo[nt][c & 1] && r < hi[nt][c & 1]))) s[mt][nt][c] = -INFINITY;
-        }
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        top[nt][c] = fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]), fmaxf(s[1][nt][c], s[1][nt][c + 2]));
-        above |= top[nt][c] > mx[nt][c] + kSlack;
+          for (int c = 0; c < 4; ++c) {
+            const int key = r + (c >> 1) * 8;
+            if (!(key < a.n_sink || (key >= lo[nt][c & 1] && key < hi[nt][c & 1]))) s[nt][c] = -INFINITY;
+          }
       }
-    }
-    if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float x = fmaxf(top[nt][c], mx[nt][c]);
+          top[nt][c] = fmaxf(s[nt][c], s[nt][c + 2]);
+          above |= top[nt][c] > limit[nt][c];
+        }
+      if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
-          for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-          const float alpha = x == -INFINITY ? 1.f : fast_exp2(mx[nt][c] - x);
-          mx[nt][c] = x;
-          lsum[nt][c] *= alpha;
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            accm[g][nt][c] *= alpha;
-            accr[g][nt][c] *= alpha;
+          for (int c = 0; c < 2; ++c) {
+            const float old = limit[nt][c] - kSlack;
+            float x = fmaxf(top[nt][c], old);
 #pragma unroll
-            for (int mm = 0; mm < 4; ++mm) {
-              acc[g][mm][nt][c] *= alpha;
-              acc[g][mm][nt][c + 2] *= alpha;
+            for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+            limit[nt][c] = x + kSlack;
+            // what was summed is in units of 2^ref, whatever limit - kSlack rounds to
+            const float now = x == -INFINITY ? 0.f : x;
+            const float alpha = old == -INFINITY ? 0.f : fast_exp2(ref[nt][c] - now);
+            ref[nt][c] = now;
+            lsum[nt][c] *= alpha;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+              accm[g][nt][c] *= alpha;
+              accr[nt][c + 2 * g] *= alpha;
+#pragma unroll
+              for (int mm = 0; mm < 4; ++mm) {
+                acc[g][mm][nt][c] *= alpha;
+                acc[g][mm][nt][c + 2] *= alpha;
+              }
             }
           }
-        }
-    }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const float ref = mx[nt][c] == -INFINITY ? 0.f : mx[nt][c];
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          s[mt][nt][c] = fast_exp2(s[mt][nt][c] - ref);
-          s[mt][nt][c + 2] = fast_exp2(s[mt][nt][c + 2] - ref);
-          lsum[nt][c] += s[mt][nt][c] + s[mt][nt][c + 2];
-        }
       }
-
-    // ---- output -----------------------------------------------------------------
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          s[nt][c] = fast_exp2(s[nt][c] - ref[nt][c]);
+          s[nt][c + 2] = fast_exp2(s[nt][c + 2] - ref[nt][c]);
+          lsum[nt][c] += s[nt][c] + s[nt][c + 2];
+        }
+
+      // ---- output -----------------------------------------------------------------
+      load_params(sp + C::kParams, pa);
+      load_params(sp + C::kParams + 8 * NG * 4, pb);
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        const uint32_t pa = lds32(sp + C::kParams + ((mt * 16 + i) * NG + g) * 4);
-        const uint32_t pb = lds32(sp + C::kParams + ((mt * 16 + i + 8) * NG + g) * 4);
-        const float sa = bf16_lo(pa), sb = bf16_lo(pb);
-        const float ca = fmaf(8.f, sa, bf16_hi(pa)), cb = fmaf(8.f, sb, bf16_hi(pb));
+        const float sa = bf16_lo(pa[g]), sb = bf16_lo(pb[g]);
+        const float ca = fmaf(8.f, sa, bf16_hi(pa[g])), cb = fmaf(8.f, sb, bf16_hi(pb[g]));
         uint32_t bw[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const float* p = s[mt][nt];
-          float x0 = p[0] * sa, x1 = p[1] * sa, x2 = p[2] * sb, x3 = p[3] * sb;
+          float x[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) x[c] = s[nt][c] * (c < 2 ? sa : sb);
           if (masked) {  // a key that a row does not see may hold anything
-            x0 = p[0] == 0.f ? 0.f : x0;
-            x1 = p[1] == 0.f ? 0.f : x1;
-            x2 = p[2] == 0.f ? 0.f : x2;
-            x3 = p[3] == 0.f ? 0.f : x3;
-            accm[g][nt][0] += (p[0] == 0.f ? 0.f : p[0] * ca) + (p[2] == 0.f ? 0.f : p[2] * cb);
-            accm[g][nt][1] += (p[1] == 0.f ? 0.f : p[1] * ca) + (p[3] == 0.f ? 0.f : p[3] * cb);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              if (s[nt][c] == 0.f) x[c] = 0.f;
+              else accm[g][nt][c & 1] = fmaf(s[nt][c], c < 2 ? ca : cb, accm[g][nt][c & 1]);
+            }
           } else {
-            accm[g][nt][0] = fmaf(p[0], ca, fmaf(p[2], cb, accm[g][nt][0]));
-            accm[g][nt][1] = fmaf(p[1], ca, fmaf(p[3], cb, accm[g][nt][1]));
+#pragma unroll
+            for (int c = 0; c < 4; ++c) accm[g][nt][c & 1] = fmaf(s[nt][c], c < 2 ? ca : cb, accm[g][nt][c & 1]);
           }
-          bw[nt][0] = movmatrix_trans(pack_bf16x2(x0, x1));
-          bw[nt][1] = movmatrix_trans(pack_bf16x2(x2, x3));
-          mma_bf16(accr[g][nt], 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, bw[nt][0], bw[nt][1]);
+          bw[nt][0] = movmatrix_trans(pack_bf16x2(x[0], x[1]));
+          bw[nt][1] = movmatrix_trans(pack_bf16x2(x[2], x[3]));
+          mma_bf16(accr[nt], g == 0 ? 0x3f803f80u : 0u, g == 1 ? 0x3f803f80u : 0u, g == 0 ? 0x3f803f80u : 0u,
+                   g == 1 ? 0x3f803f80u : 0u, bw[nt][0], bw[nt][1]);
         }
-        const uint32_t at = st + mt * 16 * C::kRow + ((g * 32) ^ v_swap);
-        const uint32_t w0 = lds32(at + v_at0), w1 = lds32(at + v_at1);
-        const uint32_t w8 = lds32(at + v_at0 + 8 * C::kRow), w9 = lds32(at + v_at1 + 8 * C::kRow);
+        const uint32_t w0 = lds32(st + v_at0[g]), w1 = lds32(st + v_at1[g]);
+        const uint32_t w8 = lds32(st + v_at0[g] + 8 * C::kRow), w9 = lds32(st + v_at1[g] + 8 * C::kRow);
         const uint32_t l0 = __byte_perm(w0, w1, 0x5410), h0 = __byte_perm(w0, w1, 0x7632);
         const uint32_t l8 = __byte_perm(w8, w9, 0x5410), h8 = __byte_perm(w8, w9, 0x7632);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          mma_bf16(acc[g][0][nt], nibbles_bf16<0>(l0), nibbles_bf16<0>(h0), nibbles_bf16<0>(l8), nibbles_bf16<0>(h8),
-                   bw[nt][0], bw[nt][1]);
-          mma_bf16(acc[g][1][nt], nibbles_bf16<1>(l0), nibbles_bf16<1>(h0), nibbles_bf16<1>(l8), nibbles_bf16<1>(h8),
-                   bw[nt][0], bw[nt][1]);
-          mma_bf16(acc[g][2][nt], nibbles_bf16<2>(l0), nibbles_bf16<2>(h0), nibbles_bf16<2>(l8), nibbles_bf16<2>(h8),
-                   bw[nt][0], bw[nt][1]);
-          mma_bf16(acc[g][3][nt], nibbles_bf16<3>(l0), nibbles_bf16<3>(h0), nibbles_bf16<3>(l8), nibbles_bf16<3>(h8),
-                   bw[nt][0], bw[nt][1]);
-        }
+        mma_values<0, NT>(acc[g][0], l0, h0, l8, h8, bw);
+        mma_values<1, NT>(acc[g][1], l0, h0, l8, h8, bw);
+        mma_values<2, NT>(acc[g][2], l0, h0, l8, h8, bw);
+        mma_values<3, NT>(acc[g][3], l0, h0, l8, h8, bw);
       }
     }
     stage = stage + 1 == C::kStages ? 0 : stage + 1;
@@ -353,7 +355,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
       if (i == 0) {
-        sml[2 * r] = mx[nt][c];
+        sml[2 * r] = limit[nt][c] == -INFINITY ? -INFINITY : ref[nt][c];
         sml[2 * r + 1] = l;
       }
 #pragma unroll
@@ -361,7 +363,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
         float m = accm[g][nt][c];
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
-        m = fmaf(-24.f, accr[g][nt][c], m);
+        m = fmaf(-24.f, accr[nt][c + 2 * g], m);
         float* o = so + r * D + g * 64 + 8 * i;
 #pragma unroll
         for (int mm = 0; mm < 4; ++mm) {
@@ -371,7 +373,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
       }
     }
   __syncthreads();
-  float* pml = a.part + (size_t)a.B * a.Tn * a.H * splits * D;
+  // a segment that this block holds alone is finished; otherwise its piece goes to a slot
+  const bool alone = step0 == 0 && step1 == piece.steps;
+  float* part = a.part + (size_t)(2 * blockIdx.x + (step0 == 0)) * C::kRows * (D + 2);
   for (int idx = threadIdx.x; idx < nrows * (D / 2); idx += kWarps * 32) {
     const int r = idx / (D / 2), d = (idx % (D / 2)) * 2;
     float top = -INFINITY, l = 0.f, x = 0.f, y = 0.f;
@@ -386,16 +390,17 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
       x = fmaf(f, so[at * D + d], x);
       y = fmaf(f, so[at * D + d + 1], y);
     }
-    const int row = row0 + r;
-    const long long head = ((long long)b * a.Tn + row / G) * a.H + hk * G + row % G;
-    if (splits == 1) {
+    if (alone) {
+      const int row = row0 + r;
+      const long long head = ((long long)b * a.Tn + row / G) * a.H + hk * G + row % G;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       reinterpret_cast<uint32_t*>(a.out)[(head * D + d) / 2] = kv4_pack2<TYPE>(x * inv, y * inv);
     } else {
-      const long long at = head * splits + split;
-      *reinterpret_cast<float2*>(a.part + at * D + d) = make_float2(x, y);
-      if (d == 0) *reinterpret_cast<float2*>(pml + at * 2) = make_float2(top, l);
+      *reinterpret_cast<float2*>(part + r * D + d) = make_float2(x, y);
+      if (d == 0) *reinterpret_cast<float2*>(part + C::kRows * D + 2 * r) = make_float2(top, l);
     }
+  }
+  __syncthreads();  // the next segment refills shared memory
   }
 }
 
@@ -404,7 +409,7 @@ void launch(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s) {
   auto kern = kv4_heads_kernel<D, NT, TYPE>;
   constexpr int smem = HeadsCfg<D, NT>::kSmem;
   ensure_smem_attr(reinterpret_cast<const void*>(kern), smem);
-  kern<<<dim3((unsigned)(p.splits * p.row_blocks), (unsigned)a.Hk, (unsigned)a.B), kWarps * 32, smem, s>>>(a, p.splits);
+  kern<<<p.blocks, kWarps * 32, smem, s>>>(a, kv4_line(a, p, kTile));
 }
 
 template <int TYPE>
@@ -415,63 +420,20 @@ void launch_dims(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s) {
     p.row_tiles == 1 ? launch<64, 1, TYPE>(a, p, s) : launch<64, 2, TYPE>(a, p, s);
 }
 
-// One output row (sequence, token, head) per block: join its splits.
-template <int TYPE>
-__global__ void kv4_combine_kernel(const Kv4Attend a, const int splits) {
-  const long long row = blockIdx.x;
-  const float* pml = a.part + (size_t)a.B * a.Tn * a.H * splits * a.V + row * splits * 2;
-  float top = -INFINITY;
-  for (int k = 0; k < splits; ++k) top = fmaxf(top, pml[2 * k]);
-  const float ref = top == -INFINITY ? 0.f : top;
-  const int d = threadIdx.x * 2;
-  float l = 0.f, x = 0.f, y = 0.f;
-  for (int k = 0; k < splits; ++k) {
-    const float f = fast_exp2(pml[2 * k] - ref);
-    const float2 v = *reinterpret_cast<const float2*>(a.part + (row * splits + k) * a.V + d);
-    l = fmaf(f, pml[2 * k + 1], l);
-    x = fmaf(f, v.x, x);
-    y = fmaf(f, v.y, y);
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  reinterpret_cast<uint32_t*>(a.out)[(row * a.V + d) / 2] = kv4_pack2<TYPE>(x * inv, y * inv);
-}
-
 }  // namespace
-
-void kv4_combine(const Kv4Attend& a, int splits, cudaStream_t s) {
-  const unsigned rows = (unsigned)((long long)a.B * a.Tn * a.H);
-  if (a.type == KV4_F16) kv4_combine_kernel<KV4_F16><<<rows, a.V / 2, 0, s>>>(a, splits);
-  else kv4_combine_kernel<KV4_BF16><<<rows, a.V / 2, 0, s>>>(a, splits);
-}
 
 void kv4_heads_plan(const Kv4Attend& a, Kv4Plan& p) {
   const int R = a.Tn * (a.H / a.Hk);
   p.kernel = 1;
   p.row_tiles = R <= 8 ? 1 : 2;
   p.row_blocks = (R + 8 * p.row_tiles - 1) / (8 * p.row_tiles);
-  // The host knows the cache's size, not the sequences' lengths: plan for a full cache (or window).
-  // Cost of a split count: waves of blocks times the tiles a warp walks, plus about four tiles' time
-  // to start and to join a block.
-  const long long rows = std::min<long long>(a.L - a.sink_rows, a.window > 0 ? a.window + a.Tn : 1 << 30);
-  const int tiles = (a.n_sink + kTile - 1) / kTile + (int)((rows + kTile - 1) / kTile) + 1;
-  const long long blocks = (long long)a.B * a.Hk * p.row_blocks, slots = 148 * (p.row_tiles == 1 ? 3 : 2);
-  long long best = -1;
-  for (int sp = 1; sp <= 64 && (sp == 1 || tiles >= sp * kWarps); ++sp) {
-    const long long waves = (blocks * sp + slots - 1) / slots;
-    const long long per_warp = ((tiles + sp - 1) / sp + kWarps - 1) / kWarps;
-    const long long cost = waves * (per_warp + 4) + (sp > 1 ? 6 : 0);
-    if (best < 0 || cost < best) {
-      best = cost;
-      p.splits = sp;
-    }
-  }
-  p.floats = p.splits > 1 ? (size_t)a.B * a.Tn * a.H * p.splits * (a.V + 2) : 0;
+  kv4_line_plan(a, p, 148 * (p.row_tiles == 1 ? 3 : 2), 1);
 }
 
 void kv4_heads_launch(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s) {
   if (a.type == KV4_F16) launch_dims<KV4_F16>(a, p, s);
   else launch_dims<KV4_BF16>(a, p, s);
-  if (p.splits > 1) kv4_combine(a, p.splits, s);
+  if (p.min_steps > 0) kv4_combine(a, p, s);
 }
 
 }  // namespace omni

@@ -46,7 +46,7 @@ struct LatentCfg {
 };
 
 template <int V, int TYPE>
-__global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Attend a, const int splits, StatusBlock* st) {
+__global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Attend a, const Kv4Line line, StatusBlock* st) {
   using C = LatentCfg<V>;
   constexpr int W = C::W, NG = C::NG, VG = C::VG;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -60,20 +60,26 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
   int* shi = slo + kRows;
   uint64_t* full = reinterpret_cast<uint64_t*>(shi + kRows);
   const int tid = threadIdx.x, lane = lane_id(), warp = warp_id(), i = lane >> 2, j = lane & 3;
-  const int split = blockIdx.x % splits, row0 = (blockIdx.x / splits) * kRows, b = blockIdx.y;
-  const int R = a.Tn * a.H, nrows = min(kRows, R - row0);
+  const int R = a.Tn * a.H;
+  if (tid == 0) {
+    for (int k = 0; k < kStages; ++k) mbar_init(&full[k], 1);
+    fence_barrier_init();
+  }
+  if (line.min_steps > 0) launch_dependents();
+  Kv4Walk walk;
+  walk.begin(a, line);
+  int used = 0;     // tiles that went through the stages
+  bool ok = true;
 
+  while (walk.at < walk.end) {
+  int t0, step1;
+  const Kv4Piece piece = walk.next(a, line, kRows, &t0, &step1);
+  const int b = piece.b, row0 = piece.segment * kRows, nrows = min(kRows, R - row0);
+  const int sink_tiles = piece.sink_tiles, first = piece.first, t1 = min(piece.tiles, step1);
   Kv4Seen seen{0, 0};
   if (lane < nrows) seen = kv4_seen(a, b, (row0 + lane) / a.H);
-  const int lo_min = __reduce_min_sync(0xffffffffu, lane < nrows ? seen.lo : a.L);
-  const int hi_max = __reduce_max_sync(0xffffffffu, lane < nrows ? seen.hi : 0);
   const int lo_max = __reduce_max_sync(0xffffffffu, lane < nrows ? seen.lo : 0);
   const int hi_min = __reduce_min_sync(0xffffffffu, lane < nrows ? seen.hi : a.L);
-  const int sink_tiles = (a.n_sink + kTile - 1) / kTile;
-  const int first = max(lo_min / kTile, sink_tiles);
-  const int tiles = sink_tiles + max(0, hi_max > lo_min ? (hi_max + kTile - 1) / kTile - first : 0);
-  const int per = (tiles + splits - 1) / splits;
-  const int t0 = split * per, t1 = min(tiles, t0 + per);
   auto row_of = [&](int tile) { return (tile < sink_tiles ? tile : first + tile - sink_tiles) * kTile; };
 
   const uint8_t* kc = a.k.codes + b * a.k.c_b;
@@ -86,12 +92,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
     bulk_load(dst, kc + r0 * C::kRow, n * C::kRow, &full[stage]);
     bulk_load(dst + C::kCodes, kp + r0 * (NG * 4), n * NG * 4, &full[stage]);
   };
-  if (tid == 0) {
-    for (int s = 0; s < kStages; ++s) mbar_init(&full[s], 1);
-    fence_barrier_init();
-    for (int s = 0; s < kStages; ++s)
-      if (t0 + s < t1) issue(t0 + s, s);
-  }
+  if (tid == 0)
+    for (int k = 0; k < kStages; ++k)
+      if (t0 + k < t1) issue(t0 + k, (used + k) % kStages);
 
   // ---- queries: normalised fp16, laid out as the operands of the scores ------------
   for (int r = warp; r < kRows; r += kWarps) {
@@ -170,10 +173,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
   const int key_i = i ^ ((i >> 2) & 1);
   const int key_0 = (2 * j) ^ ((j >> 1) & 1), key_1 = (2 * j + 1) ^ ((j >> 1) & 1);
 
-  bool ok = true;
   for (int tile = t0; tile < t1; ++tile) {
-    const int stage = (tile - t0) % kStages;
-    ok = mbar_wait(&full[stage], ((tile - t0) / kStages) & 1, st, STATUS_TIMEOUT_TMA_FULL) && ok;
+    const int stage = (used + tile - t0) % kStages;
+    ok = mbar_wait(&full[stage], ((used + tile - t0) / kStages) & 1, st, STATUS_TIMEOUT_TMA_FULL) && ok;
     const uint32_t codes = smem_u32(smem + stage * C::kStage), params = codes + C::kCodes;
     const int r0 = row_of(tile);
 
@@ -199,7 +201,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
 #pragma unroll
         for (int k = 0; k < 3; ++k) mma_bf16(s[mt][nt], m[0], m[1], m[2], m[3], qm[k][nt][0], qm[k][nt][1]);
     }
-#pragma unroll
+    // rolled, as the loop over the values below: the code must stay in the instruction cache
+#pragma unroll 1
     for (int g = 0; g < NG; ++g) {
       uint2 wa[2], wb[2];
       float d[2][NT][4];
@@ -312,7 +315,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
     __syncthreads();
 
     // ---- output: this warp's value groups over all keys of the tile -------------------
-#pragma unroll 2
+#pragma unroll 1
     for (int kt = 0; kt < kTile / 16; ++kt) {
       float2 p0[NT], p8[NT];  // weights of row i at mma rows 2j, 2j + 1 and + 8
 #pragma unroll
@@ -350,17 +353,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
         }
         const uint32_t l0 = __byte_perm(w0, w1, 0x5410), h0 = __byte_perm(w0, w1, 0x7632);
         const uint32_t l8 = __byte_perm(w8, w9, 0x5410), h8 = __byte_perm(w8, w9, 0x7632);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          mma_bf16(acc[g][0][nt], nibbles_bf16<0>(l0), nibbles_bf16<0>(h0), nibbles_bf16<0>(l8), nibbles_bf16<0>(h8),
-                   bw[nt][0], bw[nt][1]);
-          mma_bf16(acc[g][1][nt], nibbles_bf16<1>(l0), nibbles_bf16<1>(h0), nibbles_bf16<1>(l8), nibbles_bf16<1>(h8),
-                   bw[nt][0], bw[nt][1]);
-          mma_bf16(acc[g][2][nt], nibbles_bf16<2>(l0), nibbles_bf16<2>(h0), nibbles_bf16<2>(l8), nibbles_bf16<2>(h8),
-                   bw[nt][0], bw[nt][1]);
-          mma_bf16(acc[g][3][nt], nibbles_bf16<3>(l0), nibbles_bf16<3>(h0), nibbles_bf16<3>(l8), nibbles_bf16<3>(h8),
-                   bw[nt][0], bw[nt][1]);
-        }
+        mma_values<0, NT>(acc[g][0], l0, h0, l8, h8, bw);
+        mma_values<1, NT>(acc[g][1], l0, h0, l8, h8, bw);
+        mma_values<2, NT>(acc[g][2], l0, h0, l8, h8, bw);
+        mma_values<3, NT>(acc[g][3], l0, h0, l8, h8, bw);
       }
     }
     if (tile + kStages < t1) {
@@ -368,7 +364,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
       if (tid == 0) issue(tile + kStages, stage);
     }
   }
-  (void)ok;
+  used += max(0, t1 - t0);
 
   // ---- join: row maxima are the block's already; sums over the warps' keys -------------
   __syncthreads();
@@ -392,7 +388,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
       if (j == 0) sp[(warp * VG + g) * kRows + nt * 8 + i] = m;
     }
   __syncthreads();
-  float* pml = a.part + (size_t)a.B * R * splits * V;
+  const bool alone = t0 == 0 && step1 == piece.steps;
+  float* part = a.part + (size_t)(2 * blockIdx.x + (t0 == 0)) * kRows * (V + 2);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -402,8 +399,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
       float l = 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) l += smx[w * kRows + q];
-      const long long head = (long long)b * R + row0 + q;
-      const float inv = splits > 1 ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+      const float inv = !alone ? 1.f : (l == 0.f ? 0.f : 1.f / l);
 #pragma unroll
       for (int g = 0; g < VG; ++g) {
         const float m = fmaf(-24.f, accr[g][nt][c], sp[(warp * VG + g) * kRows + q]);
@@ -414,19 +410,22 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
           o[4 + mm] = (acc[g][mm][nt][c + 2] + m) * inv;
         }
         const int d = (warp * VG + g) * 64 + 8 * i;
-        if (splits > 1) {
-          float4* p = reinterpret_cast<float4*>(a.part + (head * splits + split) * V + d);
+        if (!alone) {
+          float4* p = reinterpret_cast<float4*>(part + q * V + d);
           p[0] = make_float4(o[0], o[1], o[2], o[3]);
           p[1] = make_float4(o[4], o[5], o[6], o[7]);
         } else {
-          *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + head * V + d) =
+          *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + ((long long)b * R + row0 + q) * V + d) =
               make_uint4(kv4_pack2<TYPE>(o[0], o[1]), kv4_pack2<TYPE>(o[2], o[3]), kv4_pack2<TYPE>(o[4], o[5]),
                          kv4_pack2<TYPE>(o[6], o[7]));
         }
       }
-      if (splits > 1 && warp == 0 && i == 0)
-        *reinterpret_cast<float2*>(pml + (head * splits + split) * 2) = make_float2(mx[nt][c], l);
+      if (!alone && warp == 0 && i == 0)
+        *reinterpret_cast<float2*>(part + kRows * V + 2 * q) = make_float2(mx[nt][c], l);
     }
+  __syncthreads();  // the next segment refills shared memory
+  }
+  (void)ok;
 }
 
 template <int V, int TYPE>
@@ -434,8 +433,8 @@ void launch(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s) {
   auto kern = kv4_latent_kernel<V, TYPE>;
   constexpr int smem = LatentCfg<V>::kSmem;
   ensure_smem_attr(reinterpret_cast<const void*>(kern), smem);
-  kern<<<dim3((unsigned)(p.splits * p.row_blocks), (unsigned)a.B), kWarps * 32, smem, s>>>(
-      a, p.splits, reinterpret_cast<StatusBlock*>(status_ptr()));
+  kern<<<p.blocks, kWarps * 32, smem, s>>>(a, kv4_line(a, p, kTile),
+                                           reinterpret_cast<StatusBlock*>(status_ptr()));
 }
 
 }  // namespace
@@ -444,19 +443,7 @@ void kv4_latent_plan(const Kv4Attend& a, Kv4Plan& p) {
   p.kernel = 2;
   p.row_tiles = NT;
   p.row_blocks = (a.Tn * a.H + kRows - 1) / kRows;
-  const long long rows = std::min<long long>(a.L - a.sink_rows, a.window > 0 ? a.window + a.Tn : 1 << 30);
-  const int tiles = (a.n_sink + kTile - 1) / kTile + (int)((rows + kTile - 1) / kTile) + 1;
-  const long long blocks = (long long)a.B * p.row_blocks, slots = 148 * 2;
-  long long best = -1;
-  for (int sp = 1; sp <= 64 && sp <= tiles; ++sp) {
-    const long long waves = (blocks * sp + slots - 1) / slots;
-    const long long cost = waves * (2 * ((tiles + sp - 1) / sp) + 3) + (sp > 1 ? 2 : 0);
-    if (best < 0 || cost < best) {
-      best = cost;
-      p.splits = sp;
-    }
-  }
-  p.floats = p.splits > 1 ? (size_t)a.B * a.Tn * a.H * p.splits * (a.V + 2) : 0;
+  kv4_line_plan(a, p, 148 * 2, 1);
 }
 
 void kv4_latent_launch(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s) {
@@ -464,7 +451,7 @@ void kv4_latent_launch(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s) {
     a.V == 512 ? launch<512, KV4_F16>(a, p, s) : launch<256, KV4_F16>(a, p, s);
   else
     a.V == 512 ? launch<512, KV4_BF16>(a, p, s) : launch<256, KV4_BF16>(a, p, s);
-  if (p.splits > 1) kv4_combine(a, p.splits, s);
+  if (p.min_steps > 0) kv4_combine(a, p, s);
 }
 
 }  // namespace omni

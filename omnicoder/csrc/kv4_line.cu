@@ -1,0 +1,108 @@
+// How the attention kernels over a 4-bit cache share their keys, and the kernel
+// that joins what they shared.
+#include <algorithm>
+
+#include "kv4_device.cuh"
+
+namespace omni {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+// A block per query row: V / 4 threads hold four value dims each, the rest of the
+// block takes every n-th piece; pieces are summed in a fixed order.
+template <int TYPE>
+__global__ void __launch_bounds__(kThreads) kv4_combine_kernel(const Kv4Attend a, const Kv4Line line, const int rows_per_block) {
+  __shared__ float4 s_sum[kThreads];
+  __shared__ float2 s_ml[kThreads];
+  const int G = a.H / a.Hk, R = a.Tn * G, row_blocks = line.segments / a.Hk;
+  const int row = blockIdx.x % R, hk = blockIdx.x / R % a.Hk, b = blockIdx.x / R / a.Hk;
+  const int r = row % rows_per_block, cols = a.V / 4, groups = kThreads / cols;
+  const int col = threadIdx.x % cols, group = threadIdx.x / cols;
+  wait_for_previous_grid();
+  const int2 range = line.meta[b * line.segments + hk * row_blocks + row / rows_per_block];
+  if (range.x == range.y) return;  // one block held the segment and has written the row
+  const size_t slot = (size_t)rows_per_block * (a.V + 2);
+  float top = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (group < groups) {
+#pragma unroll 4
+    for (int k = range.x + group; k <= range.y; k += groups) {
+      const float* p = a.part + (2 * (size_t)k + (k == range.x)) * slot;
+      const float2 ml = *reinterpret_cast<const float2*>(p + rows_per_block * a.V + 2 * r);
+      const float4 v = *reinterpret_cast<const float4*>(p + r * a.V + 4 * col);
+      const float m = fmaxf(top, ml.x), ref = m == -INFINITY ? 0.f : m;
+      const float f0 = fast_exp2(top - ref), f1 = fast_exp2(ml.x - ref);
+      l = l * f0 + ml.y * f1;
+      o.x = o.x * f0 + v.x * f1;
+      o.y = o.y * f0 + v.y * f1;
+      o.z = o.z * f0 + v.z * f1;
+      o.w = o.w * f0 + v.w * f1;
+      top = m;
+    }
+  }
+  s_sum[threadIdx.x] = o;
+  s_ml[threadIdx.x] = make_float2(top, l);
+  __syncthreads();
+  if (group != 0) return;
+  for (int g = 1; g < groups; ++g) top = fmaxf(top, s_ml[g * cols + col].x);
+  const float ref = top == -INFINITY ? 0.f : top;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  l = 0.f;
+  for (int g = 0; g < groups; ++g) {
+    const float2 ml = s_ml[g * cols + col];
+    const float4 v = s_sum[g * cols + col];
+    const float f = fast_exp2(ml.x - ref);
+    l = fmaf(f, ml.y, l);
+    x.x = fmaf(f, v.x, x.x);
+    x.y = fmaf(f, v.y, x.y);
+    x.z = fmaf(f, v.z, x.z);
+    x.w = fmaf(f, v.w, x.w);
+  }
+  const long long head = ((long long)b * a.Tn + row / G) * a.H + hk * G + row % G;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + head * a.V + 4 * col) =
+      make_uint2(kv4_pack2<TYPE>(x.x * inv, x.y * inv), kv4_pack2<TYPE>(x.z * inv, x.w * inv));
+}
+
+}  // namespace
+
+Kv4Line kv4_line(const Kv4Attend& a, const Kv4Plan& p, int tile) {
+  const size_t sums = (size_t)p.blocks * 2 * 8 * p.row_tiles * (a.V + 2);
+  return Kv4Line{a.Hk * p.row_blocks, tile, p.min_steps, reinterpret_cast<int2*>(a.part + sums)};
+}
+
+// The host knows the cache's size, not the sequences' lengths.  A block per segment where a full
+// cache (or window) is at most two steps, or where finding a block's place on the line would cost
+// more than uneven lengths: many sequences, many new tokens.
+void kv4_line_plan(const Kv4Attend& a, Kv4Plan& p, int slots, int min_steps) {
+  const long long rows = a.n_sink + std::min<long long>(a.L - a.sink_rows, a.window > 0 ? (long long)a.window + a.Tn : 1 << 30);
+  const long long steps = (rows + kKv4Step - 1) / kKv4Step, segments = (long long)a.B * a.Hk * p.row_blocks;
+  if (steps <= 2 || a.B > 256 || a.Tn > 16) {
+    p.min_steps = 0;
+    p.blocks = (int)segments;
+    p.floats = 0;
+    return;
+  }
+  p.min_steps = min_steps;
+  p.blocks = (int)std::min<long long>(slots, (segments * (steps + 1) + min_steps - 1) / min_steps);
+  p.floats = (size_t)p.blocks * 2 * 8 * p.row_tiles * (a.V + 2) + 2 * (size_t)segments;
+}
+
+void kv4_combine(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s) {
+  const Kv4Line line = kv4_line(a, p, 0);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((long long)a.B * a.Tn * a.H));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  if (a.type == KV4_F16) cudaLaunchKernelEx(&cfg, kv4_combine_kernel<KV4_F16>, a, line, 8 * p.row_tiles);
+  else cudaLaunchKernelEx(&cfg, kv4_combine_kernel<KV4_BF16>, a, line, 8 * p.row_tiles);
+}
+
+}  // namespace omni

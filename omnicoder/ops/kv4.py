@@ -9,7 +9,7 @@ and stands for x = n * s + m, n = 0 .. 15.  A row of a head is contiguous, and s
 head (head-major, unlike the bf16 / int8 cache): the attention kernels copy whole key tiles.  With
 groups of 64 a value takes 4.5 bits; an int8 cache of 128-wide heads takes 8.25.
 
-Quantisation of a group: m = bf16(min x), s = bf16((max x - m) / 15) with the quotient in fp32, and
+Quantisation of a group: m = bf16(min x), s = bf16((max x - m) * (1 / 15)) with the product in fp32, and
 n = clamp(round((x - m) / s), 0, 15), where the rounding (ties to even) is decided as if (x - m) / s
 were exact.  s below 2^-120 is stored as 0 (then every n is 0 and the group reads back as m).  A group
 that holds a NaN or an infinity, or whose range overflows fp32, reads back as NaN; other groups of
@@ -22,7 +22,8 @@ Position p of a sequence lives in row row_offset + p.  `kv4_write` skips positio
 outside the cache, `kv4_read` returns zeros for them.  The positions that one `kv4_write` call gives
 for a sequence have to differ: two tokens written to one row at once leave a mixture.
 
-CUDA: hand-written kernels (omnicoder/csrc/kv4.cu); CPU: the plain forms below (the oracle).
+CUDA: hand-written kernels (omnicoder/csrc/kv4*.cu; a call that does not fit raises RuntimeError);
+CPU: the plain forms below (the oracle; ValueError).
 """
 from __future__ import annotations
 
@@ -79,7 +80,7 @@ def quantize_kv4(x: torch.Tensor, group: int):
     """x [..., W] -> (codes uint8 [..., W / 2], params bf16 [..., W / group, 2])."""
     g = x.double().reshape(*x.shape[:-1], x.shape[-1] // group, group)
     m = g.amin(-1).float().to(torch.bfloat16)
-    s = ((g.amax(-1).float() - m.float()) / 15.0).to(torch.bfloat16)
+    s = ((g.amax(-1).float() - m.float()) * (1.0 / 15.0)).to(torch.bfloat16)
     bad = ~(torch.isfinite(g).all(-1) & torch.isfinite(m) & torch.isfinite(s))
     s = torch.where(s.float() < _MIN_SCALE, torch.zeros_like(s), s)
     n = torch.round((g - m.double()[..., None]) / s.double()[..., None]).clamp(0, 15)
@@ -132,6 +133,11 @@ def decode_attention_kv4_torch(q, k, v, q_pos, kv_len, *, window=0, scale=None, 
 def kv4_write(pos, k, k_codes, k_params, v=None, v_codes=None, v_params=None, row_offset: int = 0) -> None:
     """Quantise new rows k (and v) [B, T, Hk, W] into the cache rows row_offset + pos[b, t], one launch
     for both.  pos int64 [B, T]; k and v fp32, fp16 or bf16."""
+    if k.is_cuda:                        # checked by the bindings
+        _ext.load().kv4_write(pos, k, k_codes, k_params, v, v_codes, v_params, row_offset)
+        return
+    if (v is None) != (v_codes is None):
+        raise ValueError("kv4_write: v together with its cache")
     pairs = [(k, k_codes, k_params, "k")] + ([(v, v_codes, v_params, "v")] if v is not None else [])
     for x, c, p, what in pairs:
         _check_cache(c, p, f"kv4_write: {what}")
@@ -139,9 +145,6 @@ def kv4_write(pos, k, k_codes, k_params, v=None, v_codes=None, v_params=None, ro
                 or x.shape[2] != c.shape[1] or x.shape[3] != 2 * c.shape[3]:
             raise ValueError(f"kv4_write: {what} {tuple(x.shape)} does not fit positions {tuple(pos.shape)} and codes "
                              f"{tuple(c.shape)}")
-    if k.is_cuda:
-        _ext.load().kv4_write(pos, k, k_codes, k_params, v, v_codes, v_params, row_offset)
-        return
     rows = pos.long() + row_offset
     for x, c, p, _ in pairs:
         codes, params = quantize_kv4(x, x.shape[3] // p.shape[3])
@@ -156,14 +159,14 @@ def kv4_read(pos, k_codes, k_params, v_codes=None, v_params=None, row_offset: in
     dtype: float32, float16 or bfloat16."""
     if dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise ValueError(f"kv4_read: dtype {dtype}")
+    if k_codes.is_cuda:                  # checked by the bindings
+        out = _ext.load().kv4_read(pos, k_codes, k_params, v_codes, v_params, row_offset, dtype)
+        return tuple(out) if v_codes is not None else out[0]
     pairs = [(k_codes, k_params, "k")] + ([(v_codes, v_params, "v")] if v_codes is not None else [])
     for c, p, what in pairs:
         _check_cache(c, p, f"kv4_read: {what}")
         if pos.dim() != 2 or pos.shape[0] != c.shape[0]:
             raise ValueError(f"kv4_read: positions {tuple(pos.shape)} for codes {tuple(c.shape)}")
-    if k_codes.is_cuda:
-        out = _ext.load().kv4_read(pos, k_codes, k_params, v_codes, v_params, row_offset, dtype)
-        return tuple(out) if v_codes is not None else out[0]
     rows = pos.long() + row_offset
     out = []
     for c, p, _ in pairs:
@@ -180,6 +183,10 @@ def decode_attention_kv4(q, k, v, q_pos, kv_len, *, window=0, scale=None, k_para
     """Attention of new tokens q [B, Tn, H, W] against a 4-bit cache (k, v codes; v None with
     latent_v_dim = r for an MLA latent, whose value is the first r dims of a row).  Visibility as in
     omnicoder.ops.decode; a query that sees no row gets zeros.  -> [B, Tn, H, W or r]."""
+    sc = scale if scale is not None else 1.0 / math.sqrt(q.shape[3])
+    if q.is_cuda:                        # checked by the bindings
+        return _ext.load().kv4_attend(q, k, k_params, v, v_params, q_pos, kv_len, window, sc, latent_v_dim,
+                                      sink_rows, n_sink)
     _check_cache(k, k_params, "decode_attention: k")
     if q.dim() != 4 or q.shape[0] != k.shape[0] or q.shape[3] != 2 * k.shape[3] or q.shape[2] % max(1, k.shape[1]):
         raise ValueError(f"decode_attention: q {tuple(q.shape)} against codes {tuple(k.shape)}")
@@ -197,10 +204,6 @@ def decode_attention_kv4(q, k, v, q_pos, kv_len, *, window=0, scale=None, k_para
         raise ValueError("decode_attention: q_pos [B, Tn], kv_len [B]")
     if not 0 <= n_sink <= sink_rows <= k.shape[2] or window < 0:
         raise ValueError("decode_attention: 0 <= n_sink <= sink_rows <= L, window >= 0")
-    sc = scale if scale is not None else 1.0 / math.sqrt(q.shape[3])
-    if q.is_cuda:
-        return _ext.load().kv4_attend(q, k, k_params, v, v_params, q_pos, kv_len, window, sc, latent_v_dim,
-                                      sink_rows, n_sink)
     return decode_attention_kv4_torch(q, k, v, q_pos, kv_len, window=window, scale=sc, k_params=k_params,
                                       v_params=v_params, latent_v_dim=latent_v_dim, sink_rows=sink_rows,
                                       n_sink=n_sink)
