@@ -10,6 +10,11 @@ constexpr float kKv4Log2e = 1.4426950408889634f;
 __device__ __forceinline__ long long kv4_load_pos(const void* p, bool is64, long long i) {
   return is64 ? reinterpret_cast<const long long*>(p)[i] : (long long)reinterpret_cast<const int*>(p)[i];
 }
+// Positions of the attention, beyond any cache row (L < 2^30) cut off.
+__device__ __forceinline__ int kv4_load_near(const void* p, bool is64, long long i) {
+  if (!is64) return min(max(reinterpret_cast<const int*>(p)[i], -(1 << 30)), 1 << 30);
+  return (int)min(max(reinterpret_cast<const long long*>(p)[i], -(1ll << 30)), 1ll << 30);
+}
 
 template <int TYPE>
 __device__ __forceinline__ float kv4_load1(const void* base, long long i) {
@@ -31,14 +36,13 @@ struct Kv4Seen {
 };
 
 __device__ __forceinline__ Kv4Seen kv4_seen(const Kv4Attend& a, int b, int t) {
-  const long long len = kv4_load_pos(a.kv_len, a.len64, b);
-  const long long qp = kv4_load_pos(a.q_pos, a.pos64, (long long)b * a.Tn + t);
-  const long long room = a.L - a.sink_rows;
-  const long long end = max(min(min(len, qp + 1), room), 0ll);
-  const long long first = a.window > 0 ? max(qp - a.window + 1, 0ll) : 0ll;
+  const int len = kv4_load_near(a.kv_len, a.len64, b);
+  const int qp = kv4_load_near(a.q_pos, a.pos64, (long long)b * a.Tn + t), room = a.L - a.sink_rows;
+  const int end = max(min(min(len, qp + 1), room), 0);
+  const int first = a.window > 0 ? max(qp - a.window + 1, 0) : 0;
   Kv4Seen s;
-  s.lo = a.sink_rows + (int)min(first, room);
-  s.hi = max(a.sink_rows + (int)end, s.lo);
+  s.lo = a.sink_rows + min(first, room);
+  s.hi = max(a.sink_rows + end, s.lo);
   return s;
 }
 
@@ -148,10 +152,11 @@ struct Kv4Line {
   int2* meta;      // [B * segments] first and last block
 };
 
+constexpr int kKv4MaxLine = 256;   // sequences on a line
+
 struct Kv4Piece {
   int b, segment;                  // sequence, segment of it
-  long long begin;                 // its first step on the line
-  int steps;
+  int steps, step0, step1;         // of the segment; the block's own
   int sink_tiles, first, tiles;    // tiles over the memory rows; first tile behind them; all
 };
 
@@ -176,82 +181,84 @@ __device__ __forceinline__ void kv4_tiles(const Kv4Attend& a, Kv4Seen u, int til
   p->steps = max(1, (p->tiles + per_step - 1) / per_step);  // a sequence that sees nothing still writes zeros
 }
 
-// Whole warps: the segment that holds step `at` of the line, and the line's length.
-__device__ __forceinline__ Kv4Piece kv4_locate(const Kv4Attend& a, const Kv4Line& l, long long at, long long* total) {
-  Kv4Piece p{-1, 0, 0, 1, 0, 0, 0};
-  const int lane = lane_id();
-  long long base = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 32) {
-    Kv4Piece q{0, 0, 0, 0, 0, 0, 0};
-    if (b0 + lane < a.B) kv4_tiles(a, kv4_union(a, b0 + lane, 0, a.Tn, 1), l.tile, &q);
-    long long sum = q.steps;  // inclusive prefix of the sequences' steps
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long up = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += up;
-    }
-    const long long end = base + sum * l.segments;
-    const uint32_t above = __ballot_sync(0xffffffffu, end > at);
-    if (p.b < 0 && above != 0) {
-      const int src = __ffs(above) - 1;
-      p.b = b0 + src;
-      p.steps = __shfl_sync(0xffffffffu, q.steps, src);
-      p.sink_tiles = __shfl_sync(0xffffffffu, q.sink_tiles, src);
-      p.first = __shfl_sync(0xffffffffu, q.first, src);
-      p.tiles = __shfl_sync(0xffffffffu, q.tiles, src);
-      const long long start = __shfl_sync(0xffffffffu, end, src) - (long long)p.steps * l.segments;
-      p.segment = (int)((at - start) / p.steps);
-      p.begin = start + (long long)p.segment * p.steps;
-    }
-    base = __shfl_sync(0xffffffffu, end, 31);
-  }
-  *total = base;
-  return p;
-}
-
-// The pieces of one block, in turn.
+// The pieces of one block, in turn; every thread of the block calls both functions.
+// Shared memory: for each sequence the steps up to its end, its first tile and its tiles.
 struct Kv4Walk {
-  long long at, end;
-  int share;
+  int end[kKv4MaxLine], first[kKv4MaxLine], tiles[kKv4MaxLine], sums[32];
 
-  __device__ __forceinline__ void begin(const Kv4Attend& a, const Kv4Line& l) {
-    if (l.min_steps == 0) {
-      at = 0;
-      end = 1;
-      share = 0;
-      return;
+  // -> first and last step of the block on the line
+  template <int kThreads>
+  __device__ __forceinline__ int2 begin(const Kv4Attend& a, const Kv4Line& l, int* share) {
+    if (l.min_steps == 0) return make_int2(0, 1);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int before = 0;
+    for (int b0 = 0; b0 < a.B; b0 += kThreads) {
+      Kv4Piece q;
+      q.steps = 0;
+      if (b0 + tid < a.B) kv4_tiles(a, kv4_union(a, b0 + tid, 0, a.Tn, 1), l.tile, &q);
+      int sum = q.steps;  // inclusive prefix over the threads
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += up;
+      }
+      if (lane == 31) sums[warp] = sum;
+      __syncthreads();
+      int all = before;
+#pragma unroll
+      for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < warp) sum += sums[w];
+        all += sums[w];
+      }
+      if (b0 + tid < a.B) {
+        end[b0 + tid] = before + sum;
+        first[b0 + tid] = q.first;
+        tiles[b0 + tid] = q.tiles;
+      }
+      before = all;
+      __syncthreads();
     }
-    long long total;
-    kv4_locate(a, l, 0, &total);
-    share = max((int)((total + gridDim.x - 1) / gridDim.x), l.min_steps);
-    at = (long long)blockIdx.x * share;
-    end = min(total, at + share);
+    const int total = before * l.segments;
+    *share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, l.min_steps);
+    const int at = blockIdx.x * *share;
+    return make_int2(at, min(total, at + *share));
   }
-  // Whole warps; rows_per_block query rows of a segment.  step0 .. step1: this block's steps of it.
-  __device__ __forceinline__ Kv4Piece next(const Kv4Attend& a, const Kv4Line& l, int rows_per_block, int* step0, int* step1) {
+
+  // The segment that holds step span.x; moves span.x behind it.
+  __device__ __forceinline__ Kv4Piece next(const Kv4Attend& a, const Kv4Line& l, int rows_per_block, int share, int2* span) {
     Kv4Piece p;
     if (l.min_steps == 0) {
       p.b = blockIdx.x / l.segments;
       p.segment = blockIdx.x % l.segments;
-      p.begin = 0;
       const int G = a.H / a.Hk, row0 = p.segment % (l.segments / a.Hk) * rows_per_block;
       const int t0 = row0 / G, t1 = (min(row0 + rows_per_block, a.Tn * G) - 1) / G + 1;
       Kv4Seen u = kv4_union(a, p.b, t0 + lane_id(), t1, 32);
       u.lo = __reduce_min_sync(0xffffffffu, u.lo);
       u.hi = __reduce_max_sync(0xffffffffu, u.hi);
       kv4_tiles(a, u, l.tile, &p);
-      *step0 = 0;
-      *step1 = p.steps;
-      at = end;
+      p.step0 = 0;
+      p.step1 = p.steps;
+      span->x = span->y;
     } else {
-      long long total;
-      p = kv4_locate(a, l, at, &total);
-      *step0 = (int)(at - p.begin);
-      *step1 = (int)min((long long)p.steps, end - p.begin);
-      if (at == p.begin && threadIdx.x == 0)
-        l.meta[p.b * l.segments + p.segment] =
-            make_int2(blockIdx.x, (int)((p.begin + p.steps - 1) / share));
-      at = p.begin + p.steps;
+      int lo = 0, hi = a.B - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (end[mid] * l.segments > span->x) hi = mid;
+        else lo = mid + 1;
+      }
+      const int start = lo > 0 ? end[lo - 1] : 0;
+      p.b = lo;
+      p.steps = end[lo] - start;
+      p.first = first[lo];
+      p.tiles = tiles[lo];
+      p.sink_tiles = (a.n_sink + l.tile - 1) / l.tile;
+      p.segment = (span->x - start * l.segments) / p.steps;
+      const int at = start * l.segments + p.segment * p.steps;   // the segment's first step on the line
+      p.step0 = span->x - at;
+      p.step1 = min(p.steps, span->y - at);
+      if (p.step0 == 0 && threadIdx.x == 0)
+        l.meta[p.b * l.segments + p.segment] = make_int2(blockIdx.x, (at + p.steps - 1) / share);
+      span->x = at + p.steps;
     }
     return p;
   }

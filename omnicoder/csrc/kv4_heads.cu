@@ -70,16 +70,16 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
   const int G = a.H / a.Hk, R = a.Tn * G, row_blocks = line.segments / a.Hk;
   const uint32_t ring = smem_u32(smem) + warp * C::kStages * C::kStage;
   if (line.min_steps > 0) launch_dependents();
-  Kv4Walk walk;
-  walk.begin(a, line);
+  __shared__ Kv4Walk walk;
+  int share = 0;
+  int2 span = walk.begin<kWarps * 32>(a, line, &share);
 
-  while (walk.at < walk.end) {
-  int step0, step1;
-  const Kv4Piece piece = walk.next(a, line, C::kRows, &step0, &step1);
+  while (span.x < span.y) {
+  const Kv4Piece piece = walk.next(a, line, C::kRows, share, &span);
   const int b = piece.b, hk = piece.segment / row_blocks, row0 = (piece.segment % row_blocks) * C::kRows;
   const int nrows = min(C::kRows, R - row0);
   const int sink_tiles = piece.sink_tiles, first = piece.first;
-  const int t0 = step0 * kWarps, t1 = min(piece.tiles, step1 * kWarps);
+  const int t0 = piece.step0 * kWarps, t1 = min(piece.tiles, piece.step1 * kWarps);
 
   // ---- the rows each query sees; lane r holds query row r --------------------
   Kv4Seen seen{0, 0};
@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
     }
   }
 
-  float acc[NG][4][NT][4], accr[NT][4], accm[NG][NT][2], lsum[NT][2];
+  float acc[NG][4][NT][4], accr[NG][NT][4], accm[NG][NT][2], lsum[NT][2];
   float limit[NT][2], ref[NT][2];  // running maximum + slack, running maximum (0 before any key)
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -185,9 +185,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
       for (int c = 0; c < 4; ++c)
 #pragma unroll
         for (int mm = 0; mm < 4; ++mm) acc[g][mm][nt][c] = 0.f;
+      accr[g][nt][0] = accr[g][nt][1] = accr[g][nt][2] = accr[g][nt][3] = 0.f;
       accm[g][nt][0] = accm[g][nt][1] = 0.f;
     }
-    accr[nt][0] = accr[nt][1] = accr[nt][2] = accr[nt][3] = 0.f;
     lsum[nt][0] = lsum[nt][1] = 0.f;
     limit[nt][0] = limit[nt][1] = -INFINITY;
     ref[nt][0] = ref[nt][1] = 0.f;
@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
               accm[g][nt][c] *= alpha;
-              accr[nt][c + 2 * g] *= alpha;
+              accr[g][nt][c] *= alpha;
 #pragma unroll
               for (int mm = 0; mm < 4; ++mm) {
                 acc[g][mm][nt][c] *= alpha;
@@ -325,8 +325,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
           }
           bw[nt][0] = movmatrix_trans(pack_bf16x2(x[0], x[1]));
           bw[nt][1] = movmatrix_trans(pack_bf16x2(x[2], x[3]));
-          mma_bf16(accr[nt], g == 0 ? 0x3f803f80u : 0u, g == 1 ? 0x3f803f80u : 0u, g == 0 ? 0x3f803f80u : 0u,
-                   g == 1 ? 0x3f803f80u : 0u, bw[nt][0], bw[nt][1]);
+          mma_bf16(accr[g][nt], 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, bw[nt][0], bw[nt][1]);
         }
         const uint32_t w0 = lds32(st + v_at0[g]), w1 = lds32(st + v_at1[g]);
         const uint32_t w8 = lds32(st + v_at0[g] + 8 * C::kRow), w9 = lds32(st + v_at1[g] + 8 * C::kRow);
@@ -363,7 +362,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
         float m = accm[g][nt][c];
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
-        m = fmaf(-24.f, accr[nt][c + 2 * g], m);
+        m = fmaf(-24.f, accr[g][nt][c], m);
         float* o = so + r * D + g * 64 + 8 * i;
 #pragma unroll
         for (int mm = 0; mm < 4; ++mm) {
@@ -374,8 +373,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
     }
   __syncthreads();
   // a segment that this block holds alone is finished; otherwise its piece goes to a slot
-  const bool alone = step0 == 0 && step1 == piece.steps;
-  float* part = a.part + (size_t)(2 * blockIdx.x + (step0 == 0)) * C::kRows * (D + 2);
+  const bool alone = piece.step0 == 0 && piece.step1 == piece.steps;
+  float* part = a.part + (size_t)(2 * blockIdx.x + (piece.step0 == 0)) * C::kRows * (D + 2);
   for (int idx = threadIdx.x; idx < nrows * (D / 2); idx += kWarps * 32) {
     const int r = idx / (D / 2), d = (idx % (D / 2)) * 2;
     float top = -INFINITY, l = 0.f, x = 0.f, y = 0.f;

@@ -5,9 +5,9 @@
 //   o_d     = sum_t (p_t s_tg) (n_td - 8) + sum_t p_t (m_tg + 8 s_tg)
 //
 // 16 rows of up to 576 + 512 products per key are too much output for one warp's
-// registers, so the four warps of a block share a tile of 128 keys: each warp
-// scores 32 of them over all groups, then the weights go through shared memory
-// and each warp accumulates a quarter of the value dims over all 128.  A tile is
+// registers, so the eight warps of a block share a tile of 128 keys: each warp
+// scores 16 of them over all groups, then the weights go through shared memory
+// and each warp accumulates an eighth of the value dims over all 128.  A tile is
 // one contiguous piece of memory and arrives by two bulk copies on an mbarrier.
 // The sum over groups of m sum(q_g) is a product of its own, keys x groups, with
 // m in bf16 as stored and sum(q_g) split into three bf16 terms: nine
@@ -22,8 +22,8 @@ void* status_ptr();  // bindings.cpp
 
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kTile = 128;
+constexpr int kWarps = 8;
+constexpr int kTile = 16 * kWarps;
 constexpr int kStages = 2;
 constexpr int kRows = 16;       // query rows of a block (two mma columns of 8)
 constexpr int NT = kRows / 8;
@@ -34,7 +34,7 @@ template <int V>
 struct LatentCfg {
   static constexpr int W = V + 64;
   static constexpr int NG = W / 64;                  // key groups
-  static constexpr int VG = V / 64 / kWarps;         // value groups of a warp
+  static constexpr int MM = V / 16 / kWarps;         // 16-dim value tiles of a warp: 4 (a group) or 2 (half of one)
   static constexpr int kRow = W / 2;
   static constexpr int kCodes = kTile * kRow;
   static constexpr int kParams = kTile * NG * 4;
@@ -48,7 +48,7 @@ struct LatentCfg {
 template <int V, int TYPE>
 __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Attend a, const Kv4Line line, StatusBlock* st) {
   using C = LatentCfg<V>;
-  constexpr int W = C::W, NG = C::NG, VG = C::VG;
+  constexpr int W = C::W, NG = C::NG, MM = C::MM;
   extern __shared__ __align__(128) uint8_t smem[];
   uint32_t* sqf = reinterpret_cast<uint32_t*>(smem + C::kQf);
   float* sp = reinterpret_cast<float*>(smem + C::kP);
@@ -66,16 +66,17 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
     fence_barrier_init();
   }
   if (line.min_steps > 0) launch_dependents();
-  Kv4Walk walk;
-  walk.begin(a, line);
+  __shared__ Kv4Walk walk;
+  int share = 0;
+  int2 span = walk.begin<kWarps * 32>(a, line, &share);
   int used = 0;     // tiles that went through the stages
   bool ok = true;
 
-  while (walk.at < walk.end) {
-  int t0, step1;
-  const Kv4Piece piece = walk.next(a, line, kRows, &t0, &step1);
+  while (span.x < span.y) {
+  const Kv4Piece piece = walk.next(a, line, kRows, share, &span);
   const int b = piece.b, row0 = piece.segment * kRows, nrows = min(kRows, R - row0);
-  const int sink_tiles = piece.sink_tiles, first = piece.first, t1 = min(piece.tiles, step1);
+  const int sink_tiles = piece.sink_tiles, first = piece.first;
+  const int t0 = piece.step0, t1 = min(piece.tiles, piece.step1);
   Kv4Seen seen{0, 0};
   if (lane < nrows) seen = kv4_seen(a, b, (row0 + lane) / a.H);
   const int lo_max = __reduce_max_sync(0xffffffffu, lane < nrows ? seen.lo : 0);
@@ -96,33 +97,54 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
     for (int k = 0; k < kStages; ++k)
       if (t0 + k < t1) issue(t0 + k, (used + k) % kStages);
 
-  // ---- queries: normalised fp16, laid out as the operands of the scores ------------
+  // ---- queries: normalised fp16, laid out as the operands of the scores.  A lane takes the eight
+  // dims of a code word, whose nibble pairs (0, 4), (1, 5), (2, 6), (3, 7) are two k steps.
   for (int r = warp; r < kRows; r += kWarps) {
-    float x[W / 32], amax = 0.f, un;
-    const long long at = ((long long)b * R + row0 + r) * W;
+    constexpr int kWords = W / 8, kPer = (kWords + 31) / 32;
+    float amax = 0.f, un;
+    uint4 raw[kPer];
+    float x[kPer][8];
 #pragma unroll
-    for (int e = 0; e < W / 32; ++e) {
-      x[e] = r < nrows ? kv4_load1<TYPE>(a.q, at + lane + 32 * e) : 0.f;
-      amax = fmaxf(amax, fabsf(x[e]));
+    for (int e = 0; e < kPer; ++e) {
+      const int w = lane + 32 * e;
+      raw[e] = make_uint4(0, 0, 0, 0);
+      if (r < nrows && w < kWords)
+        raw[e] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.q) + ((long long)b * R + row0 + r) * W + w * 8);
+    }
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const uint32_t u[4] = {raw[e].x, raw[e].y, raw[e].z, raw[e].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = TYPE == KV4_BF16 ? make_float2(bf16_lo(u[k]), bf16_hi(u[k])) : __half22float2(*reinterpret_cast<const __half2*>(&u[k]));
+        x[e][2 * k] = f.x;
+        x[e][2 * k + 1] = f.y;
+        amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+      }
     }
     const float sc = q_normaliser(warp_max(amax), &un);
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
+    for (int e = 0; e < kPer; ++e) {
+      const int w = lane + 32 * e, g = w >> 3, jj = (w >> 1) & 3;
       float sum = 0.f;
+      if (w < kWords) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int d = lane + 32 * e;                   // dim of the group: lane d / 16 reads words d / 8
-        const __half h = __float2half_rn(x[2 * g + e] * sc);
-        sum += __half2float(h);
-        const int jj = d >> 4, ks = ((d >> 3) & 1) * 2 + ((d >> 1) & 1), odd = d & 1, hi = (d >> 2) & 1;
-        const __half v = odd ? __hmul(h, __float2half_rn(0.0625f)) : h;
-        // [g, ks][lane (r & 7, jj)][row tile, even / odd nibble][low / high half]
-        reinterpret_cast<__half*>(sqf)[(((g * 4 + ks) * 32 + (r & 7) * 4 + jj) * 4 + (r >> 3) * 2 + odd) * 2 + hi] = v;
+        for (int k = 0; k < 2; ++k) {
+          const __half2 even = __floats2half2_rn(x[e][2 * k] * sc, x[e][2 * k + 4] * sc);
+          const __half2 odd = __floats2half2_rn(x[e][2 * k + 1] * sc, x[e][2 * k + 5] * sc);
+          const __half2 odd16 = __hmul2(odd, __float2half2_rn(0.0625f));
+          const float2 fe = __half22float2(even), fo = __half22float2(odd);
+          sum += (fe.x + fe.y) + (fo.x + fo.y);
+          // [g, ks][lane (r & 7, jj)][row tile, even / odd nibbles]
+          *reinterpret_cast<uint2*>(sqf + ((g * 4 + (w & 1) * 2 + k) * 32 + (r & 7) * 4 + jj) * 4 + (r >> 3) * 2) =
+              make_uint2(*reinterpret_cast<const uint32_t*>(&even), *reinterpret_cast<const uint32_t*>(&odd16));
+        }
       }
-      sum = warp_sum(sum);
-      if (lane == 0) sqs[r * 16 + g] = sum * 5.9604644775390625e-8f;
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if ((lane & 7) == 0 && g < 16) sqs[r * 16 + g] = w < kWords ? sum * 5.9604644775390625e-8f : 0.f;
     }
-    if (lane >= NG && lane < 16) sqs[r * 16 + lane] = 0.f;
+    if (lane >= kPer * 4 && lane < 16) sqs[r * 16 + lane] = 0.f;
     if (lane == 0) srs[r] = un * (a.scale * (kKv4Log2e * kKv4Codes));
   }
   if (warp == 0 && lane < kRows) {
@@ -151,26 +173,26 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
 #pragma unroll
     for (int c = 0; c < 2; ++c) rs[nt][c] = srs[nt * 8 + 2 * j + c];
 
-  float acc[VG][4][NT][4], accr[VG][NT][4], accm[VG][NT], lsum[NT][2], mx[NT][2];
+  // acc: a value tile holds dims MM and 4 + MM of a lane's eight; accr: sums of the rounded weights;
+  // accm: sums of p (m + 8 s)
+  float acc[MM][NT][4], accr[NT][4], accm[NT], lsum[NT][2], limit[NT][2], ref[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-    for (int g = 0; g < VG; ++g) {
+    for (int mm = 0; mm < MM; ++mm)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        accr[g][nt][c] = 0.f;
-#pragma unroll
-        for (int mm = 0; mm < 4; ++mm) acc[g][mm][nt][c] = 0.f;
-      }
-      accm[g][nt] = 0.f;
-    }
+      for (int c = 0; c < 4; ++c) acc[mm][nt][c] = 0.f;
+    accr[nt][0] = accr[nt][1] = accr[nt][2] = accr[nt][3] = accm[nt] = 0.f;
     lsum[nt][0] = lsum[nt][1] = 0.f;
-    mx[nt][0] = mx[nt][1] = -INFINITY;
+    limit[nt][0] = limit[nt][1] = -INFINITY;
+    ref[nt][0] = ref[nt][1] = 0.f;
   }
 
   // Row t of an mma tile of 16 keys is key t ^ bit2(t): the rows that one load touches then start in
   // different 32-byte slots of the banks (rows are 32 bytes apart modulo 128).
   const int key_i = i ^ ((i >> 2) & 1);
+  // this warp's value group; the upper half of its nibbles for the odd warp of a pair that shares one
+  const int vg = warp * MM / 4, v_shift = MM == 4 ? 0 : (warp & 1) * 8;
   const int key_0 = (2 * j) ^ ((j >> 1) & 1), key_1 = (2 * j + 1) ^ ((j >> 1) & 1);
 
   for (int tile = t0; tile < t1; ++tile) {
@@ -179,85 +201,69 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
     const uint32_t codes = smem_u32(smem + stage * C::kStage), params = codes + C::kCodes;
     const int r0 = row_of(tile);
 
-    // ---- scores of this warp's 32 keys ---------------------------------------------
-    float s[2][NT][4];
-    const uint32_t k_at = codes + (warp * 32 + key_i) * C::kRow + j * 8;
-    const uint32_t p_at = params + (warp * 32 + key_i) * NG * 4;
+    // ---- scores of this warp's 16 keys (this lane: mma rows i and i + 8) ----------------
+    const uint32_t k_at = codes + (warp * 16 + key_i) * C::kRow + j * 8;
+    const uint32_t p_at = params + (warp * 16 + key_i) * NG * 4;
+    float s[NT][4];
+    uint32_t m[4];
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) s[mt][nt][c] = 0.f;
-      uint32_t m[4];
-#pragma unroll
-      for (int h = 0; h < 4; ++h) {  // keys i, i + 8 against groups 2j, 2j + 1, then + 8
-        const uint32_t at = p_at + (mt * 16 + (h & 1) * 8) * NG * 4;
-        const int g = 2 * j + (h >> 1) * 8;
-        m[h] = __byte_perm(g < NG ? lds32(at + g * 4) : 0u, g + 1 < NG ? lds32(at + g * 4 + 4) : 0u, 0x7632);
-      }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int k = 0; k < 3; ++k) mma_bf16(s[mt][nt], m[0], m[1], m[2], m[3], qm[k][nt][0], qm[k][nt][1]);
+    for (int h = 0; h < 4; ++h) {  // keys i, i + 8 against groups 2j, 2j + 1, then + 8
+      const uint32_t at = p_at + (h & 1) * 8 * NG * 4;
+      const int g = 2 * j + (h >> 1) * 8;
+      m[h] = __byte_perm(g < NG ? lds32(at + g * 4) : 0u, g + 1 < NG ? lds32(at + g * 4 + 4) : 0u, 0x7632);
     }
-    // rolled, as the loop over the values below: the code must stay in the instruction cache
-#pragma unroll 1
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 3; ++k) mma_bf16(s[nt], m[0], m[1], m[2], m[3], qm[k][nt][0], qm[k][nt][1]);
+    }
+#pragma unroll 3
     for (int g = 0; g < NG; ++g) {
-      uint2 wa[2], wb[2];
-      float d[2][NT][4];
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        wa[mt] = lds64(k_at + mt * 16 * C::kRow + g * 32);
-        wb[mt] = lds64(k_at + (mt * 16 + 8) * C::kRow + g * 32);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) d[mt][nt][c] = 0.f;
-      }
+      const uint2 wa = lds64(k_at + g * 32), wb = lds64(k_at + 8 * C::kRow + g * 32);
+      const float sa = bf16_lo(lds32(p_at + g * 4)), sb = bf16_lo(lds32(p_at + (8 * NG + g) * 4));
+      float d[NT][4];
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
         const uint4 q = *reinterpret_cast<const uint4*>(sqf + ((g * 4 + ks) * 32 + lane) * 4);
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          const uint32_t xa = (ks < 2 ? wa[mt].x : wa[mt].y) >> ((ks & 1) * 8);
-          const uint32_t xb = (ks < 2 ? wb[mt].x : wb[mt].y) >> ((ks & 1) * 8);
-          mma_f16(d[mt][0], xa & 0x000f000fu, xb & 0x000f000fu, xa & 0x00f000f0u, xb & 0x00f000f0u, q.x, q.y);
-          mma_f16(d[mt][1], xa & 0x000f000fu, xb & 0x000f000fu, xa & 0x00f000f0u, xb & 0x00f000f0u, q.z, q.w);
+        const uint32_t xa = (ks < 2 ? wa.x : wa.y) >> ((ks & 1) * 8), xb = (ks < 2 ? wb.x : wb.y) >> ((ks & 1) * 8);
+        const uint32_t a0 = xa & 0x000f000fu, a1 = xb & 0x000f000fu, a2 = xa & 0x00f000f0u, a3 = xb & 0x00f000f0u;
+        if (ks == 0) {
+          mma_f16_zero(d[0], a0, a1, a2, a3, q.x, q.y);
+          mma_f16_zero(d[1], a0, a1, a2, a3, q.z, q.w);
+        } else {
+          mma_f16(d[0], a0, a1, a2, a3, q.x, q.y);
+          mma_f16(d[1], a0, a1, a2, a3, q.z, q.w);
         }
       }
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        const float sa = bf16_lo(lds32(p_at + (mt * 16 * NG + g) * 4));
-        const float sb = bf16_lo(lds32(p_at + ((mt * 16 + 8) * NG + g) * 4));
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          s[mt][nt][0] = fmaf(d[mt][nt][0], sa, s[mt][nt][0]);
-          s[mt][nt][1] = fmaf(d[mt][nt][1], sa, s[mt][nt][1]);
-          s[mt][nt][2] = fmaf(d[mt][nt][2], sb, s[mt][nt][2]);
-          s[mt][nt][3] = fmaf(d[mt][nt][3], sb, s[mt][nt][3]);
-        }
-      }
+        for (int c = 0; c < 4; ++c) s[nt][c] = fmaf(d[nt][c], c < 2 ? sa : sb, s[nt][c]);
     }
     const bool masked = !(r0 + kTile <= a.n_sink || (r0 >= lo_max && r0 + kTile <= hi_min));
     bool above = false;
     float top[NT][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
+      for (int c = 0; c < 4; ++c) s[nt][c] *= rs[nt][c & 1];
+    if (masked) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const int r = r0 + warp * 32 + mt * 16 + key_i + (c >> 1) * 8, q = nt * 8 + 2 * j + (c & 1);
-          s[mt][nt][c] *= rs[nt][c & 1];
-          if (masked && !(r < a.n_sink || (r >= slo[q] && r < shi[q]))) s[mt][nt][c] = -INFINITY;
+          const int r = r0 + warp * 16 + key_i + (c >> 1) * 8, q = nt * 8 + 2 * j + (c & 1);
+          if (!(r < a.n_sink || (r >= slo[q] && r < shi[q]))) s[nt][c] = -INFINITY;
         }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        top[nt][c] = fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]), fmaxf(s[1][nt][c], s[1][nt][c + 2]));
-        above |= top[nt][c] > mx[nt][c] + kSlack;
+        top[nt][c] = fmaxf(s[nt][c], s[nt][c + 2]);
+        above |= top[nt][c] > limit[nt][c];
       }
-    }
     // also the barrier behind the previous tile's reads of the weights
     if (__syncthreads_or(above)) {
 #pragma unroll
@@ -275,88 +281,80 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const int q = nt * 8 + 2 * j + c;
-          float x = mx[nt][c];
+          const float old = limit[nt][c] - kSlack;
+          float x = old;
 #pragma unroll
           for (int w = 0; w < kWarps; ++w) x = fmaxf(x, smx[w * kRows + q]);
-          const float alpha = x == -INFINITY ? 1.f : fast_exp2(mx[nt][c] - x);
-          mx[nt][c] = x;
+          limit[nt][c] = x + kSlack;
+          // what was summed is in units of 2^ref, whatever limit - kSlack rounds to
+          const float now = x == -INFINITY ? 0.f : x;
+          const float alpha = old == -INFINITY ? 0.f : fast_exp2(ref[nt][c] - now);
+          ref[nt][c] = now;
           lsum[nt][c] *= alpha;
+          accr[nt][c] *= alpha;
           if (warp == 0 && i == 0) sal[q] = alpha;
 #pragma unroll
-          for (int g = 0; g < VG; ++g) {
-            accr[g][nt][c] *= alpha;
-#pragma unroll
-            for (int mm = 0; mm < 4; ++mm) {
-              acc[g][mm][nt][c] *= alpha;
-              acc[g][mm][nt][c + 2] *= alpha;
-            }
+          for (int mm = 0; mm < MM; ++mm) {
+            acc[mm][nt][c] *= alpha;
+            acc[mm][nt][c + 2] *= alpha;
           }
         }
       __syncthreads();
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int g = 0; g < VG; ++g) accm[g][nt] *= sal[nt * 8 + i];
+      for (int nt = 0; nt < NT; ++nt) accm[nt] *= sal[nt * 8 + i];
     }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const float ref = mx[nt][c] == -INFINITY ? 0.f : mx[nt][c];
-        float* o = sp + (nt * 8 + 2 * j + c) * kPRow + warp * 32 + i;   // by mma row, not by key
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          const float x = fast_exp2(s[mt][nt][c] - ref), y = fast_exp2(s[mt][nt][c + 2] - ref);
-          lsum[nt][c] += x + y;
-          o[mt * 16] = x;
-          o[mt * 16 + 8] = y;
-        }
+        float* o = sp + (nt * 8 + 2 * j + c) * kPRow + warp * 16 + i;   // by mma row, not by key
+        const float x = fast_exp2(s[nt][c] - ref[nt][c]), y = fast_exp2(s[nt][c + 2] - ref[nt][c]);
+        lsum[nt][c] += x + y;
+        o[0] = x;
+        o[8] = y;
       }
     __syncthreads();
 
-    // ---- output: this warp's value groups over all keys of the tile -------------------
+    // ---- output: this warp's value dims over all keys of the tile ---------------------
 #pragma unroll 1
     for (int kt = 0; kt < kTile / 16; ++kt) {
-      float2 p0[NT], p8[NT];  // weights of row i at mma rows 2j, 2j + 1 and + 8
+      const uint32_t c0 = codes + (kt * 16 + key_0) * C::kRow + i * 4 + vg * 32;
+      const uint32_t c1 = codes + (kt * 16 + key_1) * C::kRow + i * 4 + vg * 32;
+      const uint32_t q0 = params + ((kt * 16 + key_0) * NG + vg) * 4, q1 = params + ((kt * 16 + key_1) * NG + vg) * 4;
+      const uint32_t w0 = lds32(c0), w1 = lds32(c1), w8 = lds32(c0 + 8 * C::kRow), w9 = lds32(c1 + 8 * C::kRow);
+      const uint32_t u0 = lds32(q0), u1 = lds32(q1), u8 = lds32(q0 + 8 * NG * 4), u9 = lds32(q1 + 8 * NG * 4);
+      const float s0 = bf16_lo(u0), s1 = bf16_lo(u1), s8 = bf16_lo(u8), s9 = bf16_lo(u9);
+      const float m0 = fmaf(8.f, s0, bf16_hi(u0)), m1 = fmaf(8.f, s1, bf16_hi(u1));
+      const float m8 = fmaf(8.f, s8, bf16_hi(u8)), m9 = fmaf(8.f, s9, bf16_hi(u9));
+      uint32_t bw[NT][2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int nt = 0; nt < NT; ++nt) {  // weights of row i at mma rows 2j, 2j + 1 and + 8
         const float* p = sp + (nt * 8 + i) * kPRow + kt * 16 + 2 * j;
-        p0[nt] = *reinterpret_cast<const float2*>(p);
-        p8[nt] = *reinterpret_cast<const float2*>(p + 8);
-      }
-      const uint32_t c0 = codes + (kt * 16 + key_0) * C::kRow + i * 4, c1 = codes + (kt * 16 + key_1) * C::kRow + i * 4;
-      const uint32_t q0 = params + (kt * 16 + key_0) * NG * 4, q1 = params + (kt * 16 + key_1) * NG * 4;
-#pragma unroll
-      for (int g = 0; g < VG; ++g) {
-        const int vg = warp * VG + g;
-        const uint32_t w0 = lds32(c0 + vg * 32), w1 = lds32(c1 + vg * 32);
-        const uint32_t w8 = lds32(c0 + 8 * C::kRow + vg * 32), w9 = lds32(c1 + 8 * C::kRow + vg * 32);
-        const uint32_t u0 = lds32(q0 + vg * 4), u1 = lds32(q1 + vg * 4);
-        const uint32_t u8 = lds32(q0 + (8 * NG + vg) * 4), u9 = lds32(q1 + (8 * NG + vg) * 4);
-        const float s0 = bf16_lo(u0), s1 = bf16_lo(u1), s8 = bf16_lo(u8), s9 = bf16_lo(u9);
-        const float m0 = fmaf(8.f, s0, bf16_hi(u0)), m1 = fmaf(8.f, s1, bf16_hi(u1));
-        const float m8 = fmaf(8.f, s8, bf16_hi(u8)), m9 = fmaf(8.f, s9, bf16_hi(u9));
-        uint32_t bw[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          if (masked) {  // a key that a row does not see may hold anything
-            auto times = [](float p, float x) { return p == 0.f ? 0.f : p * x; };
-            bw[nt][0] = pack_bf16x2(times(p0[nt].x, s0), times(p0[nt].y, s1));
-            bw[nt][1] = pack_bf16x2(times(p8[nt].x, s8), times(p8[nt].y, s9));
-            accm[g][nt] += times(p0[nt].x, m0) + times(p0[nt].y, m1) + times(p8[nt].x, m8) + times(p8[nt].y, m9);
-          } else {
-            bw[nt][0] = pack_bf16x2(p0[nt].x * s0, p0[nt].y * s1);
-            bw[nt][1] = pack_bf16x2(p8[nt].x * s8, p8[nt].y * s9);
-            accm[g][nt] = fmaf(p0[nt].x, m0, fmaf(p0[nt].y, m1, fmaf(p8[nt].x, m8, fmaf(p8[nt].y, m9, accm[g][nt]))));
-          }
-          mma_bf16(accr[g][nt], 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, bw[nt][0], bw[nt][1]);
+        const float2 p0 = *reinterpret_cast<const float2*>(p), p8 = *reinterpret_cast<const float2*>(p + 8);
+        float x0 = p0.x * s0, x1 = p0.y * s1, x8 = p8.x * s8, x9 = p8.y * s9;
+        if (masked) {  // a key that a row does not see may hold anything
+          auto times = [](float p, float x) { return p == 0.f ? 0.f : p * x; };
+          if (p0.x == 0.f) x0 = 0.f;
+          if (p0.y == 0.f) x1 = 0.f;
+          if (p8.x == 0.f) x8 = 0.f;
+          if (p8.y == 0.f) x9 = 0.f;
+          accm[nt] += times(p0.x, m0) + times(p0.y, m1) + times(p8.x, m8) + times(p8.y, m9);
+        } else {
+          accm[nt] = fmaf(p0.x, m0, fmaf(p0.y, m1, fmaf(p8.x, m8, fmaf(p8.y, m9, accm[nt]))));
         }
-        const uint32_t l0 = __byte_perm(w0, w1, 0x5410), h0 = __byte_perm(w0, w1, 0x7632);
-        const uint32_t l8 = __byte_perm(w8, w9, 0x5410), h8 = __byte_perm(w8, w9, 0x7632);
-        mma_values<0, NT>(acc[g][0], l0, h0, l8, h8, bw);
-        mma_values<1, NT>(acc[g][1], l0, h0, l8, h8, bw);
-        mma_values<2, NT>(acc[g][2], l0, h0, l8, h8, bw);
-        mma_values<3, NT>(acc[g][3], l0, h0, l8, h8, bw);
+        bw[nt][0] = pack_bf16x2(x0, x1);
+        bw[nt][1] = pack_bf16x2(x8, x9);
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        mma_bf16(accr[nt], 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, bw[nt][0], bw[nt][1]);
+      const uint32_t l0 = __byte_perm(w0, w1, 0x5410) >> v_shift, h0 = __byte_perm(w0, w1, 0x7632) >> v_shift;
+      const uint32_t l8 = __byte_perm(w8, w9, 0x5410) >> v_shift, h8 = __byte_perm(w8, w9, 0x7632) >> v_shift;
+      mma_values<0, NT>(acc[0], l0, h0, l8, h8, bw);
+      mma_values<1, NT>(acc[1], l0, h0, l8, h8, bw);
+      if (MM == 4) {
+        mma_values<2, NT>(acc[MM - 2], l0, h0, l8, h8, bw);
+        mma_values<3, NT>(acc[MM - 1], l0, h0, l8, h8, bw);
       }
     }
     if (tile + kStages < t1) {
@@ -379,16 +377,14 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
     }
   // sums of p (m + 8 s): lane (i, j) holds row i over the keys of j
 #pragma unroll
-  for (int g = 0; g < VG; ++g)
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float m = accm[g][nt];
-      m += __shfl_xor_sync(0xffffffffu, m, 1);
-      m += __shfl_xor_sync(0xffffffffu, m, 2);
-      if (j == 0) sp[(warp * VG + g) * kRows + nt * 8 + i] = m;
-    }
+  for (int nt = 0; nt < NT; ++nt) {
+    float m = accm[nt];
+    m += __shfl_xor_sync(0xffffffffu, m, 1);
+    m += __shfl_xor_sync(0xffffffffu, m, 2);
+    if (j == 0) sp[warp * kRows + nt * 8 + i] = m;
+  }
   __syncthreads();
-  const bool alone = t0 == 0 && step1 == piece.steps;
+  const bool alone = t0 == 0 && piece.step1 == piece.steps;
   float* part = a.part + (size_t)(2 * blockIdx.x + (t0 == 0)) * kRows * (V + 2);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
@@ -400,28 +396,25 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) l += smx[w * kRows + q];
       const float inv = !alone ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+      const float m = fmaf(-24.f, accr[nt][c], sp[warp * kRows + q]);
+      const int d = vg * 64 + 8 * i + (v_shift >> 2);
 #pragma unroll
-      for (int g = 0; g < VG; ++g) {
-        const float m = fmaf(-24.f, accr[g][nt][c], sp[(warp * VG + g) * kRows + q]);
-        float o[8];
+      for (int h = 0; h < 2; ++h) {  // dims d .. d + MM - 1, then the same 4 up
+        float o[MM];
 #pragma unroll
-        for (int mm = 0; mm < 4; ++mm) {
-          o[mm] = (acc[g][mm][nt][c] + m) * inv;
-          o[4 + mm] = (acc[g][mm][nt][c + 2] + m) * inv;
-        }
-        const int d = (warp * VG + g) * 64 + 8 * i;
+        for (int mm = 0; mm < MM; ++mm) o[mm] = (acc[mm][nt][c + 2 * h] + m) * inv;
         if (!alone) {
-          float4* p = reinterpret_cast<float4*>(part + q * V + d);
-          p[0] = make_float4(o[0], o[1], o[2], o[3]);
-          p[1] = make_float4(o[4], o[5], o[6], o[7]);
+          float* p = part + q * V + d + 4 * h;
+          if (MM == 4) *reinterpret_cast<float4*>(p) = make_float4(o[0], o[1], o[MM - 2], o[MM - 1]);
+          else *reinterpret_cast<float2*>(p) = make_float2(o[0], o[1]);
         } else {
-          *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + ((long long)b * R + row0 + q) * V + d) =
-              make_uint4(kv4_pack2<TYPE>(o[0], o[1]), kv4_pack2<TYPE>(o[2], o[3]), kv4_pack2<TYPE>(o[4], o[5]),
-                         kv4_pack2<TYPE>(o[6], o[7]));
+          uint16_t* p = reinterpret_cast<uint16_t*>(a.out) + ((long long)b * R + row0 + q) * V + d + 4 * h;
+          if (MM == 4) *reinterpret_cast<uint2*>(p) = make_uint2(kv4_pack2<TYPE>(o[0], o[1]), kv4_pack2<TYPE>(o[MM - 2], o[MM - 1]));
+          else *reinterpret_cast<uint32_t*>(p) = kv4_pack2<TYPE>(o[0], o[1]);
         }
       }
       if (!alone && warp == 0 && i == 0)
-        *reinterpret_cast<float2*>(part + kRows * V + 2 * q) = make_float2(mx[nt][c], l);
+        *reinterpret_cast<float2*>(part + kRows * V + 2 * q) = make_float2(limit[nt][c] == -INFINITY ? -INFINITY : ref[nt][c], l);
     }
   __syncthreads();  // the next segment refills shared memory
   }

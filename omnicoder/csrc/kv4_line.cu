@@ -10,49 +10,50 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// A block per query row: V / 4 threads hold four value dims each, the rest of the
-// block takes every n-th piece; pieces are summed in a fixed order.
+// A block per query row and 64 value dims: 16 threads hold four dims each, 16 such
+// groups take every 16th piece; pieces are summed in a fixed order.
+constexpr int kCols = 16, kGroups = kThreads / kCols;
+
 template <int TYPE>
 __global__ void __launch_bounds__(kThreads) kv4_combine_kernel(const Kv4Attend a, const Kv4Line line, const int rows_per_block) {
   __shared__ float4 s_sum[kThreads];
   __shared__ float2 s_ml[kThreads];
   const int G = a.H / a.Hk, R = a.Tn * G, row_blocks = line.segments / a.Hk;
   const int row = blockIdx.x % R, hk = blockIdx.x / R % a.Hk, b = blockIdx.x / R / a.Hk;
-  const int r = row % rows_per_block, cols = a.V / 4, groups = kThreads / cols;
-  const int col = threadIdx.x % cols, group = threadIdx.x / cols;
+  const int r = row % rows_per_block, group = threadIdx.x / kCols, col = blockIdx.y * kCols + threadIdx.x % kCols;
   wait_for_previous_grid();
   const int2 range = line.meta[b * line.segments + hk * row_blocks + row / rows_per_block];
   if (range.x == range.y) return;  // one block held the segment and has written the row
   const size_t slot = (size_t)rows_per_block * (a.V + 2);
   float top = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (group < groups) {
 #pragma unroll 4
-    for (int k = range.x + group; k <= range.y; k += groups) {
-      const float* p = a.part + (2 * (size_t)k + (k == range.x)) * slot;
-      const float2 ml = *reinterpret_cast<const float2*>(p + rows_per_block * a.V + 2 * r);
-      const float4 v = *reinterpret_cast<const float4*>(p + r * a.V + 4 * col);
-      const float m = fmaxf(top, ml.x), ref = m == -INFINITY ? 0.f : m;
-      const float f0 = fast_exp2(top - ref), f1 = fast_exp2(ml.x - ref);
-      l = l * f0 + ml.y * f1;
-      o.x = o.x * f0 + v.x * f1;
-      o.y = o.y * f0 + v.y * f1;
-      o.z = o.z * f0 + v.z * f1;
-      o.w = o.w * f0 + v.w * f1;
-      top = m;
-    }
+  for (int k = range.x + group; k <= range.y; k += kGroups) {
+    const float* p = a.part + (2 * (size_t)k + (k == range.x)) * slot;
+    const float2 ml = *reinterpret_cast<const float2*>(p + rows_per_block * a.V + 2 * r);
+    const float4 v = *reinterpret_cast<const float4*>(p + r * a.V + 4 * col);
+    const float m = fmaxf(top, ml.x), ref = m == -INFINITY ? 0.f : m;
+    const float f0 = fast_exp2(top - ref), f1 = fast_exp2(ml.x - ref);
+    l = l * f0 + ml.y * f1;
+    o.x = o.x * f0 + v.x * f1;
+    o.y = o.y * f0 + v.y * f1;
+    o.z = o.z * f0 + v.z * f1;
+    o.w = o.w * f0 + v.w * f1;
+    top = m;
   }
   s_sum[threadIdx.x] = o;
   s_ml[threadIdx.x] = make_float2(top, l);
   __syncthreads();
   if (group != 0) return;
-  for (int g = 1; g < groups; ++g) top = fmaxf(top, s_ml[g * cols + col].x);
+#pragma unroll
+  for (int g = 1; g < kGroups; ++g) top = fmaxf(top, s_ml[g * kCols + threadIdx.x].x);
   const float ref = top == -INFINITY ? 0.f : top;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
   l = 0.f;
-  for (int g = 0; g < groups; ++g) {
-    const float2 ml = s_ml[g * cols + col];
-    const float4 v = s_sum[g * cols + col];
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    const float2 ml = s_ml[g * kCols + threadIdx.x];
+    const float4 v = s_sum[g * kCols + threadIdx.x];
     const float f = fast_exp2(ml.x - ref);
     l = fmaf(f, ml.y, l);
     x.x = fmaf(f, v.x, x.x);
@@ -79,7 +80,7 @@ Kv4Line kv4_line(const Kv4Attend& a, const Kv4Plan& p, int tile) {
 void kv4_line_plan(const Kv4Attend& a, Kv4Plan& p, int slots, int min_steps) {
   const long long rows = a.n_sink + std::min<long long>(a.L - a.sink_rows, a.window > 0 ? (long long)a.window + a.Tn : 1 << 30);
   const long long steps = (rows + kKv4Step - 1) / kKv4Step, segments = (long long)a.B * a.Hk * p.row_blocks;
-  if (steps <= 2 || a.B > 256 || a.Tn > 16) {
+  if (steps <= 2 || a.B > kKv4MaxLine || a.Tn > 16 || segments * (steps + 1) > (1 << 30)) {
     p.min_steps = 0;
     p.blocks = (int)segments;
     p.floats = 0;
@@ -93,7 +94,7 @@ void kv4_line_plan(const Kv4Attend& a, Kv4Plan& p, int slots, int min_steps) {
 void kv4_combine(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s) {
   const Kv4Line line = kv4_line(a, p, 0);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((long long)a.B * a.Tn * a.H));
+  cfg.gridDim = dim3((unsigned)((long long)a.B * a.Tn * a.H), (unsigned)(a.V / 64));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = s;
   cudaLaunchAttribute early{};

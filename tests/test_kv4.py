@@ -304,6 +304,22 @@ def test_attention_ignores_what_it_does_not_see(H, Hk, W, latent):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,Hk,W,latent", HEADS)
+def test_attention_nan_of_one_group(H, Hk, W, latent):
+    """A NaN among the values of one group of a row: the dims of that group, of the queries that see
+    the row, and nothing else (latent rows are keys too: there the whole query)."""
+    q, kc, kp, vc, vp, q_pos, kv_len = _attend_case(2, 3, H, Hk, W, latent, 200, seed=17, lens=[150, 60])
+    kw = dict(scale=W ** -0.5, latent_v_dim=latent)
+    clean = decode_attention(q, kc, vc, q_pos, kv_len, k_scale=kp, v_scale=vp, **kw)
+    g = W // kp.shape[3]
+    (kp if latent else vp)[0, :, 149, 0] = float("nan")        # seen by the last query of sequence 0
+    out = decode_attention(q, kc, vc, q_pos, kv_len, k_scale=kp, v_scale=vp, **kw)
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    bad[0, 2, :, :(out.shape[3] if latent else g)] = True
+    assert torch.equal(torch.isnan(out), bad) and torch.equal(out[~bad], clean[~bad])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("H,Hk,W,latent", [(8, 8, 128, 0), (16, 1, 576, 512), (4, 4, 32, 0)])
 def test_attention_extreme_values(H, Hk, W, latent):
     """Scores far apart, large and tiny queries, scales of very different size, one head of zeros."""
