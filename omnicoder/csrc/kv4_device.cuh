@@ -46,11 +46,16 @@ __device__ __forceinline__ Kv4Seen kv4_seen(const Kv4Attend& a, int b, int t) {
   return s;
 }
 
-// ---- legacy tensor-core tiles on registers -----------------------------------
+// ---- tensor-core tiles on registers ---------------------------------------------
 // Codes become matrix operands in registers, straight from the 4-bit tile in
 // shared memory; tcgen05 operands would have to be written back to shared or
-// tensor memory as 16-bit tiles first, four times the bytes of the codes, for a
-// product of 8 or 16 columns that the memory-bound kernel does not wait for.
+// tensor memory as wider tiles first, for a product of 8 or 16 columns that the
+// memory-bound kernel does not wait for.
+//
+// The two low nibbles of a 16-bit half, masked out, are the fp16 subnormals n 2^-24
+// and 16 n 2^-24, which the fp16 product takes exactly: two codes per AND.  (The
+// 8-bit float product, for which a nibble in a byte would be a number as it is, is
+// no instruction of its own here: 29 cycles against 8 for the fp16 one.)
 __device__ __forceinline__ void mma_f16(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
   asm volatile(
@@ -63,6 +68,13 @@ __device__ __forceinline__ void mma_f16_zero(float* d, uint32_t a0, uint32_t a1,
                                              uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_bf16_zero(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                              uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
@@ -88,14 +100,49 @@ __device__ __forceinline__ uint32_t nibbles_bf16(uint32_t x) {
   return (y & 0x00780078u) | 0x41804180u;
 }
 
-// acc[nt] += value dims x keys (nibble MM: dims MM in the low, 4 + MM in the high halves of a
-// lane's eight) times the weights of row tile nt.
+// Weights meet value codes as x = p s f in fp16, f a power of two for which every scale s of the
+// keys at hand has s f in [2^-8, 2^6], or 0: then x < 2^14 (p < 2^8), eleven bits of it count down
+// to 2^-14, and what is lost below 2^-25 is 2^-17 of a row's largest weight.  Where the scales of
+// neighbouring keys lie further apart, x is rounded to bf16 instead (slow).
+constexpr float kKv4Low = 0.00390625f, kKv4High = 64.f;
+
+// f = 0: none yet.  A NaN or an infinity fits any f: it stays one, for the queries that see it.
+__device__ __forceinline__ bool kv4_in_range(float s, float f) {
+  return !(s * f < kKv4Low && s > 0.f) && !(s * f > kKv4High && s <= 3.4e38f);
+}
+
+// acc[mm][nt] += 16 value dims x 16 keys (nibble mm of a lane's paired words: dims mm in the low, 4 + mm
+// in the high halves of its eight) times the weights w of row tile nt.  The sums are in units of
+// 2^-24, 2^-20 for odd mm.
 template <int MM, int NT>
 __device__ __forceinline__ void mma_values(float (*acc)[4], uint32_t l0, uint32_t h0, uint32_t l8, uint32_t h8,
                                            const uint32_t (*w)[2]) {
+  constexpr uint32_t kMask = MM & 1 ? 0x00f000f0u : 0x000f000fu;
+  const uint32_t a0 = (l0 >> (MM & 2) * 4) & kMask, a1 = (h0 >> (MM & 2) * 4) & kMask;
+  const uint32_t a2 = (l8 >> (MM & 2) * 4) & kMask, a3 = (h8 >> (MM & 2) * 4) & kMask;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) mma_f16(acc[nt], a0, a1, a2, a3, w[nt][0], w[nt][1]);
+}
+
+// The same for bf16 weights, whose sum sums[nt][] over the keys is known.
+template <int MM, int NT>
+__device__ __forceinline__ void mma_values_bf16(float (*acc)[4], uint32_t l0, uint32_t h0, uint32_t l8, uint32_t h8,
+                                                const uint32_t (*w)[2], const float (*sums)[4]) {
   const uint32_t a0 = nibbles_bf16<MM>(l0), a1 = nibbles_bf16<MM>(h0), a2 = nibbles_bf16<MM>(l8), a3 = nibbles_bf16<MM>(h8);
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) mma_bf16(acc[nt], a0, a1, a2, a3, w[nt][0], w[nt][1]);
+  for (int nt = 0; nt < NT; ++nt) {
+    float d[4];
+    mma_bf16_zero(d, a0, a1, a2, a3, w[nt][0], w[nt][1]);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      acc[nt][c] = fmaf(fmaf(-16.f, sums[nt][c & 1], d[c]), MM & 1 ? 9.5367431640625e-7f : 5.9604644775390625e-8f, acc[nt][c]);
+  }
+}
+__device__ __forceinline__ float value_unit(int mm) { return mm & 1 ? 1048576.f : 16777216.f; }
+
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 __device__ __forceinline__ void kv4_cp16(uint32_t dst, const void* src) {
@@ -124,7 +171,7 @@ __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
   return v;
 }
 
-// Query rows enter the fp16 product with codes as q * 2^e, the largest |q| of the
+// Query rows enter the fp16 product with codes as q 2^e, the largest |q| of the
 // row in [2^14, 2^15): bf16 and fp16 values keep every bit down to 2^-39 of it.
 // `unscale` is 2^-e; the codes' 2^-24 is undone separately (kKv4Codes).
 constexpr float kKv4Codes = 16777216.f;
@@ -132,6 +179,35 @@ __device__ __forceinline__ float q_normaliser(float amax, float* unscale) {
   const uint32_t e = min(max((__float_as_uint(amax) >> 23) & 255u, 40u), 254u);
   *unscale = __uint_as_float((e - 14u) << 23);  // 2^(e - 127 - 14)
   return __uint_as_float((268u - e) << 23);     // 2^(14 - (e - 127))
+}
+
+// Eight dims of a normalised query, the partners of a code word: operands of two k steps (nibbles
+// 0 and 4 with 1 and 5, 2 and 6 with 3 and 7; the second pair of each counts 16-fold); -> their sum.
+__device__ __forceinline__ float query_pairs(const float* x, uint2* out) {
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const __half2 even = __floats2half2_rn(x[2 * k], x[2 * k + 4]), odd = __floats2half2_rn(x[2 * k + 1], x[2 * k + 5]);
+    const __half2 odd16 = __hmul2(odd, __float2half2_rn(0.0625f));
+    const float2 e = __half22float2(even), o = __half22float2(odd);
+    sum += (e.x + e.y) + (o.x + o.y);
+    out[k] = make_uint2(*reinterpret_cast<const uint32_t*>(&even), *reinterpret_cast<const uint32_t*>(&odd16));
+  }
+  return sum;
+}
+
+// Eight consecutive fp16 or bf16 values.
+template <int TYPE>
+__device__ __forceinline__ void kv4_load8(const void* base, long long i, float* x) {
+  const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(base) + i);
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 f = TYPE == KV4_BF16 ? make_float2(bf16_lo(u[k]), bf16_hi(u[k]))
+                                      : __half22float2(*reinterpret_cast<const __half2*>(&u[k]));
+    x[2 * k] = f.x;
+    x[2 * k + 1] = f.y;
+  }
 }
 
 // ---- work of the blocks ---------------------------------------------------------

@@ -6,7 +6,7 @@
 //   score_t = sum_g s_tg (q_g . n_tg) + m_tg sum(q_g)
 //   o_d     = sum_t (p_t s_tg) (n_td - 8) + sum_t p_t (m_tg + 8 s_tg)
 // so that the tensor cores multiply integers: the query with the codes, and the
-// weights p s (rounded to bf16, the only rounding before the output's) with the
+// weights p s (rounded to fp16, the only rounding before the output's) with the
 // codes.  The second sums stay in fp32; the weights meet n - 8 instead of n
 // because the rounding error then scales with at most 8 steps, not 15.
 //
@@ -15,12 +15,9 @@
 // tiles arrive by cp.async in a ring private to the warp, so that the loop has
 // no block-wide barrier, and the codes go from shared memory to matrix operands
 // in registers.  The 8 query rows (two tiles of 8 for up to 16) are the n side of
-// m16n8k16, 16 keys the m side of the scores, 16 value dims the m side of the
-// output: one mma for 256 codes.  Nibbles as fp16 bits are subnormals n 2^-24
-// (or n 2^-20 one nibble up), which the fp16 product takes exactly: one AND for
-// two key codes.  Value codes become bf16 16 + n by a shift and a LOP3 after a
-// byte permute has paired two keys; the constant 24 = 16 + 8 is taken out
-// through the sum of the rounded weights, an mma against ones.
+// tensor-core products, 16 keys the m side of the scores, 16 value dims the m side
+// of the output; a byte permute pairs the codes of two keys before they become
+// operands (kv4_device.cuh).
 //
 // The running maximum moves only when a score exceeds it by 2^8, which keeps
 // the shuffles and the rescaling out of most tiles.
@@ -39,7 +36,7 @@ constexpr float kSlack = 8.f;   // log2 units a score may exceed the running max
 template <int D, int NT>
 struct HeadsCfg {
   static constexpr int NG = D / 64;
-  static constexpr int kStages = NT == 1 ? 3 : 3;
+  static constexpr int kStages = 3;
   static constexpr int kRow = D / 2;
   static constexpr int kCodes = kTile * kRow;
   static constexpr int kParams = kTile * NG * 4;
@@ -63,7 +60,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
   using C = HeadsCfg<D, NT>;
   constexpr int NG = C::NG;
   extern __shared__ __align__(16) uint8_t smem[];
-  __half* sq = reinterpret_cast<__half*>(smem + C::kQ);                     // [kRows][D]
+  uint2* sq = reinterpret_cast<uint2*>(smem + C::kQ);                       // [kRows][D / 8 words][2]
   float* sqs = reinterpret_cast<float*>(smem + C::kQ + C::kRows * D * 2);   // [kRows][NG]: sum(q_g) 2^-24
   float* srs = sqs + C::kRows * NG;                                         // [kRows]: factor of the scores
   const int lane = lane_id(), warp = warp_id(), i = lane >> 2, j = lane & 3;
@@ -86,6 +83,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
   if (lane < nrows) seen = kv4_seen(a, b, (row0 + lane) / G);
   const int lo_max = __reduce_max_sync(0xffffffffu, lane < nrows ? seen.lo : 0);
   const int hi_min = __reduce_min_sync(0xffffffffu, lane < nrows ? seen.hi : a.L);
+  const int lo_min = __reduce_min_sync(0xffffffffu, lane < nrows ? seen.lo : a.L);
+  const int hi_max = __reduce_max_sync(0xffffffffu, lane < nrows ? seen.hi : 0);
   auto row_of = [&](int tile) { return (tile < sink_tiles ? tile : first + tile - sink_tiles) * kTile; };
 
   const uint8_t* kc = a.k.codes + b * a.k.c_b + hk * a.k.c_h;
@@ -122,48 +121,36 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
     next += kWarps;
   }
 
-  // ---- queries: normalised fp16 rows, group sums, score factors --------------
+  // ---- queries: normalised fp16 rows, group sums, score factors; a lane takes the eight
+  // dims of a code word ---------------------------------------------------------------------------
   for (int r = warp; r < C::kRows; r += kWarps) {
-    constexpr int kPerLane = D / 32;
-    float x[kPerLane], amax = 0.f, sum = 0.f, un;
+    constexpr int kWords = D / 8;
+    float x[8] = {}, amax = 0.f, sum = 0.f, un;
     const int row = row0 + r;
-    const long long at = (((long long)b * a.Tn + row / G) * a.H + hk * G + row % G) * D + lane * kPerLane;
+    if (r < nrows && lane < kWords)
+      kv4_load8<TYPE>(a.q, (((long long)b * a.Tn + row / G) * a.H + hk * G + row % G) * D + lane * 8, x);
 #pragma unroll
-    for (int e = 0; e < kPerLane; ++e) {
-      x[e] = r < nrows ? kv4_load1<TYPE>(a.q, at + e) : 0.f;
-      amax = fmaxf(amax, fabsf(x[e]));
-    }
+    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
     const float sc = q_normaliser(warp_max(amax), &un);
 #pragma unroll
-    for (int e = 0; e < kPerLane; ++e) {
-      const __half h = __float2half_rn(x[e] * sc);
-      sq[r * D + lane * kPerLane + e] = h;
-      sum += __half2float(h);
-    }
+    for (int e = 0; e < 8; ++e) x[e] *= sc;
+    if (lane < kWords) sum = query_pairs(x, sq + (r * kWords + lane) * 2);
 #pragma unroll
-    for (int o = 16 / NG; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane % (32 / NG) == 0) sqs[r * NG + lane / (32 / NG)] = sum * 5.9604644775390625e-8f;
+    for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane < kWords && (lane & 7) == 0) sqs[r * NG + (lane >> 3)] = sum * (1.f / kKv4Codes);
     if (lane == 0) srs[r] = un * (a.scale * (kKv4Log2e * kKv4Codes));
   }
   __syncthreads();
-  // operand of the scores: lane (i, j) holds query row i against the 16 dims that it reads of each
-  // group; dims one nibble up count 16-fold
-  uint32_t qf[NG][4][NT][2];
+  // operand of the scores: lane (i, j) holds query row i against the 16 dims that it reads of each group
+  uint2 qf[NG][4][NT];
   float qs[NG][NT][2], rs[NT][2];
   int lo[NT][2], hi[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      const __half* q = sq + (nt * 8 + i) * D + g * 64 + j * 16;
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        const __half* p = q + (ks >> 1) * 8 + (ks & 1) * 2;
-        const __half2 even = __halves2half2(p[0], p[4]), odd = __halves2half2(p[1], p[5]);
-        const __half2 odd16 = __hmul2(odd, __float2half2_rn(0.0625f));
-        qf[g][ks][nt][0] = *reinterpret_cast<const uint32_t*>(&even);
-        qf[g][ks][nt][1] = *reinterpret_cast<const uint32_t*>(&odd16);
-      }
+      for (int ks = 0; ks < 4; ++ks) qf[g][ks][nt] = sq[((nt * 8 + i) * (D / 8) + g * 8 + 2 * j) * 2 + ks];
 #pragma unroll
       for (int c = 0; c < 2; ++c) qs[g][nt][c] = sqs[(nt * 8 + 2 * j + c) * NG + g];
     }
@@ -175,6 +162,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
     }
   }
 
+  float f[NG];                     // the values' power of two; 0 before any
+#pragma unroll
+  for (int g = 0; g < NG; ++g) f[g] = 0.f;
   float acc[NG][4][NT][4], accr[NG][NT][4], accm[NG][NT][2], lsum[NT][2];
   float limit[NT][2], ref[NT][2];  // running maximum + slack, running maximum (0 before any key)
 #pragma unroll
@@ -211,6 +201,43 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
     const int r0 = row_of(tile);
     const bool masked = !(r0 + kTile <= a.n_sink || (r0 >= lo_max && r0 + kTile <= hi_min));
     uint32_t st = ring + stage * C::kStage, sp = st + 2 * C::kCodes + i * NG * 4;
+    // ---- do the scales of the tile's values fit their power of two?  Lane: key r0 + lane ----
+    bool slow[NG];
+    {
+      uint32_t v[NG];
+      load_params(st + 2 * C::kCodes + C::kParams + lane * NG * 4, v);
+      const int r = r0 + lane;
+      const bool used = !masked || r < a.n_sink || (r >= lo_min && r < hi_max);
+      bool fit = true;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        slow[g] = false;
+        fit = fit && (!used || kv4_in_range(bf16_lo(v[g]), f[g]));
+      }
+      if (!__all_sync(0xffffffffu, fit)) {
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const float sc = bf16_lo(v[g]);
+          const uint32_t e = __reduce_max_sync(0xffffffffu, used && sc <= 3.4e38f ? __float_as_uint(sc) >> 23 : 0u);
+          if (e > 0) {  // largest scale in [2^3, 2^4); sums made before move along
+            const float now = __uint_as_float(min(257u - e, 254u) << 23);
+            const float move = f[g] == 0.f ? 0.f : now / f[g];
+            if (f[g] == 0.f || (move >= 8.67e-19f && move <= 1.15e18f)) {
+              f[g] = now;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                  accr[g][nt][c] *= move;
+#pragma unroll
+                  for (int mm = 0; mm < 4; ++mm) acc[g][mm][nt][c] *= move;
+                }
+            }
+          }
+          slow[g] = !__all_sync(0xffffffffu, !used || kv4_in_range(sc, f[g]));
+        }
+      }
+    }
     // Rolled: the loop's code must stay in the instruction cache next to the scheduler.
 #pragma unroll 1
     for (int r = r0 + i; r < r0 + kTile; r += 16, st += 16 * C::kRow, sp += 16 * NG * 4) {
@@ -229,8 +256,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
           const uint32_t a0 = xa & 0x000f000fu, a1 = xb & 0x000f000fu, a2 = xa & 0x00f000f0u, a3 = xb & 0x00f000f0u;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            if (ks == 0) mma_f16_zero(d[nt], a0, a1, a2, a3, qf[g][ks][nt][0], qf[g][ks][nt][1]);
-            else mma_f16(d[nt], a0, a1, a2, a3, qf[g][ks][nt][0], qf[g][ks][nt][1]);
+            const uint2 q = qf[g][ks][nt];
+            if (ks == 0) mma_f16_zero(d[nt], a0, a1, a2, a3, q.x, q.y);
+            else mma_f16(d[nt], a0, a1, a2, a3, q.x, q.y);
           }
         }
         const float sa = bf16_lo(pa[g]), ma = bf16_hi(pa[g]), sb = bf16_lo(pb[g]), mb = bf16_hi(pb[g]);
@@ -307,34 +335,54 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
       for (int g = 0; g < NG; ++g) {
         const float sa = bf16_lo(pa[g]), sb = bf16_lo(pb[g]);
         const float ca = fmaf(8.f, sa, bf16_hi(pa[g])), cb = fmaf(8.f, sb, bf16_hi(pb[g]));
-        uint32_t bw[NT][2];
+        float x[NT][4];
+        const float fa = sa * f[g], fb = sb * f[g];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float x[4];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) x[c] = s[nt][c] * (c < 2 ? sa : sb);
+          for (int c = 0; c < 4; ++c) x[nt][c] = s[nt][c] * (c < 2 ? fa : fb);
           if (masked) {  // a key that a row does not see may hold anything
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              if (s[nt][c] == 0.f) x[c] = 0.f;
+              if (s[nt][c] == 0.f) x[nt][c] = 0.f;
               else accm[g][nt][c & 1] = fmaf(s[nt][c], c < 2 ? ca : cb, accm[g][nt][c & 1]);
             }
           } else {
 #pragma unroll
             for (int c = 0; c < 4; ++c) accm[g][nt][c & 1] = fmaf(s[nt][c], c < 2 ? ca : cb, accm[g][nt][c & 1]);
           }
-          bw[nt][0] = movmatrix_trans(pack_bf16x2(x[0], x[1]));
-          bw[nt][1] = movmatrix_trans(pack_bf16x2(x[2], x[3]));
-          mma_bf16(accr[g][nt], 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, bw[nt][0], bw[nt][1]);
         }
         const uint32_t w0 = lds32(st + v_at0[g]), w1 = lds32(st + v_at1[g]);
         const uint32_t w8 = lds32(st + v_at0[g] + 8 * C::kRow), w9 = lds32(st + v_at1[g] + 8 * C::kRow);
         const uint32_t l0 = __byte_perm(w0, w1, 0x5410), h0 = __byte_perm(w0, w1, 0x7632);
         const uint32_t l8 = __byte_perm(w8, w9, 0x5410), h8 = __byte_perm(w8, w9, 0x7632);
-        mma_values<0, NT>(acc[g][0], l0, h0, l8, h8, bw);
-        mma_values<1, NT>(acc[g][1], l0, h0, l8, h8, bw);
-        mma_values<2, NT>(acc[g][2], l0, h0, l8, h8, bw);
-        mma_values<3, NT>(acc[g][3], l0, h0, l8, h8, bw);
+        uint32_t bw[NT][2];
+        if (!slow[g]) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            bw[nt][0] = movmatrix_trans(pack_f16x2(x[nt][0], x[nt][1]));
+            bw[nt][1] = movmatrix_trans(pack_f16x2(x[nt][2], x[nt][3]));
+            mma_f16(accr[g][nt], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, bw[nt][0], bw[nt][1]);
+          }
+          mma_values<0, NT>(acc[g][0], l0, h0, l8, h8, bw);
+          mma_values<1, NT>(acc[g][1], l0, h0, l8, h8, bw);
+          mma_values<2, NT>(acc[g][2], l0, h0, l8, h8, bw);
+          mma_values<3, NT>(acc[g][3], l0, h0, l8, h8, bw);
+        } else {
+          float sums[NT][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            bw[nt][0] = movmatrix_trans(pack_bf16x2(x[nt][0], x[nt][1]));
+            bw[nt][1] = movmatrix_trans(pack_bf16x2(x[nt][2], x[nt][3]));
+            mma_bf16_zero(sums[nt], 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, bw[nt][0], bw[nt][1]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) accr[g][nt][c] += sums[nt][c];
+          }
+          mma_values_bf16<0, NT>(acc[g][0], l0, h0, l8, h8, bw, sums);
+          mma_values_bf16<1, NT>(acc[g][1], l0, h0, l8, h8, bw, sums);
+          mma_values_bf16<2, NT>(acc[g][2], l0, h0, l8, h8, bw, sums);
+          mma_values_bf16<3, NT>(acc[g][3], l0, h0, l8, h8, bw, sums);
+        }
       }
     }
     stage = stage + 1 == C::kStages ? 0 : stage + 1;
@@ -362,12 +410,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
         float m = accm[g][nt][c];
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
-        m = fmaf(-24.f, accr[g][nt][c], m);
+        const float unit = f[g] == 0.f ? 0.f : 1.f / f[g];
+        m = fmaf(-8.f * unit, accr[g][nt][c], m);
         float* o = so + r * D + g * 64 + 8 * i;
 #pragma unroll
         for (int mm = 0; mm < 4; ++mm) {
-          o[mm] = acc[g][mm][nt][c] + m;
-          o[4 + mm] = acc[g][mm][nt][c + 2] + m;
+          o[mm] = fmaf(acc[g][mm][nt][c], unit * value_unit(mm), m);
+          o[4 + mm] = fmaf(acc[g][mm][nt][c + 2], unit * value_unit(mm), m);
         }
       }
     }

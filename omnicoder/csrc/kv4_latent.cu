@@ -39,7 +39,7 @@ struct LatentCfg {
   static constexpr int kCodes = kTile * kRow;
   static constexpr int kParams = kTile * NG * 4;
   static constexpr int kStage = kCodes + kParams;
-  static constexpr int kQf = kStages * kStage;       // query operands [NG * 4][32 lanes][4]
+  static constexpr int kQf = kStages * kStage;       // query operands [NG * 4 k steps][32 lanes][row tile]
   static constexpr int kP = kQf + NG * 4 * 32 * 16;  // weights [kRows][kPRow]
   static constexpr int kMisc = kP + kRows * kPRow * 4;  // sums of q, factors, maxima, barriers
   static constexpr int kSmem = kMisc + kRows * (16 + 1 + kWarps + 1) * 4 + kRows * 2 * 4 + kStages * 8;
@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
   using C = LatentCfg<V>;
   constexpr int W = C::W, NG = C::NG, MM = C::MM;
   extern __shared__ __align__(128) uint8_t smem[];
-  uint32_t* sqf = reinterpret_cast<uint32_t*>(smem + C::kQf);
+  uint2* sqf = reinterpret_cast<uint2*>(smem + C::kQf);
   float* sp = reinterpret_cast<float*>(smem + C::kP);
   float* sqs = reinterpret_cast<float*>(smem + C::kMisc);  // [kRows][16]: sum(q_g) 2^-24, zero from NG on
   float* srs = sqs + kRows * 16;                           // [kRows]: factor of the scores
@@ -81,6 +81,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
   if (lane < nrows) seen = kv4_seen(a, b, (row0 + lane) / a.H);
   const int lo_max = __reduce_max_sync(0xffffffffu, lane < nrows ? seen.lo : 0);
   const int hi_min = __reduce_min_sync(0xffffffffu, lane < nrows ? seen.hi : a.L);
+  const int lo_min = __reduce_min_sync(0xffffffffu, lane < nrows ? seen.lo : a.L);
+  const int hi_max = __reduce_max_sync(0xffffffffu, lane < nrows ? seen.hi : 0);
   auto row_of = [&](int tile) { return (tile < sink_tiles ? tile : first + tile - sink_tiles) * kTile; };
 
   const uint8_t* kc = a.k.codes + b * a.k.c_b;
@@ -97,52 +99,37 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
     for (int k = 0; k < kStages; ++k)
       if (t0 + k < t1) issue(t0 + k, (used + k) % kStages);
 
-  // ---- queries: normalised fp16, laid out as the operands of the scores.  A lane takes the eight
-  // dims of a code word, whose nibble pairs (0, 4), (1, 5), (2, 6), (3, 7) are two k steps.
+  // ---- queries: normalised fp16, laid out as the operands of the scores; a lane takes
+  // the eight dims of a code word -------------------------------------------------------------------
   for (int r = warp; r < kRows; r += kWarps) {
     constexpr int kWords = W / 8, kPer = (kWords + 31) / 32;
-    float amax = 0.f, un;
-    uint4 raw[kPer];
-    float x[kPer][8];
+    float x[kPer][8] = {}, amax = 0.f, un;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
       const int w = lane + 32 * e;
-      raw[e] = make_uint4(0, 0, 0, 0);
-      if (r < nrows && w < kWords)
-        raw[e] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.q) + ((long long)b * R + row0 + r) * W + w * 8);
+      if (r < nrows && w < kWords) kv4_load8<TYPE>(a.q, ((long long)b * R + row0 + r) * W + w * 8, x[e]);
     }
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      const uint32_t u[4] = {raw[e].x, raw[e].y, raw[e].z, raw[e].w};
+    for (int e = 0; e < kPer; ++e)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 f = TYPE == KV4_BF16 ? make_float2(bf16_lo(u[k]), bf16_hi(u[k])) : __half22float2(*reinterpret_cast<const __half2*>(&u[k]));
-        x[e][2 * k] = f.x;
-        x[e][2 * k + 1] = f.y;
-        amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
-      }
-    }
+      for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(x[e][k]));
     const float sc = q_normaliser(warp_max(amax), &un);
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-      const int w = lane + 32 * e, g = w >> 3, jj = (w >> 1) & 3;
+      const int w = lane + 32 * e, g = w >> 3;
       float sum = 0.f;
       if (w < kWords) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const __half2 even = __floats2half2_rn(x[e][2 * k] * sc, x[e][2 * k + 4] * sc);
-          const __half2 odd = __floats2half2_rn(x[e][2 * k + 1] * sc, x[e][2 * k + 5] * sc);
-          const __half2 odd16 = __hmul2(odd, __float2half2_rn(0.0625f));
-          const float2 fe = __half22float2(even), fo = __half22float2(odd);
-          sum += (fe.x + fe.y) + (fo.x + fo.y);
-          // [g, ks][lane (r & 7, jj)][row tile, even / odd nibbles]
-          *reinterpret_cast<uint2*>(sqf + ((g * 4 + (w & 1) * 2 + k) * 32 + (r & 7) * 4 + jj) * 4 + (r >> 3) * 2) =
-              make_uint2(*reinterpret_cast<const uint32_t*>(&even), *reinterpret_cast<const uint32_t*>(&odd16));
-        }
+        for (int k = 0; k < 8; ++k) x[e][k] *= sc;
+        uint2 q[2];
+        sum = query_pairs(x[e], q);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          sqf[((g * 4 + (w & 1) * 2 + k) * 32 + (r & 7) * 4 + ((w >> 1) & 3)) * NT + (r >> 3)] = q[k];
       }
 #pragma unroll
       for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if ((lane & 7) == 0 && g < 16) sqs[r * 16 + g] = w < kWords ? sum * 5.9604644775390625e-8f : 0.f;
+      if ((lane & 7) == 0 && g < 16) sqs[r * 16 + g] = w < kWords ? sum * (1.f / kKv4Codes) : 0.f;
     }
     if (lane >= kPer * 4 && lane < 16) sqs[r * 16 + lane] = 0.f;
     if (lane == 0) srs[r] = un * (a.scale * (kKv4Log2e * kKv4Codes));
@@ -175,6 +162,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
 
   // acc: a value tile holds dims MM and 4 + MM of a lane's eight; accr: sums of the rounded weights;
   // accm: sums of p (m + 8 s)
+  float f = 0.f;   // the values' power of two; 0 before any
   float acc[MM][NT][4], accr[NT][4], accm[NT], lsum[NT][2], limit[NT][2], ref[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -225,7 +213,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
       float d[NT][4];
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
-        const uint4 q = *reinterpret_cast<const uint4*>(sqf + ((g * 4 + ks) * 32 + lane) * 4);
+        const uint4 q = *reinterpret_cast<const uint4*>(sqf + ((g * 4 + ks) * 32 + lane) * NT);
         const uint32_t xa = (ks < 2 ? wa.x : wa.y) >> ((ks & 1) * 8), xb = (ks < 2 ? wb.x : wb.y) >> ((ks & 1) * 8);
         const uint32_t a0 = xa & 0x000f000fu, a1 = xb & 0x000f000fu, a2 = xa & 0x00f000f0u, a3 = xb & 0x00f000f0u;
         if (ks == 0) {
@@ -315,6 +303,45 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
       }
     __syncthreads();
 
+    // ---- do the scales of the tile's values fit their power of two?  Lane: keys lane + 32 k ----
+    bool slow = false;
+    {
+      float sc[kTile / 32];
+      bool used[kTile / 32], fit = true;
+#pragma unroll
+      for (int k = 0; k < kTile / 32; ++k) {
+        const int r = lane + 32 * k;
+        sc[k] = bf16_lo(lds32(params + (r * NG + vg) * 4));
+        used[k] = !masked || r0 + r < a.n_sink || (r0 + r >= lo_min && r0 + r < hi_max);
+        fit = fit && (!used[k] || kv4_in_range(sc[k], f));
+      }
+      if (!__all_sync(0xffffffffu, fit)) {
+        uint32_t e = 0;
+#pragma unroll
+        for (int k = 0; k < kTile / 32; ++k)
+          if (used[k] && sc[k] <= 3.4e38f) e = max(e, __float_as_uint(sc[k]) >> 23);
+        e = __reduce_max_sync(0xffffffffu, e);
+        if (e > 0) {  // largest scale in [2^3, 2^4); sums made before move along
+          const float now = __uint_as_float(min(257u - e, 254u) << 23);
+          const float move = f == 0.f ? 0.f : now / f;
+          if (f == 0.f || (move >= 8.67e-19f && move <= 1.15e18f)) {
+            f = now;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                accr[nt][c] *= move;
+#pragma unroll
+                for (int mm = 0; mm < MM; ++mm) acc[mm][nt][c] *= move;
+              }
+          }
+        }
+        fit = true;
+#pragma unroll
+        for (int k = 0; k < kTile / 32; ++k) fit = fit && (!used[k] || kv4_in_range(sc[k], f));
+        slow = !__all_sync(0xffffffffu, fit);
+      }
+    }
     // ---- output: this warp's value dims over all keys of the tile ---------------------
 #pragma unroll 1
     for (int kt = 0; kt < kTile / 16; ++kt) {
@@ -326,35 +353,60 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
       const float s0 = bf16_lo(u0), s1 = bf16_lo(u1), s8 = bf16_lo(u8), s9 = bf16_lo(u9);
       const float m0 = fmaf(8.f, s0, bf16_hi(u0)), m1 = fmaf(8.f, s1, bf16_hi(u1));
       const float m8 = fmaf(8.f, s8, bf16_hi(u8)), m9 = fmaf(8.f, s9, bf16_hi(u9));
-      uint32_t bw[NT][2];
+      const float f0 = s0 * f, f1 = s1 * f, f8 = s8 * f, f9 = s9 * f;
+      float x[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {  // weights of row i at mma rows 2j, 2j + 1 and + 8
         const float* p = sp + (nt * 8 + i) * kPRow + kt * 16 + 2 * j;
         const float2 p0 = *reinterpret_cast<const float2*>(p), p8 = *reinterpret_cast<const float2*>(p + 8);
-        float x0 = p0.x * s0, x1 = p0.y * s1, x8 = p8.x * s8, x9 = p8.y * s9;
+        x[nt][0] = p0.x * f0;
+        x[nt][1] = p0.y * f1;
+        x[nt][2] = p8.x * f8;
+        x[nt][3] = p8.y * f9;
         if (masked) {  // a key that a row does not see may hold anything
           auto times = [](float p, float x) { return p == 0.f ? 0.f : p * x; };
-          if (p0.x == 0.f) x0 = 0.f;
-          if (p0.y == 0.f) x1 = 0.f;
-          if (p8.x == 0.f) x8 = 0.f;
-          if (p8.y == 0.f) x9 = 0.f;
+          if (p0.x == 0.f) x[nt][0] = 0.f;
+          if (p0.y == 0.f) x[nt][1] = 0.f;
+          if (p8.x == 0.f) x[nt][2] = 0.f;
+          if (p8.y == 0.f) x[nt][3] = 0.f;
           accm[nt] += times(p0.x, m0) + times(p0.y, m1) + times(p8.x, m8) + times(p8.y, m9);
         } else {
           accm[nt] = fmaf(p0.x, m0, fmaf(p0.y, m1, fmaf(p8.x, m8, fmaf(p8.y, m9, accm[nt]))));
         }
-        bw[nt][0] = pack_bf16x2(x0, x1);
-        bw[nt][1] = pack_bf16x2(x8, x9);
       }
+      uint32_t l0 = __byte_perm(w0, w1, 0x5410), h0 = __byte_perm(w0, w1, 0x7632);
+      uint32_t l8 = __byte_perm(w8, w9, 0x5410), h8 = __byte_perm(w8, w9, 0x7632);
+      if (MM == 2) l0 >>= v_shift, h0 >>= v_shift, l8 >>= v_shift, h8 >>= v_shift;
+      uint32_t bw[NT][2];
+      if (!slow) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        mma_bf16(accr[nt], 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, bw[nt][0], bw[nt][1]);
-      const uint32_t l0 = __byte_perm(w0, w1, 0x5410) >> v_shift, h0 = __byte_perm(w0, w1, 0x7632) >> v_shift;
-      const uint32_t l8 = __byte_perm(w8, w9, 0x5410) >> v_shift, h8 = __byte_perm(w8, w9, 0x7632) >> v_shift;
-      mma_values<0, NT>(acc[0], l0, h0, l8, h8, bw);
-      mma_values<1, NT>(acc[1], l0, h0, l8, h8, bw);
-      if (MM == 4) {
-        mma_values<2, NT>(acc[MM - 2], l0, h0, l8, h8, bw);
-        mma_values<3, NT>(acc[MM - 1], l0, h0, l8, h8, bw);
+        for (int nt = 0; nt < NT; ++nt) {
+          bw[nt][0] = pack_f16x2(x[nt][0], x[nt][1]);
+          bw[nt][1] = pack_f16x2(x[nt][2], x[nt][3]);
+          mma_f16(accr[nt], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, bw[nt][0], bw[nt][1]);
+        }
+        mma_values<0, NT>(acc[0], l0, h0, l8, h8, bw);
+        mma_values<1, NT>(acc[1], l0, h0, l8, h8, bw);
+        if (MM == 4) {
+          mma_values<2, NT>(acc[MM - 2], l0, h0, l8, h8, bw);
+          mma_values<3, NT>(acc[MM - 1], l0, h0, l8, h8, bw);
+        }
+      } else {
+        float sums[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          bw[nt][0] = pack_bf16x2(x[nt][0], x[nt][1]);
+          bw[nt][1] = pack_bf16x2(x[nt][2], x[nt][3]);
+          mma_bf16_zero(sums[nt], 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, bw[nt][0], bw[nt][1]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) accr[nt][c] += sums[nt][c];
+        }
+        mma_values_bf16<0, NT>(acc[0], l0, h0, l8, h8, bw, sums);
+        mma_values_bf16<1, NT>(acc[1], l0, h0, l8, h8, bw, sums);
+        if (MM == 4) {
+          mma_values_bf16<2, NT>(acc[MM - 2], l0, h0, l8, h8, bw, sums);
+          mma_values_bf16<3, NT>(acc[MM - 1], l0, h0, l8, h8, bw, sums);
+        }
       }
     }
     if (tile + kStages < t1) {
@@ -396,13 +448,14 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) l += smx[w * kRows + q];
       const float inv = !alone ? 1.f : (l == 0.f ? 0.f : 1.f / l);
-      const float m = fmaf(-24.f, accr[nt][c], sp[warp * kRows + q]);
+      const float unit = f == 0.f ? 0.f : 1.f / f;
+      const float m = fmaf(-8.f * unit, accr[nt][c], sp[warp * kRows + q]);
       const int d = vg * 64 + 8 * i + (v_shift >> 2);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {  // dims d .. d + MM - 1, then the same 4 up
         float o[MM];
 #pragma unroll
-        for (int mm = 0; mm < MM; ++mm) o[mm] = (acc[mm][nt][c + 2 * h] + m) * inv;
+        for (int mm = 0; mm < MM; ++mm) o[mm] = fmaf(acc[mm][nt][c + 2 * h], unit * value_unit(mm), m) * inv;
         if (!alone) {
           float* p = part + q * V + d + 4 * h;
           if (MM == 4) *reinterpret_cast<float4*>(p) = make_float4(o[0], o[1], o[MM - 2], o[MM - 1]);

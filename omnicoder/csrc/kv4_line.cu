@@ -10,50 +10,54 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// A block per query row and 64 value dims: 16 threads hold four dims each, 16 such
-// groups take every 16th piece; pieces are summed in a fixed order.
-constexpr int kCols = 16, kGroups = kThreads / kCols;
-
-template <int TYPE>
+// A thread holds four value dims of a query row; GROUPS threads take every GROUPS-th
+// piece each and are summed in a fixed order.
+template <int TYPE, int GROUPS>
 __global__ void __launch_bounds__(kThreads) kv4_combine_kernel(const Kv4Attend a, const Kv4Line line, const int rows_per_block) {
+  constexpr int kItems = kThreads / GROUPS;
   __shared__ float4 s_sum[kThreads];
   __shared__ float2 s_ml[kThreads];
-  const int G = a.H / a.Hk, R = a.Tn * G, row_blocks = line.segments / a.Hk;
-  const int row = blockIdx.x % R, hk = blockIdx.x / R % a.Hk, b = blockIdx.x / R / a.Hk;
-  const int r = row % rows_per_block, group = threadIdx.x / kCols, col = blockIdx.y * kCols + threadIdx.x % kCols;
+  const int G = a.H / a.Hk, R = a.Tn * G, row_blocks = line.segments / a.Hk, cols = a.V / 4;
+  const int item = threadIdx.x % kItems, group = threadIdx.x / kItems;
+  const long long at = (long long)blockIdx.x * kItems + item, total = (long long)a.B * a.Hk * R * cols;
+  const int col = (int)(at % cols), place = (int)(at / cols);
+  const int row = place % R, hk = place / R % a.Hk, b = place / R / a.Hk, r = row % rows_per_block;
   wait_for_previous_grid();
-  const int2 range = line.meta[b * line.segments + hk * row_blocks + row / rows_per_block];
-  if (range.x == range.y) return;  // one block held the segment and has written the row
+  int2 range = make_int2(0, 0);
+  if (at < total) range = line.meta[b * line.segments + hk * row_blocks + row / rows_per_block];
+  const bool join = range.x != range.y;  // otherwise one block held the segment and has written the row
   const size_t slot = (size_t)rows_per_block * (a.V + 2);
   float top = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (join) {
 #pragma unroll 4
-  for (int k = range.x + group; k <= range.y; k += kGroups) {
-    const float* p = a.part + (2 * (size_t)k + (k == range.x)) * slot;
-    const float2 ml = *reinterpret_cast<const float2*>(p + rows_per_block * a.V + 2 * r);
-    const float4 v = *reinterpret_cast<const float4*>(p + r * a.V + 4 * col);
-    const float m = fmaxf(top, ml.x), ref = m == -INFINITY ? 0.f : m;
-    const float f0 = fast_exp2(top - ref), f1 = fast_exp2(ml.x - ref);
-    l = l * f0 + ml.y * f1;
-    o.x = o.x * f0 + v.x * f1;
-    o.y = o.y * f0 + v.y * f1;
-    o.z = o.z * f0 + v.z * f1;
-    o.w = o.w * f0 + v.w * f1;
-    top = m;
+    for (int k = range.x + group; k <= range.y; k += GROUPS) {
+      const float* p = a.part + (2 * (size_t)k + (k == range.x)) * slot;
+      const float2 ml = *reinterpret_cast<const float2*>(p + rows_per_block * a.V + 2 * r);
+      const float4 v = *reinterpret_cast<const float4*>(p + r * a.V + 4 * col);
+      const float m = fmaxf(top, ml.x), ref = m == -INFINITY ? 0.f : m;
+      const float f0 = fast_exp2(top - ref), f1 = fast_exp2(ml.x - ref);
+      l = l * f0 + ml.y * f1;
+      o.x = o.x * f0 + v.x * f1;
+      o.y = o.y * f0 + v.y * f1;
+      o.z = o.z * f0 + v.z * f1;
+      o.w = o.w * f0 + v.w * f1;
+      top = m;
+    }
   }
   s_sum[threadIdx.x] = o;
   s_ml[threadIdx.x] = make_float2(top, l);
   __syncthreads();
-  if (group != 0) return;
+  if (group != 0 || !join) return;
 #pragma unroll
-  for (int g = 1; g < kGroups; ++g) top = fmaxf(top, s_ml[g * kCols + threadIdx.x].x);
+  for (int g = 1; g < GROUPS; ++g) top = fmaxf(top, s_ml[g * kItems + item].x);
   const float ref = top == -INFINITY ? 0.f : top;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
   l = 0.f;
 #pragma unroll
-  for (int g = 0; g < kGroups; ++g) {
-    const float2 ml = s_ml[g * kCols + threadIdx.x];
-    const float4 v = s_sum[g * kCols + threadIdx.x];
+  for (int g = 0; g < GROUPS; ++g) {
+    const float2 ml = s_ml[g * kItems + item];
+    const float4 v = s_sum[g * kItems + item];
     const float f = fast_exp2(ml.x - ref);
     l = fmaf(f, ml.y, l);
     x.x = fmaf(f, v.x, x.x);
@@ -65,6 +69,21 @@ __global__ void __launch_bounds__(kThreads) kv4_combine_kernel(const Kv4Attend a
   const float inv = l == 0.f ? 0.f : 1.f / l;
   *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + head * a.V + 4 * col) =
       make_uint2(kv4_pack2<TYPE>(x.x * inv, x.y * inv), kv4_pack2<TYPE>(x.z * inv, x.w * inv));
+}
+
+template <int TYPE, int GROUPS>
+void launch(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s) {
+  const long long items = (long long)a.B * a.Tn * a.H * (a.V / 4), per = kThreads / GROUPS;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((items + per - 1) / per));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kv4_combine_kernel<TYPE, GROUPS>, a, kv4_line(a, p, 0), 8 * p.row_tiles);
 }
 
 }  // namespace
@@ -92,18 +111,11 @@ void kv4_line_plan(const Kv4Attend& a, Kv4Plan& p, int slots, int min_steps) {
 }
 
 void kv4_combine(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s) {
-  const Kv4Line line = kv4_line(a, p, 0);
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((long long)a.B * a.Tn * a.H), (unsigned)(a.V / 64));
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = s;
-  cudaLaunchAttribute early{};
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &early;
-  cfg.numAttrs = 1;
-  if (a.type == KV4_F16) cudaLaunchKernelEx(&cfg, kv4_combine_kernel<KV4_F16>, a, line, 8 * p.row_tiles);
-  else cudaLaunchKernelEx(&cfg, kv4_combine_kernel<KV4_BF16>, a, line, 8 * p.row_tiles);
+  // a segment has about blocks / segments + 1 pieces
+  const long long segments = (long long)a.B * a.Hk * p.row_blocks;
+  const bool many = p.blocks > 6 * segments;
+  if (a.type == KV4_F16) many ? launch<KV4_F16, 16>(a, p, s) : launch<KV4_F16, 2>(a, p, s);
+  else many ? launch<KV4_BF16, 16>(a, p, s) : launch<KV4_BF16, 2>(a, p, s);
 }
 
 }  // namespace omni
