@@ -221,11 +221,22 @@ __device__ __forceinline__ void kv4_load8(const void* base, long long i, float* 
 // segment notes its first and last block for the kernel that joins them.
 constexpr int kKv4Step = 128;
 
+// n / d for 0 <= n < 2^31 as a multiplication.
+struct Kv4Div {
+  int d;
+  uint32_t mul, shift;
+  explicit Kv4Div(int n) : d(n), mul(0), shift(0) {  // mul = ceil(2^(32 + shift) / d), shift = ceil(log2 d) - 1
+    while ((2ull << shift) < (unsigned long long)d) ++shift;
+    if (d > 1) mul = (uint32_t)(((1ull << (32 + shift)) + d - 1) / d);
+  }
+  __device__ __forceinline__ int of(int n) const { return d == 1 ? n : (int)(__umulhi((uint32_t)n, mul) >> shift); }
+};
+
 struct Kv4Line {
-  int segments;    // of one sequence: Hk * row_blocks
-  int tile;        // rows per tile: 32 (four warps a step) or 128
-  int min_steps;   // smallest share of a block; 0: a block per segment
-  int2* meta;      // [B * segments] first and last block
+  Kv4Div segments;    // of one sequence: Hk * row_blocks
+  Kv4Div row_blocks, group, rows;  // row blocks of a head, heads that share one, query rows of it: Tn * group
+  int min_steps;      // smallest share of a block; 0: a block per segment
+  int2* meta;         // [B * segments] first and last block
 };
 
 constexpr int kKv4MaxLine = 256;   // sequences on a line
@@ -236,10 +247,10 @@ struct Kv4Piece {
   int sink_tiles, first, tiles;    // tiles over the memory rows; first tile behind them; all
 };
 
-// Rows [lo, hi) that any of the queries t0, t0 + stride, .. < t1 sees.
-__device__ __forceinline__ Kv4Seen kv4_union(const Kv4Attend& a, int b, int t0, int t1, int stride) {
+// Rows [lo, hi) that any query of a sequence sees.
+__device__ __forceinline__ Kv4Seen kv4_union(const Kv4Attend& a, int b) {
   Kv4Seen u{a.L, 0};
-  for (int t = t0; t < t1; t += stride) {
+  for (int t = 0; t < a.Tn; ++t) {
     const Kv4Seen s = kv4_seen(a, b, t);
     if (s.hi > s.lo) {
       u.lo = min(u.lo, s.lo);
@@ -249,12 +260,13 @@ __device__ __forceinline__ Kv4Seen kv4_union(const Kv4Attend& a, int b, int t0, 
   return u;
 }
 
-__device__ __forceinline__ void kv4_tiles(const Kv4Attend& a, Kv4Seen u, int tile, Kv4Piece* p) {
-  p->sink_tiles = (a.n_sink + tile - 1) / tile;
-  p->first = max(u.lo / tile, p->sink_tiles);
-  p->tiles = p->sink_tiles + max(0, u.hi > u.lo ? (u.hi + tile - 1) / tile - p->first : 0);
-  const int per_step = kKv4Step / tile;
-  p->steps = max(1, (p->tiles + per_step - 1) / per_step);  // a sequence that sees nothing still writes zeros
+template <int kTile>
+__device__ __forceinline__ void kv4_tiles(const Kv4Attend& a, Kv4Seen u, Kv4Piece* p) {
+  p->sink_tiles = (a.n_sink + kTile - 1) / kTile;
+  p->first = max(u.lo / kTile, p->sink_tiles);
+  p->tiles = p->sink_tiles + max(0, u.hi > u.lo ? (u.hi + kTile - 1) / kTile - p->first : 0);
+  constexpr int kPerStep = kKv4Step / kTile;
+  p->steps = max(1, (p->tiles + kPerStep - 1) / kPerStep);  // a sequence that sees nothing still writes zeros
 }
 
 // The pieces of one block, in turn; every thread of the block calls both functions.
@@ -263,7 +275,7 @@ struct Kv4Walk {
   int end[kKv4MaxLine], first[kKv4MaxLine], tiles[kKv4MaxLine], sums[32];
 
   // -> first and last step of the block on the line
-  template <int kThreads>
+  template <int kThreads, int kTile>
   __device__ __forceinline__ int2 begin(const Kv4Attend& a, const Kv4Line& l, int* share) {
     if (l.min_steps == 0) return make_int2(0, 1);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -271,7 +283,7 @@ struct Kv4Walk {
     for (int b0 = 0; b0 < a.B; b0 += kThreads) {
       Kv4Piece q;
       q.steps = 0;
-      if (b0 + tid < a.B) kv4_tiles(a, kv4_union(a, b0 + tid, 0, a.Tn, 1), l.tile, &q);
+      if (b0 + tid < a.B) kv4_tiles<kTile>(a, kv4_union(a, b0 + tid), &q);
       int sum = q.steps;  // inclusive prefix over the threads
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -294,32 +306,27 @@ struct Kv4Walk {
       before = all;
       __syncthreads();
     }
-    const int total = before * l.segments;
+    const int total = before * l.segments.d;
     *share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, l.min_steps);
     const int at = blockIdx.x * *share;
     return make_int2(at, min(total, at + *share));
   }
 
-  // The segment that holds step span.x; moves span.x behind it.
-  __device__ __forceinline__ Kv4Piece next(const Kv4Attend& a, const Kv4Line& l, int rows_per_block, int share, int2* span) {
+  // The segment that holds step span.x; moves span.x behind it.  A block per segment: tiles and
+  // steps are left to kv4_tiles() of the rows that its queries see.
+  template <int kTile>
+  __device__ __forceinline__ Kv4Piece next(const Kv4Attend& a, const Kv4Line& l, int share, int2* span) {
     Kv4Piece p;
     if (l.min_steps == 0) {
-      p.b = blockIdx.x / l.segments;
-      p.segment = blockIdx.x % l.segments;
-      const int G = a.H / a.Hk, row0 = p.segment % (l.segments / a.Hk) * rows_per_block;
-      const int t0 = row0 / G, t1 = (min(row0 + rows_per_block, a.Tn * G) - 1) / G + 1;
-      Kv4Seen u = kv4_union(a, p.b, t0 + lane_id(), t1, 32);
-      u.lo = __reduce_min_sync(0xffffffffu, u.lo);
-      u.hi = __reduce_max_sync(0xffffffffu, u.hi);
-      kv4_tiles(a, u, l.tile, &p);
-      p.step0 = 0;
-      p.step1 = p.steps;
+      p.b = l.segments.of(blockIdx.x);
+      p.segment = blockIdx.x - p.b * l.segments.d;
+      p.steps = p.step0 = p.step1 = p.sink_tiles = p.first = p.tiles = 0;
       span->x = span->y;
     } else {
       int lo = 0, hi = a.B - 1;
       while (lo < hi) {
         const int mid = (lo + hi) >> 1;
-        if (end[mid] * l.segments > span->x) hi = mid;
+        if (end[mid] * l.segments.d > span->x) hi = mid;
         else lo = mid + 1;
       }
       const int start = lo > 0 ? end[lo - 1] : 0;
@@ -327,18 +334,43 @@ struct Kv4Walk {
       p.steps = end[lo] - start;
       p.first = first[lo];
       p.tiles = tiles[lo];
-      p.sink_tiles = (a.n_sink + l.tile - 1) / l.tile;
-      p.segment = (span->x - start * l.segments) / p.steps;
-      const int at = start * l.segments + p.segment * p.steps;   // the segment's first step on the line
+      p.sink_tiles = (a.n_sink + kTile - 1) / kTile;
+      p.segment = (span->x - start * l.segments.d) / p.steps;
+      const int at = start * l.segments.d + p.segment * p.steps;   // the segment's first step on the line
       p.step0 = span->x - at;
       p.step1 = min(p.steps, span->y - at);
       if (p.step0 == 0 && threadIdx.x == 0)
-        l.meta[p.b * l.segments + p.segment] = make_int2(blockIdx.x, (at + p.steps - 1) / share);
+        l.meta[p.b * l.segments.d + p.segment] = make_int2(blockIdx.x, (at + p.steps - 1) / share);
       span->x = at + p.steps;
     }
     return p;
   }
 };
+
+// What the queries of a block see.  Lane r holds query row r; the other numbers are the warp's.
+struct Kv4Rows4 {
+  Kv4Seen seen;
+  int lo_min, hi_max;   // rows that any of them sees
+  int lo_max, hi_min;   // rows that all of them see
+};
+
+template <int kTile>
+__device__ __forceinline__ Kv4Rows4 kv4_rows(const Kv4Attend& a, const Kv4Line& l, Kv4Piece* p, int row0, int nrows) {
+  Kv4Rows4 r{Kv4Seen{0, 0}, 0, 0, 0, 0};
+  const int lane = lane_id();
+  const bool valid = lane < nrows;
+  if (valid) r.seen = kv4_seen(a, p->b, l.group.of(row0 + lane));
+  const bool any = valid && r.seen.hi > r.seen.lo;
+  r.lo_min = __reduce_min_sync(0xffffffffu, any ? r.seen.lo : a.L);
+  r.hi_max = __reduce_max_sync(0xffffffffu, any ? r.seen.hi : 0);
+  r.lo_max = __reduce_max_sync(0xffffffffu, valid ? r.seen.lo : 0);
+  r.hi_min = __reduce_min_sync(0xffffffffu, valid ? r.seen.hi : a.L);
+  if (l.min_steps == 0) {
+    kv4_tiles<kTile>(a, Kv4Seen{r.lo_min, r.hi_max}, p);
+    p->step1 = p->steps;
+  }
+  return r;
+}
 
 // The kernel that joins the pieces may start its blocks early; they wait for this one's end.
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
@@ -346,7 +378,7 @@ __device__ __forceinline__ void wait_for_previous_grid() { asm volatile("griddep
 
 // Grid and workspace: slots blocks stay resident, shares of at least min_steps.
 void kv4_line_plan(const Kv4Attend& a, Kv4Plan& p, int slots, int min_steps);
-Kv4Line kv4_line(const Kv4Attend& a, const Kv4Plan& p, int tile);
+Kv4Line kv4_line(const Kv4Attend& a, const Kv4Plan& p);
 // Joins the pieces: 8 * row_tiles rows of V sums and then (max, sum) pairs per slot.
 void kv4_combine(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s);
 void kv4_heads_launch(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s);

@@ -64,27 +64,24 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
   float* sqs = reinterpret_cast<float*>(smem + C::kQ + C::kRows * D * 2);   // [kRows][NG]: sum(q_g) 2^-24
   float* srs = sqs + C::kRows * NG;                                         // [kRows]: factor of the scores
   const int lane = lane_id(), warp = warp_id(), i = lane >> 2, j = lane & 3;
-  const int G = a.H / a.Hk, R = a.Tn * G, row_blocks = line.segments / a.Hk;
   const uint32_t ring = smem_u32(smem) + warp * C::kStages * C::kStage;
   if (line.min_steps > 0) launch_dependents();
   __shared__ Kv4Walk walk;
   int share = 0;
-  int2 span = walk.begin<kWarps * 32>(a, line, &share);
+  int2 span = walk.begin<kWarps * 32, kTile>(a, line, &share);
 
   while (span.x < span.y) {
-  const Kv4Piece piece = walk.next(a, line, C::kRows, share, &span);
-  const int b = piece.b, hk = piece.segment / row_blocks, row0 = (piece.segment % row_blocks) * C::kRows;
-  const int nrows = min(C::kRows, R - row0);
+  Kv4Piece piece = walk.next<kTile>(a, line, share, &span);
+  const int b = piece.b, hk = line.row_blocks.of(piece.segment), row0 = (piece.segment - hk * line.row_blocks.d) * C::kRows;
+  const int nrows = min(C::kRows, line.rows.d - row0);
+  const Kv4Rows4 see = kv4_rows<kTile>(a, line, &piece, row0, nrows);
   const int sink_tiles = piece.sink_tiles, first = piece.first;
   const int t0 = piece.step0 * kWarps, t1 = min(piece.tiles, piece.step1 * kWarps);
-
-  // ---- the rows each query sees; lane r holds query row r --------------------
-  Kv4Seen seen{0, 0};
-  if (lane < nrows) seen = kv4_seen(a, b, (row0 + lane) / G);
-  const int lo_max = __reduce_max_sync(0xffffffffu, lane < nrows ? seen.lo : 0);
-  const int hi_min = __reduce_min_sync(0xffffffffu, lane < nrows ? seen.hi : a.L);
-  const int lo_min = __reduce_min_sync(0xffffffffu, lane < nrows ? seen.lo : a.L);
-  const int hi_max = __reduce_max_sync(0xffffffffu, lane < nrows ? seen.hi : 0);
+  // place of query row r in q and in the output, in heads
+  auto head_of = [&](int r) {
+    const int t = line.group.of(row0 + r);
+    return ((long long)b * a.Tn + t) * a.H + hk * line.group.d + row0 + r - t * line.group.d;
+  };
   auto row_of = [&](int tile) { return (tile < sink_tiles ? tile : first + tile - sink_tiles) * kTile; };
 
   const uint8_t* kc = a.k.codes + b * a.k.c_b + hk * a.k.c_h;
@@ -126,9 +123,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
   for (int r = warp; r < C::kRows; r += kWarps) {
     constexpr int kWords = D / 8;
     float x[8] = {}, amax = 0.f, sum = 0.f, un;
-    const int row = row0 + r;
-    if (r < nrows && lane < kWords)
-      kv4_load8<TYPE>(a.q, (((long long)b * a.Tn + row / G) * a.H + hk * G + row % G) * D + lane * 8, x);
+    if (r < nrows && lane < kWords) kv4_load8<TYPE>(a.q, head_of(r) * D + lane * 8, x);
 #pragma unroll
     for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
     const float sc = q_normaliser(warp_max(amax), &un);
@@ -157,8 +152,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       rs[nt][c] = srs[nt * 8 + 2 * j + c];
-      lo[nt][c] = __shfl_sync(0xffffffffu, seen.lo, nt * 8 + 2 * j + c);
-      hi[nt][c] = __shfl_sync(0xffffffffu, seen.hi, nt * 8 + 2 * j + c);
+      lo[nt][c] = __shfl_sync(0xffffffffu, see.seen.lo, nt * 8 + 2 * j + c);
+      hi[nt][c] = __shfl_sync(0xffffffffu, see.seen.hi, nt * 8 + 2 * j + c);
     }
   }
 
@@ -199,7 +194,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
     if (next < t1) issue(next, stage == 0 ? C::kStages - 1 : stage - 1);
     kv4_cp_commit();
     const int r0 = row_of(tile);
-    const bool masked = !(r0 + kTile <= a.n_sink || (r0 >= lo_max && r0 + kTile <= hi_min));
+    const bool masked = !(r0 + kTile <= a.n_sink || (r0 >= see.lo_max && r0 + kTile <= see.hi_min));
     uint32_t st = ring + stage * C::kStage, sp = st + 2 * C::kCodes + i * NG * 4;
     // ---- do the scales of the tile's values fit their power of two?  Lane: key r0 + lane ----
     bool slow[NG];
@@ -207,7 +202,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
       uint32_t v[NG];
       load_params(st + 2 * C::kCodes + C::kParams + lane * NG * 4, v);
       const int r = r0 + lane;
-      const bool used = !masked || r < a.n_sink || (r >= lo_min && r < hi_max);
+      const bool used = !masked || r < a.n_sink || (r >= see.lo_min && r < see.hi_max);
       bool fit = true;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
@@ -439,8 +434,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
       y = fmaf(f, so[at * D + d + 1], y);
     }
     if (alone) {
-      const int row = row0 + r;
-      const long long head = ((long long)b * a.Tn + row / G) * a.H + hk * G + row % G;
+      const long long head = head_of(r);
       const float inv = l == 0.f ? 0.f : 1.f / l;
       reinterpret_cast<uint32_t*>(a.out)[(head * D + d) / 2] = kv4_pack2<TYPE>(x * inv, y * inv);
     } else {
@@ -457,7 +451,7 @@ void launch(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s) {
   auto kern = kv4_heads_kernel<D, NT, TYPE>;
   constexpr int smem = HeadsCfg<D, NT>::kSmem;
   ensure_smem_attr(reinterpret_cast<const void*>(kern), smem);
-  kern<<<p.blocks, kWarps * 32, smem, s>>>(a, kv4_line(a, p, kTile));
+  kern<<<p.blocks, kWarps * 32, smem, s>>>(a, kv4_line(a, p));
 }
 
 template <int TYPE>

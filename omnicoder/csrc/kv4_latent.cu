@@ -68,21 +68,15 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
   if (line.min_steps > 0) launch_dependents();
   __shared__ Kv4Walk walk;
   int share = 0;
-  int2 span = walk.begin<kWarps * 32>(a, line, &share);
+  int2 span = walk.begin<kWarps * 32, kTile>(a, line, &share);
   int used = 0;     // tiles that went through the stages
   bool ok = true;
 
   while (span.x < span.y) {
-  const Kv4Piece piece = walk.next(a, line, kRows, share, &span);
+  Kv4Piece piece = walk.next<kTile>(a, line, share, &span);
   const int b = piece.b, row0 = piece.segment * kRows, nrows = min(kRows, R - row0);
-  const int sink_tiles = piece.sink_tiles, first = piece.first;
-  const int t0 = piece.step0, t1 = min(piece.tiles, piece.step1);
-  Kv4Seen seen{0, 0};
-  if (lane < nrows) seen = kv4_seen(a, b, (row0 + lane) / a.H);
-  const int lo_max = __reduce_max_sync(0xffffffffu, lane < nrows ? seen.lo : 0);
-  const int hi_min = __reduce_min_sync(0xffffffffu, lane < nrows ? seen.hi : a.L);
-  const int lo_min = __reduce_min_sync(0xffffffffu, lane < nrows ? seen.lo : a.L);
-  const int hi_max = __reduce_max_sync(0xffffffffu, lane < nrows ? seen.hi : 0);
+  const Kv4Rows4 see = kv4_rows<kTile>(a, line, &piece, row0, nrows);
+  const int sink_tiles = piece.sink_tiles, first = piece.first, t0 = piece.step0, t1 = min(piece.tiles, piece.step1);
   auto row_of = [&](int tile) { return (tile < sink_tiles ? tile : first + tile - sink_tiles) * kTile; };
 
   const uint8_t* kc = a.k.codes + b * a.k.c_b;
@@ -135,8 +129,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
     if (lane == 0) srs[r] = un * (a.scale * (kKv4Log2e * kKv4Codes));
   }
   if (warp == 0 && lane < kRows) {
-    slo[lane] = seen.lo;
-    shi[lane] = seen.hi;
+    slo[lane] = see.seen.lo;
+    shi[lane] = see.seen.hi;
   }
   __syncthreads();
 
@@ -229,7 +223,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
 #pragma unroll
         for (int c = 0; c < 4; ++c) s[nt][c] = fmaf(d[nt][c], c < 2 ? sa : sb, s[nt][c]);
     }
-    const bool masked = !(r0 + kTile <= a.n_sink || (r0 >= lo_max && r0 + kTile <= hi_min));
+    const bool masked = !(r0 + kTile <= a.n_sink || (r0 >= see.lo_max && r0 + kTile <= see.hi_min));
     bool above = false;
     float top[NT][2];
 #pragma unroll
@@ -312,7 +306,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
       for (int k = 0; k < kTile / 32; ++k) {
         const int r = lane + 32 * k;
         sc[k] = bf16_lo(lds32(params + (r * NG + vg) * 4));
-        used[k] = !masked || r0 + r < a.n_sink || (r0 + r >= lo_min && r0 + r < hi_max);
+        used[k] = !masked || r0 + r < a.n_sink || (r0 + r >= see.lo_min && r0 + r < see.hi_max);
         fit = fit && (!used[k] || kv4_in_range(sc[k], f));
       }
       if (!__all_sync(0xffffffffu, fit)) {
@@ -479,7 +473,7 @@ void launch(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s) {
   auto kern = kv4_latent_kernel<V, TYPE>;
   constexpr int smem = LatentCfg<V>::kSmem;
   ensure_smem_attr(reinterpret_cast<const void*>(kern), smem);
-  kern<<<p.blocks, kWarps * 32, smem, s>>>(a, kv4_line(a, p, kTile),
+  kern<<<p.blocks, kWarps * 32, smem, s>>>(a, kv4_line(a, p),
                                            reinterpret_cast<StatusBlock*>(status_ptr()));
 }
 

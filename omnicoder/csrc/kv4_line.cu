@@ -13,18 +13,18 @@ constexpr int kThreads = 256;
 // A thread holds four value dims of a query row; GROUPS threads take every GROUPS-th
 // piece each and are summed in a fixed order.
 template <int TYPE, int GROUPS>
-__global__ void __launch_bounds__(kThreads) kv4_combine_kernel(const Kv4Attend a, const Kv4Line line, const int rows_per_block) {
+__global__ void __launch_bounds__(kThreads) kv4_combine_kernel(const Kv4Attend a, const Kv4Line line, const Kv4Div cols,
+                                                              const int rows_per_block) {
   constexpr int kItems = kThreads / GROUPS;
   __shared__ float4 s_sum[kThreads];
   __shared__ float2 s_ml[kThreads];
-  const int G = a.H / a.Hk, R = a.Tn * G, row_blocks = line.segments / a.Hk, cols = a.V / 4;
-  const int item = threadIdx.x % kItems, group = threadIdx.x / kItems;
-  const long long at = (long long)blockIdx.x * kItems + item, total = (long long)a.B * a.Hk * R * cols;
-  const int col = (int)(at % cols), place = (int)(at / cols);
-  const int row = place % R, hk = place / R % a.Hk, b = place / R / a.Hk, r = row % rows_per_block;
+  const int item = threadIdx.x % kItems, group = threadIdx.x / kItems, at = blockIdx.x * kItems + item;
+  const int place = cols.of(at), col = at - place * cols.d;                      // (sequence, head, row), four dims
+  const int head = line.rows.of(place), row = place - head * line.rows.d, t = line.group.of(row);
+  const int r = row & (rows_per_block - 1), b = head / a.Hk, hk = head - b * a.Hk;
   wait_for_previous_grid();
   int2 range = make_int2(0, 0);
-  if (at < total) range = line.meta[b * line.segments + hk * row_blocks + row / rows_per_block];
+  if (b < a.B) range = line.meta[b * line.segments.d + hk * line.row_blocks.d + row / rows_per_block];
   const bool join = range.x != range.y;  // otherwise one block held the segment and has written the row
   const size_t slot = (size_t)rows_per_block * (a.V + 2);
   float top = -INFINITY, l = 0.f;
@@ -65,9 +65,9 @@ __global__ void __launch_bounds__(kThreads) kv4_combine_kernel(const Kv4Attend a
     x.z = fmaf(f, v.z, x.z);
     x.w = fmaf(f, v.w, x.w);
   }
-  const long long head = ((long long)b * a.Tn + row / G) * a.H + hk * G + row % G;
+  const long long out = ((long long)b * a.Tn + t) * a.H + hk * line.group.d + row - t * line.group.d;
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + head * a.V + 4 * col) =
+  *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + out * a.V + 4 * col) =
       make_uint2(kv4_pack2<TYPE>(x.x * inv, x.y * inv), kv4_pack2<TYPE>(x.z * inv, x.w * inv));
 }
 
@@ -83,14 +83,16 @@ void launch(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s) {
   early.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, kv4_combine_kernel<TYPE, GROUPS>, a, kv4_line(a, p, 0), 8 * p.row_tiles);
+  cudaLaunchKernelEx(&cfg, kv4_combine_kernel<TYPE, GROUPS>, a, kv4_line(a, p), Kv4Div(a.V / 4), 8 * p.row_tiles);
 }
 
 }  // namespace
 
-Kv4Line kv4_line(const Kv4Attend& a, const Kv4Plan& p, int tile) {
+Kv4Line kv4_line(const Kv4Attend& a, const Kv4Plan& p) {
   const size_t sums = (size_t)p.blocks * 2 * 8 * p.row_tiles * (a.V + 2);
-  return Kv4Line{a.Hk * p.row_blocks, tile, p.min_steps, reinterpret_cast<int2*>(a.part + sums)};
+  const int group = a.H / a.Hk;
+  return Kv4Line{Kv4Div(a.Hk * p.row_blocks), Kv4Div(p.row_blocks), Kv4Div(group), Kv4Div(a.Tn * group), p.min_steps,
+                 reinterpret_cast<int2*>(a.part + sums)};
 }
 
 // The host knows the cache's size, not the sequences' lengths.  A block per segment where a full
