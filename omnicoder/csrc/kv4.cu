@@ -26,13 +26,30 @@ constexpr float kMinScale = 7.52316384526264e-37f;  // 2^-120
 // ---------------------------------------------------------------------------
 constexpr int kPiece = 16;
 
+// 32 bytes at once, where they start on a 32-byte boundary.
+__device__ __forceinline__ void load32(const void* p, bool wide, uint32_t* w) {
+  if (wide) {
+    asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                 : "l"(p));
+  } else {
+    *reinterpret_cast<uint4*>(w) = reinterpret_cast<const uint4*>(p)[0];
+    *reinterpret_cast<uint4*>(w + 4) = reinterpret_cast<const uint4*>(p)[1];
+  }
+}
+__device__ __forceinline__ void store32(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
 template <int TYPE>
-__device__ __forceinline__ void load_piece(const void* base, long long i, float* x, uint32_t* bits) {
+__device__ __forceinline__ void load_piece(const void* base, long long i, bool wide, float* x, uint32_t* bits) {
   constexpr int kWords = TYPE == KV4_F32 ? 16 : 8;
-  const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(base) + i * (TYPE == KV4_F32 ? 4 : 2));
+  const uint8_t* p = reinterpret_cast<const uint8_t*>(base) + i * (TYPE == KV4_F32 ? 4 : 2);
   uint32_t w[kWords];
 #pragma unroll
-  for (int k = 0; k < kWords / 4; ++k) *reinterpret_cast<uint4*>(w + 4 * k) = p[k];
+  for (int k = 0; k < kWords / 8; ++k) load32(p + 32 * k, wide, w + 8 * k);
 #pragma unroll
   for (int k = 0; k < kWords; ++k) {
     if (TYPE == KV4_F32) {
@@ -52,13 +69,13 @@ __device__ __forceinline__ void load_piece(const void* base, long long i, float*
 template <int TYPE>
 __device__ __forceinline__ void store_piece(void* base, long long i, const float* x) {
   constexpr int kWords = TYPE == KV4_F32 ? 16 : 8;
-  uint4* p = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(base) + i * (TYPE == KV4_F32 ? 4 : 2));
+  uint8_t* p = reinterpret_cast<uint8_t*>(base) + i * (TYPE == KV4_F32 ? 4 : 2);
   uint32_t w[kWords];
 #pragma unroll
   for (int k = 0; k < kWords; ++k)
     w[k] = TYPE == KV4_F32 ? __float_as_uint(x[k]) : kv4_pack2<TYPE>(x[2 * k], x[2 * k + 1]);
 #pragma unroll
-  for (int k = 0; k < kWords / 4; ++k) p[k] = *reinterpret_cast<uint4*>(w + 4 * k);
+  for (int k = 0; k < kWords / 8; ++k) store32(p + 32 * k, w + 8 * k);
 }
 
 template <int TYPE>
@@ -79,8 +96,10 @@ constexpr int kIoThreads = 256;
 constexpr int kPasses = 4;
 
 struct IoGrid {
-  int pieces, rows_per_pass, passes;  // threads of a row, rows of a pass
-  uint32_t total, mul_t, shift_t;     // rows Hk * T of a sequence; n / T = (n * mul_t) >> 32 >> shift_t
+  Kv4Div pieces, tokens;       // threads of a row; T
+  int rows_per_pass, passes;
+  int total;                   // rows Hk * T of a sequence
+  int groups, lanes_shift;     // groups of a row; 2^lanes_shift threads hold one
 };
 
 struct IoRow {
@@ -88,13 +107,20 @@ struct IoRow {
   long long row;  // of the cache; -1: nothing to do
 };
 
-__device__ __forceinline__ IoRow io_row(const Kv4IO& a, const IoGrid& g, uint32_t r) {
+__device__ __forceinline__ IoRow io_row(const Kv4IO& a, const IoGrid& g, int r) {
   IoRow x;
-  x.h = a.T == 1 ? (int)r : (int)(__umulhi(r, g.mul_t) >> g.shift_t);
-  x.t = (int)r - x.h * a.T;
+  x.h = g.tokens.of(r);
+  x.t = r - x.h * a.T;
   x.row = a.row_offset + kv4_load_pos(a.pos, a.pos64, (long long)blockIdx.y * a.T + x.t);
   if (x.row < 0 || x.row >= a.L) x.row = -1;
   return x;
+}
+
+__device__ __forceinline__ uint8_t* io_codes(const Kv4IO& a, const Kv4Cache& c, const IoRow& x, int piece) {
+  return c.codes + blockIdx.y * c.c_b + x.h * c.c_h + x.row * (a.W / 2) + piece * 8;
+}
+__device__ __forceinline__ uint32_t* io_params(const Kv4Cache& c, const IoGrid& g, const IoRow& x, int piece) {
+  return reinterpret_cast<uint32_t*>(c.params + blockIdx.y * c.p_b + x.h * c.p_h + (x.row * g.groups + (piece >> g.lanes_shift)) * 4);
 }
 
 // Round (x - m) / s, .. < 15.5, decided as if the quotient were exact: d + e = x - m exactly,
@@ -116,40 +142,52 @@ __device__ __forceinline__ uint32_t kv4_codes8_exact(const float* x, float m, fl
   return code;
 }
 
-// Eight codes of bf16 rows whose values are 0 or at least 2^-16 of the range R.  Then x, m and s are
-// multiples of 2^-24 R: d = x - m is exact, and a quotient d / s that is not exactly halfway between
-// two codes is 2^-24 R / s > 2^-21 or more away, half a unit of the quotient's last place.  q' is the quotient rounded to fp32 (the residual
-// correction of Markstein, 1990), so adding 2^23
-// rounds it to the right code, ties to even.  Codes join by multiply-adds on the sums' bits.
+// Eight codes from q', the quotient (x - m) / s with one residual correction (Markstein, 1990):
+// within 2^-20 of it, and exactly k + 1/2 where the quotient is that and x - m is exact.  Adding
+// 2^23 rounds it, ties to even.  That decides as an exact quotient would
+//   - for bf16 rows whose values are 0 or at least 2^-16 of the range R: x, m and s are then
+//     multiples of 2^-24 R, x - m is exact, and a quotient that is not halfway between two codes is
+//     2^-24 R / s > 2^-21 or more away, half a unit of the quotient's last place;
+//   - for any row where no quotient lies within 10^-4 of halfway (kv4_near_border).
+// Codes join by multiply-adds on the sums' bits.
+template <int TYPE>
 __device__ __forceinline__ uint32_t kv4_codes8(const float* x, float m, float s, float inv) {
   uint32_t acc = 0;
 #pragma unroll
   for (int i = 7; i >= 0; --i) {
-    const float d = x[i] - m, q = d * inv, q1 = fmaf(fmaf(-q, s, d), inv, q);
+    const float d = x[i] - m, q = d * inv;
+    float q1 = fmaf(fmaf(-q, s, d), inv, q);
+    if (TYPE != KV4_BF16) q1 = fminf(fmaxf(q1, 0.f), 15.f);  // the minimum was rounded to bf16
     acc = acc * 16u + __float_as_uint(q1 + 8388608.f);
   }
   return acc - 0xfb000000u;  // the sum of 0x4b000000 * 16^i, the bits of 2^23, modulo 2^32
 }
 
+__device__ __forceinline__ bool kv4_near_border(const float* x, float m, float inv) {
+  float far = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPiece; ++i) {
+    const float t = fminf(fmaxf((x[i] - m) * inv, 0.f), 15.f);
+    far = fmaxf(far, fabsf(t - ((t + 8388608.f) - 8388608.f)));
+  }
+  return far > 0.4999f;
+}
+
 template <int TYPE>
 __global__ void __launch_bounds__(kIoThreads) kv4_write_kernel(const Kv4IO a, const IoGrid g) {
-  const int b = blockIdx.y, r_in = threadIdx.x / g.pieces, piece = threadIdx.x - r_in * g.pieces;
+  const int b = blockIdx.y, r_in = g.pieces.of(threadIdx.x), piece = threadIdx.x - r_in * g.pieces.d;
   const Kv4Cache& c = a.cache[blockIdx.z];
   const Kv4Rows& src = a.rows[blockIdx.z];
-  const int lanes = a.group / kPiece;  // 1, 2 or 4 neighbouring threads hold a group
-  const uint32_t first = blockIdx.x * (uint32_t)(g.rows_per_pass * g.passes) + r_in;
+  const int lanes = 1 << g.lanes_shift;  // 1, 2 or 4 neighbouring threads hold a group
+  const int first = blockIdx.x * (g.rows_per_pass * g.passes) + r_in;
   const bool idle = r_in >= g.rows_per_pass;
 #pragma unroll 1
   for (int k = 0; k < g.passes; ++k) {
-    const uint32_t r = first + k * g.rows_per_pass;
-    float x[kPiece] = {};
-    uint32_t bits[8] = {};
-    IoRow row;
-    row.row = -1;
-    if (!idle && r < g.total) {
-      row = io_row(a, g, r);
-      load_piece<TYPE>(src.x, b * src.x_b + row.t * src.x_t + row.h * src.x_h + piece * kPiece, x, bits);
-    }
+    const int r = first + k * g.rows_per_pass;
+    float x[kPiece];
+    uint32_t bits[8];
+    const IoRow row = io_row(a, g, min(r, g.total - 1));   // threads behind the last row repeat it and write nothing
+    load_piece<TYPE>(src.x, b * src.x_b + row.t * src.x_t + row.h * src.x_h + piece * kPiece, a.wide, x, bits);
     float lo, hi, probe;  // probe: NaN behind a NaN or an infinity
     if (TYPE == KV4_BF16) {
       const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(bits);
@@ -197,7 +235,9 @@ __global__ void __launch_bounds__(kIoThreads) kv4_write_kernel(const Kv4IO a, co
     }
     uint64_t code = 0;
     if (!bad && s > 0.f) {
-      bool exact = TYPE != KV4_BF16;
+      float inv;  // within 2^-23: candidates and residual corrections need no more
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+      bool check = TYPE != KV4_BF16 || s < 1e-27f;
       if (TYPE == KV4_BF16) {
         // the smallest |x| - 1 as bits; 0 becomes the largest
         uint32_t least = 0xffffffffu;
@@ -205,85 +245,96 @@ __global__ void __launch_bounds__(kIoThreads) kv4_write_kernel(const Kv4IO a, co
         for (int i = 0; i < 8; ++i) least = __viaddmin_u16x2(bits[i] & 0x7fff7fffu, 0xffffffffu, least);
         const float smallest = __uint_as_float((min(least & 0xffffu, least >> 16) + 1u) << 16);
         const float limit = range * 1.52587890625e-5f;
-        exact = smallest < limit || (m != 0.f && fabsf(m) < limit) || s < 1e-27f;
+        check = check || smallest < limit || (m != 0.f && fabsf(m) < limit);
       }
-      float inv;  // within 2^-23: candidates and residual corrections need no more
-      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
-      if (exact) {
+      if (check && (s < 1e-27f || kv4_near_border(x, m, inv)))
         code = (uint64_t)kv4_codes8_exact(x, m, s, inv) | ((uint64_t)kv4_codes8_exact(x + 8, m, s, inv) << 32);
-      } else {
-        code = (uint64_t)kv4_codes8(x, m, s, inv) | ((uint64_t)kv4_codes8(x + 8, m, s, inv) << 32);
-      }
+      else
+        code = (uint64_t)kv4_codes8<TYPE>(x, m, s, inv) | ((uint64_t)kv4_codes8<TYPE>(x + 8, m, s, inv) << 32);
     }
-    if (row.row < 0) continue;
-    *reinterpret_cast<uint64_t*>(c.codes + b * c.c_b + row.h * c.c_h + row.row * (a.W / 2) + piece * 8) = code;
+    if (row.row < 0 || idle || r >= g.total) continue;
+    *reinterpret_cast<uint64_t*>(io_codes(a, c, row, piece)) = code;
     if ((piece & (lanes - 1)) == 0) {
       const uint32_t word = (uint32_t)__bfloat16_as_ushort(sb) | ((uint32_t)__bfloat16_as_ushort(mb) << 16);
-      *reinterpret_cast<uint32_t*>(c.params + b * c.p_b + row.h * c.p_h +
-                                   (row.row * (a.W / a.group) + piece / lanes) * 4) = bad ? 0x7fc07fc0u : word;
+      *io_params(c, g, row, piece) = bad ? 0x7fc07fc0u : word;
     }
   }
 }
 
 template <int TYPE>
 __global__ void __launch_bounds__(kIoThreads) kv4_read_kernel(const Kv4IO a, const IoGrid g) {
-  const int b = blockIdx.y, r_in = threadIdx.x / g.pieces, piece = threadIdx.x - r_in * g.pieces;
+  const int b = blockIdx.y, r_in = g.pieces.of(threadIdx.x), piece = threadIdx.x - r_in * g.pieces.d;
   if (r_in >= g.rows_per_pass) return;
   const Kv4Cache& c = a.cache[blockIdx.z];
   const Kv4Rows& dst = a.rows[blockIdx.z];
-  const int lanes = a.group / kPiece;
-  const uint32_t first = blockIdx.x * (uint32_t)(g.rows_per_pass * g.passes) + r_in;
+  const int first = blockIdx.x * (g.rows_per_pass * g.passes) + r_in;
   uint2 code[kPasses];
   uint32_t word[kPasses];
   IoRow row[kPasses];
 #pragma unroll
   for (int k = 0; k < kPasses; ++k) {
-    const uint32_t r = first + k * g.rows_per_pass;
+    const int r = first + k * g.rows_per_pass;
     code[k] = make_uint2(0, 0);  // rows outside the cache read as zeros
     word[k] = 0;
     if (k < g.passes && r < g.total) {
       row[k] = io_row(a, g, r);
       if (row[k].row >= 0) {
-        code[k] = *reinterpret_cast<const uint2*>(c.codes + b * c.c_b + row[k].h * c.c_h + row[k].row * (a.W / 2) + piece * 8);
-        word[k] = *reinterpret_cast<const uint32_t*>(c.params + b * c.p_b + row[k].h * c.p_h +
-                                                     (row[k].row * (a.W / a.group) + piece / lanes) * 4);
+        code[k] = *reinterpret_cast<const uint2*>(io_codes(a, c, row[k], piece));
+        word[k] = *io_params(c, g, row[k], piece);
       }
     }
   }
 #pragma unroll
   for (int k = 0; k < kPasses; ++k) {
     if (k >= g.passes || first + k * g.rows_per_pass >= g.total) break;
-    const float s = bf16_lo(word[k]), m = bf16_hi(word[k]);
-    float x[kPiece];
+    const long long at = b * dst.x_b + row[k].t * dst.x_t + row[k].h * dst.x_h + piece * kPiece;
+    if (TYPE == KV4_BF16) {
+      // n s + m in one bf16 multiply-add, rounded once; nibbles 0..3 of both halves of a code word as
+      // 128 + n give the dims e and e + 4
+      const uint32_t s2 = __byte_perm(word[k], word[k], 0x1010), m2 = __byte_perm(word[k], word[k], 0x3232);
+      uint32_t v[8];
 #pragma unroll
-    for (int w = 0; w < 2; ++w)
+      for (int w = 0; w < 2; ++w)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        // nibbles 2h and 4 + 2h as 1024 + n, 2h + 1 and 5 + 2h as 1024 + 16 n in fp16
-        const uint32_t u = (w ? code[k].y : code[k].x) >> (8 * h);
-        const uint32_t e = (u & 0x000f000fu) | 0x64006400u, o = (u & 0x00f000f0u) | 0x64006400u;
-        const __half2 ne = __hsub2(*reinterpret_cast<const __half2*>(&e), __float2half2_rn(1024.f));
-        const __half2 no = __hfma2(*reinterpret_cast<const __half2*>(&o), __float2half2_rn(0.0625f), __float2half2_rn(-64.f));
-        const float2 fe = __half22float2(ne), fo = __half22float2(no);
-        x[8 * w + 2 * h] = fmaf(fe.x, s, m);
-        x[8 * w + 2 * h + 4] = fmaf(fe.y, s, m);
-        x[8 * w + 2 * h + 1] = fmaf(fo.x, s, m);
-        x[8 * w + 2 * h + 5] = fmaf(fo.y, s, m);
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t u = (((w ? code[k].y : code[k].x) >> (4 * e)) & 0x000f000fu) | 0x43004300u;
+          const __nv_bfloat162 n = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), __float2bfloat162_rn(128.f));
+          const __nv_bfloat162 x = __hfma2(n, *reinterpret_cast<const __nv_bfloat162*>(&s2), *reinterpret_cast<const __nv_bfloat162*>(&m2));
+          v[4 * w + e] = *reinterpret_cast<const uint32_t*>(&x);
+        }
+      uint32_t o[8];
+#pragma unroll
+      for (int w = 0; w < 8; w += 4) {  // (0, 4), (1, 5), .. -> (0, 1), (2, 3), (4, 5), (6, 7)
+        o[w] = __byte_perm(v[w], v[w + 1], 0x5410);
+        o[w + 1] = __byte_perm(v[w + 2], v[w + 3], 0x5410);
+        o[w + 2] = __byte_perm(v[w], v[w + 1], 0x7632);
+        o[w + 3] = __byte_perm(v[w + 2], v[w + 3], 0x7632);
       }
-    store_piece<TYPE>(dst.x, b * dst.x_b + row[k].t * dst.x_t + row[k].h * dst.x_h + piece * kPiece, x);
+      store32(reinterpret_cast<uint16_t*>(dst.x) + at, o);
+    } else {
+      const float s = bf16_lo(word[k]), m = bf16_hi(word[k]);
+      float x[kPiece];
+#pragma unroll
+      for (int i = 0; i < kPiece; ++i) {
+        // 2^23 + n as bits, less 2^23: the code as a float
+        const uint32_t n = ((i < 8 ? code[k].x : code[k].y) >> (4 * (i & 7))) & 15u;
+        x[i] = fmaf(__uint_as_float(n | 0x4b000000u) - 8388608.f, s, m);
+      }
+      store_piece<TYPE>(dst.x, at, x);
+    }
   }
 }
 
 // Enough blocks first, then several rows per thread.
 dim3 io_grid(const Kv4IO& a, IoGrid* g) {
-  g->pieces = a.W / kPiece;
-  g->rows_per_pass = kIoThreads / g->pieces;
-  g->total = (uint32_t)(a.T * a.Hk);
+  g->pieces = Kv4Div(a.W / kPiece);
+  g->tokens = Kv4Div(a.T);
+  g->rows_per_pass = kIoThreads / g->pieces.d;
+  g->total = a.T * a.Hk;
+  g->groups = a.W / a.group;
+  g->lanes_shift = a.group == 64 ? 2 : a.group == 32 ? 1 : 0;
   const long long blocks1 = (g->total + g->rows_per_pass - 1) / g->rows_per_pass;
   g->passes = (int)std::min<long long>(kPasses, std::max<long long>(1, blocks1 * a.B * a.count / (148 * 4)));
-  g->shift_t = 0;  // n / T for n < 2^31: mul = ceil(2^(32 + shift) / T), shift = ceil(log2 T) - 1
-  while ((2ull << g->shift_t) < (unsigned long long)a.T) ++g->shift_t;
-  g->mul_t = a.T > 1 ? (uint32_t)(((1ull << (32 + g->shift_t)) + a.T - 1) / a.T) : 0;
   const long long per_block = (long long)g->rows_per_pass * g->passes;
   return dim3((unsigned)((g->total + per_block - 1) / per_block), (unsigned)a.B, (unsigned)a.count);
 }
@@ -398,7 +449,7 @@ void launch_rows(const Kv4Attend& a, cudaStream_t s) {
 }  // namespace
 
 void kv4_write(const Kv4IO& a, cudaStream_t s) {
-  IoGrid g;
+  IoGrid g{Kv4Div(1), Kv4Div(1), 0, 0, 0, 0, 0};
   const dim3 grid = io_grid(a, &g);
   if (a.type == KV4_F32) kv4_write_kernel<KV4_F32><<<grid, kIoThreads, 0, s>>>(a, g);
   else if (a.type == KV4_F16) kv4_write_kernel<KV4_F16><<<grid, kIoThreads, 0, s>>>(a, g);
@@ -406,7 +457,7 @@ void kv4_write(const Kv4IO& a, cudaStream_t s) {
 }
 
 void kv4_read(const Kv4IO& a, cudaStream_t s) {
-  IoGrid g;
+  IoGrid g{Kv4Div(1), Kv4Div(1), 0, 0, 0, 0, 0};
   const dim3 grid = io_grid(a, &g);
   if (a.type == KV4_F32) kv4_read_kernel<KV4_F32><<<grid, kIoThreads, 0, s>>>(a, g);
   else if (a.type == KV4_F16) kv4_read_kernel<KV4_F16><<<grid, kIoThreads, 0, s>>>(a, g);
