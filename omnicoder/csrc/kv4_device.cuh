@@ -101,8 +101,8 @@ __device__ __forceinline__ uint32_t nibbles_bf16(uint32_t x) {
 }
 
 // Weights meet value codes as x = p s f in fp16, f a power of two for which every scale s of the
-// keys at hand has s f in [2^-8, 2^6], or 0: then x < 2^14 (p < 2^8), eleven bits of it count down
-// to 2^-14, and what is lost below 2^-25 is 2^-17 of a row's largest weight.  Where the scales of
+// keys at hand has s f in [2^-8, 2^6], or 0: then x < 2^14 (p < 2^8), its rounding is 2^-11 of it
+// down to 2^-14 and 2^-25 below, 2^-17 of a row's largest weight.  Where the scales of
 // neighbouring keys lie further apart, x is rounded to bf16 instead (slow).
 constexpr float kKv4Low = 0.00390625f, kKv4High = 64.f;
 
@@ -124,7 +124,8 @@ __device__ __forceinline__ void mma_values(float (*acc)[4], uint32_t l0, uint32_
   for (int nt = 0; nt < NT; ++nt) mma_f16(acc[nt], a0, a1, a2, a3, w[nt][0], w[nt][1]);
 }
 
-// The same for bf16 weights, whose sum sums[nt][] over the keys is known.
+// The same for bf16 weights, whose sum sums[nt][] over the keys is known, and codes n - 8: the
+// rounding of a weight then counts for eight steps at most.
 template <int MM, int NT>
 __device__ __forceinline__ void mma_values_bf16(float (*acc)[4], uint32_t l0, uint32_t h0, uint32_t l8, uint32_t h8,
                                                 const uint32_t (*w)[2], const float (*sums)[4]) {
@@ -135,7 +136,7 @@ __device__ __forceinline__ void mma_values_bf16(float (*acc)[4], uint32_t l0, ui
     mma_bf16_zero(d, a0, a1, a2, a3, w[nt][0], w[nt][1]);
 #pragma unroll
     for (int c = 0; c < 4; ++c)
-      acc[nt][c] = fmaf(fmaf(-16.f, sums[nt][c & 1], d[c]), MM & 1 ? 9.5367431640625e-7f : 5.9604644775390625e-8f, acc[nt][c]);
+      acc[nt][c] = fmaf(fmaf(-24.f, sums[nt][c & 1], d[c]), MM & 1 ? 9.5367431640625e-7f : 5.9604644775390625e-8f, acc[nt][c]);
   }
 }
 __device__ __forceinline__ float value_unit(int mm) { return mm & 1 ? 1048576.f : 16777216.f; }

@@ -4,11 +4,10 @@
 // With codes n, scales s and minima m per (row t, group g) and normalised
 // queries q:
 //   score_t = sum_g s_tg (q_g . n_tg) + m_tg sum(q_g)
-//   o_d     = sum_t (p_t s_tg) (n_td - 8) + sum_t p_t (m_tg + 8 s_tg)
+//   o_d     = sum_t (p_t s_tg) n_td + sum_t p_t m_tg
 // so that the tensor cores multiply integers: the query with the codes, and the
 // weights p s (rounded to fp16, the only rounding before the output's) with the
-// codes.  The second sums stay in fp32; the weights meet n - 8 instead of n
-// because the rounding error then scales with at most 8 steps, not 15.
+// codes.  The second sums stay in fp32.
 //
 // A block owns (sequence, key / value head, up to 16 query rows, one split of
 // the keys).  Each of its four warps takes every fourth 32-row tile on its own:
@@ -139,7 +138,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
   // operand of the scores: lane (i, j) holds query row i against the 16 dims that it reads of each group
   uint2 qf[NG][4][NT];
   float qs[NG][NT][2], rs[NT][2];
-  int lo[NT][2], hi[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -152,15 +150,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       rs[nt][c] = srs[nt * 8 + 2 * j + c];
-      lo[nt][c] = __shfl_sync(0xffffffffu, see.seen.lo, nt * 8 + 2 * j + c);
-      hi[nt][c] = __shfl_sync(0xffffffffu, see.seen.hi, nt * 8 + 2 * j + c);
     }
   }
 
   float f[NG];                     // the values' power of two; 0 before any
 #pragma unroll
   for (int g = 0; g < NG; ++g) f[g] = 0.f;
-  float acc[NG][4][NT][4], accr[NG][NT][4], accm[NG][NT][2], lsum[NT][2];
+  float acc[NG][4][NT][4], accm[NG][NT][2], lsum[NT][2];
   float limit[NT][2], ref[NT][2];  // running maximum + slack, running maximum (0 before any key)
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -170,7 +166,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
       for (int c = 0; c < 4; ++c)
 #pragma unroll
         for (int mm = 0; mm < 4; ++mm) acc[g][mm][nt][c] = 0.f;
-      accr[g][nt][0] = accr[g][nt][1] = accr[g][nt][2] = accr[g][nt][3] = 0.f;
       accm[g][nt][0] = accm[g][nt][1] = 0.f;
     }
     lsum[nt][0] = lsum[nt][1] = 0.f;
@@ -222,11 +217,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                  accr[g][nt][c] *= move;
+                for (int c = 0; c < 4; ++c)
 #pragma unroll
                   for (int mm = 0; mm < 4; ++mm) acc[g][mm][nt][c] *= move;
-                }
             }
           }
           slow[g] = !__all_sync(0xffffffffu, !used || kv4_in_range(sc, f[g]));
@@ -275,9 +268,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int key = r + (c >> 1) * 8;
-            if (!(key < a.n_sink || (key >= lo[nt][c & 1] && key < hi[nt][c & 1]))) s[nt][c] = -INFINITY;
+          for (int c = 0; c < 2; ++c) {
+            const int lo = __shfl_sync(0xffffffffu, see.seen.lo, nt * 8 + 2 * j + c);
+            const int hi = __shfl_sync(0xffffffffu, see.seen.hi, nt * 8 + 2 * j + c);
+            if (!(r < a.n_sink || (r >= lo && r < hi))) s[nt][c] = -INFINITY;
+            if (!(r + 8 < a.n_sink || (r + 8 >= lo && r + 8 < hi))) s[nt][c + 2] = -INFINITY;
           }
       }
 #pragma unroll
@@ -305,7 +300,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
               accm[g][nt][c] *= alpha;
-              accr[g][nt][c] *= alpha;
 #pragma unroll
               for (int mm = 0; mm < 4; ++mm) {
                 acc[g][mm][nt][c] *= alpha;
@@ -329,7 +323,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         const float sa = bf16_lo(pa[g]), sb = bf16_lo(pb[g]);
-        const float ca = fmaf(8.f, sa, bf16_hi(pa[g])), cb = fmaf(8.f, sb, bf16_hi(pb[g]));
+        const float ma = bf16_hi(pa[g]), mb = bf16_hi(pb[g]);
         float x[NT][4];
         const float fa = sa * f[g], fb = sb * f[g];
 #pragma unroll
@@ -340,11 +334,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               if (s[nt][c] == 0.f) x[nt][c] = 0.f;
-              else accm[g][nt][c & 1] = fmaf(s[nt][c], c < 2 ? ca : cb, accm[g][nt][c & 1]);
+              else accm[g][nt][c & 1] = fmaf(s[nt][c], c < 2 ? ma : mb, accm[g][nt][c & 1]);
             }
           } else {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) accm[g][nt][c & 1] = fmaf(s[nt][c], c < 2 ? ca : cb, accm[g][nt][c & 1]);
+            for (int c = 0; c < 4; ++c) accm[g][nt][c & 1] = fmaf(s[nt][c], c < 2 ? ma : mb, accm[g][nt][c & 1]);
           }
         }
         const uint32_t w0 = lds32(st + v_at0[g]), w1 = lds32(st + v_at1[g]);
@@ -357,7 +351,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
           for (int nt = 0; nt < NT; ++nt) {
             bw[nt][0] = movmatrix_trans(pack_f16x2(x[nt][0], x[nt][1]));
             bw[nt][1] = movmatrix_trans(pack_f16x2(x[nt][2], x[nt][3]));
-            mma_f16(accr[g][nt], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, bw[nt][0], bw[nt][1]);
           }
           mma_values<0, NT>(acc[g][0], l0, h0, l8, h8, bw);
           mma_values<1, NT>(acc[g][1], l0, h0, l8, h8, bw);
@@ -371,7 +364,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
             bw[nt][1] = movmatrix_trans(pack_bf16x2(x[nt][2], x[nt][3]));
             mma_bf16_zero(sums[nt], 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, bw[nt][0], bw[nt][1]);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) accr[g][nt][c] += sums[nt][c];
+            for (int c = 0; c < 4; ++c)  // p 8 s: these weights meet n - 8
+              if (x[nt][c] != 0.f) accm[g][nt][c & 1] = fmaf(s[nt][c], 8.f * (c < 2 ? sa : sb), accm[g][nt][c & 1]);
           }
           mma_values_bf16<0, NT>(acc[g][0], l0, h0, l8, h8, bw, sums);
           mma_values_bf16<1, NT>(acc[g][1], l0, h0, l8, h8, bw, sums);
@@ -406,7 +400,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
         const float unit = f[g] == 0.f ? 0.f : 1.f / f[g];
-        m = fmaf(-8.f * unit, accr[g][nt][c], m);
         float* o = so + r * D + g * 64 + 8 * i;
 #pragma unroll
         for (int mm = 0; mm < 4; ++mm) {

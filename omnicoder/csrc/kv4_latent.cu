@@ -2,7 +2,7 @@
 // head reads the same rows of W = r + 64 dims, whose first r dims are the value
 // (r = 512 or 256, groups of 64).  The algebra is that of kv4_heads.cu:
 //   score_t = sum_g s_tg (q_g . n_tg) + sum_g m_tg sum(q_g)
-//   o_d     = sum_t (p_t s_tg) (n_td - 8) + sum_t p_t (m_tg + 8 s_tg)
+//   o_d     = sum_t (p_t s_tg) n_td + sum_t p_t m_tg
 //
 // 16 rows of up to 576 + 512 products per key are too much output for one warp's
 // registers, so the eight warps of a block share a tile of 128 keys: each warp
@@ -154,17 +154,16 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
 #pragma unroll
     for (int c = 0; c < 2; ++c) rs[nt][c] = srs[nt * 8 + 2 * j + c];
 
-  // acc: a value tile holds dims MM and 4 + MM of a lane's eight; accr: sums of the rounded weights;
-  // accm: sums of p (m + 8 s)
+  // acc: a value tile holds dims MM and 4 + MM of a lane's eight; accm: sums of p m
   float f = 0.f;   // the values' power of two; 0 before any
-  float acc[MM][NT][4], accr[NT][4], accm[NT], lsum[NT][2], limit[NT][2], ref[NT][2];
+  float acc[MM][NT][4], accm[NT], lsum[NT][2], limit[NT][2], ref[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
     for (int mm = 0; mm < MM; ++mm)
 #pragma unroll
       for (int c = 0; c < 4; ++c) acc[mm][nt][c] = 0.f;
-    accr[nt][0] = accr[nt][1] = accr[nt][2] = accr[nt][3] = accm[nt] = 0.f;
+    accm[nt] = 0.f;
     lsum[nt][0] = lsum[nt][1] = 0.f;
     limit[nt][0] = limit[nt][1] = -INFINITY;
     ref[nt][0] = ref[nt][1] = 0.f;
@@ -273,7 +272,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
           const float alpha = old == -INFINITY ? 0.f : fast_exp2(ref[nt][c] - now);
           ref[nt][c] = now;
           lsum[nt][c] *= alpha;
-          accr[nt][c] *= alpha;
           if (warp == 0 && i == 0) sal[q] = alpha;
 #pragma unroll
           for (int mm = 0; mm < MM; ++mm) {
@@ -323,11 +321,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                accr[nt][c] *= move;
+              for (int c = 0; c < 4; ++c)
 #pragma unroll
                 for (int mm = 0; mm < MM; ++mm) acc[mm][nt][c] *= move;
-              }
           }
         }
         fit = true;
@@ -345,8 +341,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
       const uint32_t w0 = lds32(c0), w1 = lds32(c1), w8 = lds32(c0 + 8 * C::kRow), w9 = lds32(c1 + 8 * C::kRow);
       const uint32_t u0 = lds32(q0), u1 = lds32(q1), u8 = lds32(q0 + 8 * NG * 4), u9 = lds32(q1 + 8 * NG * 4);
       const float s0 = bf16_lo(u0), s1 = bf16_lo(u1), s8 = bf16_lo(u8), s9 = bf16_lo(u9);
-      const float m0 = fmaf(8.f, s0, bf16_hi(u0)), m1 = fmaf(8.f, s1, bf16_hi(u1));
-      const float m8 = fmaf(8.f, s8, bf16_hi(u8)), m9 = fmaf(8.f, s9, bf16_hi(u9));
+      const float m0 = bf16_hi(u0), m1 = bf16_hi(u1), m8 = bf16_hi(u8), m9 = bf16_hi(u9);
       const float f0 = s0 * f, f1 = s1 * f, f8 = s8 * f, f9 = s9 * f;
       float x[NT][4];
 #pragma unroll
@@ -377,7 +372,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
         for (int nt = 0; nt < NT; ++nt) {
           bw[nt][0] = pack_f16x2(x[nt][0], x[nt][1]);
           bw[nt][1] = pack_f16x2(x[nt][2], x[nt][3]);
-          mma_f16(accr[nt], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, bw[nt][0], bw[nt][1]);
         }
         mma_values<0, NT>(acc[0], l0, h0, l8, h8, bw);
         mma_values<1, NT>(acc[1], l0, h0, l8, h8, bw);
@@ -392,8 +386,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
           bw[nt][0] = pack_bf16x2(x[nt][0], x[nt][1]);
           bw[nt][1] = pack_bf16x2(x[nt][2], x[nt][3]);
           mma_bf16_zero(sums[nt], 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, bw[nt][0], bw[nt][1]);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) accr[nt][c] += sums[nt][c];
+          // p 8 s: these weights meet n - 8
+          accm[nt] = fmaf(8.f / f, (x[nt][0] + x[nt][1]) + (x[nt][2] + x[nt][3]), accm[nt]);
         }
         mma_values_bf16<0, NT>(acc[0], l0, h0, l8, h8, bw, sums);
         mma_values_bf16<1, NT>(acc[1], l0, h0, l8, h8, bw, sums);
@@ -421,7 +415,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
       for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
       if (i == 0) smx[warp * kRows + nt * 8 + 2 * j + c] = l;
     }
-  // sums of p (m + 8 s): lane (i, j) holds row i over the keys of j
+  // sums of p m: lane (i, j) holds row i over the keys of j
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     float m = accm[nt];
@@ -443,7 +437,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
       for (int w = 0; w < kWarps; ++w) l += smx[w * kRows + q];
       const float inv = !alone ? 1.f : (l == 0.f ? 0.f : 1.f / l);
       const float unit = f == 0.f ? 0.f : 1.f / f;
-      const float m = fmaf(-8.f * unit, accr[nt][c], sp[warp * kRows + q]);
+      const float m = sp[warp * kRows + q];
       const int d = vg * 64 + 8 * i + (v_shift >> 2);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {  // dims d .. d + MM - 1, then the same 4 up

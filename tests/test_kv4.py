@@ -5,7 +5,8 @@ Tolerances.  Codes and parameters are whole numbers and stored bf16 values: equa
 is exact in fp32, so the kernel's fused form and the plain one round the same number: equal.
 Attention: with w the softmax weights, an output element is off by
     its own rounding                              eps / 2 * |o|
-    the rounding of each weight times its scale   2^-8 * w * s * |n - 8|, at most 2^-8 * w * 8 s
+    the rounding of each weight times its scale   2^-11 * w * s * n in fp16, 2^-8 * w * s * |n - 8| in
+                                                  bf16: both at most 2^-8 * w * 8 s
     the error ds of the scores, which changes each weight by a factor within 1 +- 2 ds:
         2 ds * sum w |v|,  ds = (W + 16) * 2^-23 * scale * max_t sum_d |q_d| (15 s + |m|)
         (fp32 sums of W products, none larger than that sum)
@@ -335,6 +336,34 @@ def test_attention_extreme_values(H, Hk, W, latent):
                                       scale=2.0 ** -18)
     _check_attention(q, kc, kp, vc, vp, q_pos, kv_len, latent=latent, scale=2.0 ** -18)
     assert torch.isfinite(out).all() and torch.isfinite(want).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,Hk,W,latent", [(8, 8, 128, 0), (48, 8, 128, 0), (4, 2, 64, 0), (16, 1, 576, 512), (16, 1, 320, 256)])
+@pytest.mark.parametrize("far", [2.0 ** 9, 2.0 ** 40])
+def test_attention_scales_far_apart(H, Hk, W, latent, far):
+    """Neighbouring rows whose values differ by 2^9 (still one power of two for all) and 2^40 (not any
+    more): the large ones carry weights of e^-120, the small ones the result; then the other way
+    round, row after row and in long runs."""
+    kw = dict(latent=latent, scale=0.5)
+    for period, big_first in ((3, False), (3, True), (128, False), (128, True)):
+        q, kc, kp, vc, vp, q_pos, kv_len = _attend_case(2, 2, H, Hk, W, latent, 700, seed=18, lens=[700, 333])
+        big = (torch.arange(kc.shape[2], device="cuda") // max(1, period // 3)) % 3 == 0
+        seen = ~big if not big_first else big
+        level = torch.where(seen, 60.0, -60.0).to(torch.bfloat16)       # logits of the rows
+        g = W // kp.shape[3]
+        q.zero_()
+        if latent:
+            q[..., latent] = 2.0                                        # one rope dim against constant groups
+            kp[:, :, :, latent // g:, 0], kp[:, :, :, latent // g:, 1] = 0, level[None, None, :, None]
+            kp[:, :, big, :latent // g] *= far
+        else:
+            q[..., 0] = 2.0
+            kp[..., 0], kp[..., 1] = 0, level[None, None, :, None]
+            vp[:, :, big] *= far
+        out, want = _check_attention(q, kc, kp, vc, vp, q_pos, kv_len, **kw)
+        # weights of one size, at most 700: half a step of the output and 2^-8 of eight scales
+        assert (out.double() - want).abs().max() <= 2.0 ** -7 * want.abs().max()
 
 
 @pytest.mark.gpu
