@@ -369,10 +369,10 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv4_row_kernel(const Kv4Attend
 #pragma unroll
   for (int i = 0; i < kRowDims; ++i) o[i] = 0.f;
   float mx = -INFINITY, sum = 0.f;
-  const int tiles = (a.L + 31) / 32;
-  for (int tile = warp; tile < tiles; tile += kRowWarps) {
-    const int r0 = tile * 32;
-    if (r0 >= a.n_sink && (r0 + 32 <= seen.lo || r0 >= seen.hi)) continue;
+  Kv4Piece piece;
+  kv4_tiles<32>(a, seen, &piece);
+  for (int tile = warp; tile < piece.tiles; tile += kRowWarps) {
+    const int r0 = (tile < piece.sink_tiles ? tile : piece.first + tile - piece.sink_tiles) * 32;
     const int r = r0 + lane;
     const bool vis = r < a.n_sink || (r >= seen.lo && r < seen.hi);
     float s = -INFINITY;

@@ -101,7 +101,8 @@ Kv4Line kv4_line(const Kv4Attend& a, const Kv4Plan& p) {
 void kv4_line_plan(const Kv4Attend& a, Kv4Plan& p, int slots, int min_steps) {
   const long long rows = a.n_sink + std::min<long long>(a.L - a.sink_rows, a.window > 0 ? (long long)a.window + a.Tn : 1 << 30);
   const long long steps = (rows + kKv4Step - 1) / kKv4Step, segments = (long long)a.B * a.Hk * p.row_blocks;
-  if (steps <= 2 || a.B > kKv4MaxLine || a.Tn > 16 || segments * (steps + 1) > (1 << 30)) {
+  if (steps <= 2 || a.B > kKv4MaxLine || a.Tn > 16 || segments * (steps + 1) > (1 << 30) ||
+      (long long)a.B * a.Tn * a.H * a.V > (1 << 30)) {
     p.min_steps = 0;
     p.blocks = (int)segments;
     p.floats = 0;

@@ -189,7 +189,7 @@ class KVCache:
         """Dequantised (k, v) of a layer (MLA: latent, None)."""
         dtype = dtype or self.dtype
         if self.kv_dtype == "int4":          # head-major storage -> [B, L, Hk, D] (MLA: [B, L, r + dr])
-            rows = torch.arange(self.k[layer].shape[2], device=self.device).expand(self.batch, -1)
+            rows = torch.arange(self.sink + self.max_len, device=self.device).expand(self.batch, -1)
             if self.mla:
                 return kv4_read(rows, self.k[layer], self.ks[layer], dtype=dtype)[:, :, 0], None
             return kv4_read(rows, self.k[layer], self.ks[layer], self.v[layer], self.vs[layer], dtype=dtype)

@@ -3,8 +3,9 @@ store -- the reference's KV-cache formats (src/omnicoder/modeling/quant/
 kv_cache.py:46-257), used for export sidecars and ONNX-runtime style paging.
 
 The batched decode path of this framework keeps its cache in int8 with one
-symmetric scale per token (and head) instead (omnicoder.inference.kv_cache),
-which the decode attention kernel dequantises in its inner loop.
+symmetric scale per token (and head) instead (omnicoder.inference.kv_cache), or in
+4 bits with a scale and minimum per group (omnicoder.ops.kv4), which the decode
+attention kernels dequantise in their inner loops.
 
 Formats (last dim split in groups of `group_size`, padded with zeros):
   u8   scale = (max - min) / 255, zero = round(-min / scale) in [0, 255],

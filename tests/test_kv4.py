@@ -535,7 +535,7 @@ def test_model_on_cpu(kind, attn):
     for x, y in zip(a.out, b.out):
         assert (x - y).abs().max() <= 1e-4 * y.abs().max()
     k4, v4 = a.layer_kv(1)
-    assert k4.shape[:2] == (2, 64) and (v4 is None) == a.mla
+    assert k4.shape[:2] == (2, 40) and (v4 is None) == a.mla
     assert torch.allclose(k4[:, :18], b.layer_kv(1)[0][:, :18], atol=1e-3)   # layer 1's inputs differ by fp32 sums
 
 
