@@ -7,7 +7,8 @@
 // 16 rows of up to 576 + 512 products per key are too much output for one warp's
 // registers, so the eight warps of a block share a tile of 128 keys: each warp
 // scores 16 of them over all groups, then the weights go through shared memory
-// and each warp accumulates an eighth of the value dims over all 128.  A tile is
+// and each warp accumulates one group of the value dims over all 128 (r = 256: over
+// half of them).  A tile is
 // one contiguous piece of memory and arrives by two bulk copies on an mbarrier.
 // The sum over groups of m sum(q_g) is a product of its own, keys x groups, with
 // m in bf16 as stored and sum(q_g) split into three bf16 terms: nine
@@ -34,7 +35,8 @@ template <int V>
 struct LatentCfg {
   static constexpr int W = V + 64;
   static constexpr int NG = W / 64;                  // key groups
-  static constexpr int MM = V / 16 / kWarps;         // 16-dim value tiles of a warp: 4 (a group) or 2 (half of one)
+  static constexpr int VG = V / 64;                  // value groups: one per warp,
+  static constexpr int KS = kWarps / VG;             // or per pair of warps that halve the keys
   static constexpr int kRow = W / 2;
   static constexpr int kCodes = kTile * kRow;
   static constexpr int kParams = kTile * NG * 4;
@@ -48,7 +50,7 @@ struct LatentCfg {
 template <int V, int TYPE>
 __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Attend a, const Kv4Line line, StatusBlock* st) {
   using C = LatentCfg<V>;
-  constexpr int W = C::W, NG = C::NG, MM = C::MM;
+  constexpr int W = C::W, NG = C::NG, KS = C::KS;
   extern __shared__ __align__(128) uint8_t smem[];
   uint2* sqf = reinterpret_cast<uint2*>(smem + C::kQf);
   float* sp = reinterpret_cast<float*>(smem + C::kP);
@@ -156,11 +158,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
 
   // acc: a value tile holds dims MM and 4 + MM of a lane's eight; accm: sums of p m
   float f = 0.f;   // the values' power of two; 0 before any
-  float acc[MM][NT][4], accm[NT], lsum[NT][2], limit[NT][2], ref[NT][2];
+  float acc[4][NT][4], accm[NT], lsum[NT][2], limit[NT][2], ref[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-    for (int mm = 0; mm < MM; ++mm)
+    for (int mm = 0; mm < 4; ++mm)
 #pragma unroll
       for (int c = 0; c < 4; ++c) acc[mm][nt][c] = 0.f;
     accm[nt] = 0.f;
@@ -172,8 +174,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
   // Row t of an mma tile of 16 keys is key t ^ bit2(t): the rows that one load touches then start in
   // different 32-byte slots of the banks (rows are 32 bytes apart modulo 128).
   const int key_i = i ^ ((i >> 2) & 1);
-  // this warp's value group; the upper half of its nibbles for the odd warp of a pair that shares one
-  const int vg = warp * MM / 4, v_shift = MM == 4 ? 0 : (warp & 1) * 8;
+  // this warp's value group and, of the tile's key tiles, its share
+  const int vg = warp % C::VG, kt0 = warp / C::VG * (kTile / 16 / KS);
   const int key_0 = (2 * j) ^ ((j >> 1) & 1), key_1 = (2 * j + 1) ^ ((j >> 1) & 1);
 
   for (int tile = t0; tile < t1; ++tile) {
@@ -274,7 +276,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
           lsum[nt][c] *= alpha;
           if (warp == 0 && i == 0) sal[q] = alpha;
 #pragma unroll
-          for (int mm = 0; mm < MM; ++mm) {
+          for (int mm = 0; mm < 4; ++mm) {
             acc[mm][nt][c] *= alpha;
             acc[mm][nt][c + 2] *= alpha;
           }
@@ -295,14 +297,15 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
       }
     __syncthreads();
 
-    // ---- do the scales of the tile's values fit their power of two?  Lane: keys lane + 32 k ----
+    // ---- do the scales of the tile's values fit their power of two?  Lane: every 32nd of the warp's keys ----
     bool slow = false;
     {
-      float sc[kTile / 32];
-      bool used[kTile / 32], fit = true;
+      constexpr int kOwn = kTile / 32 / KS;   // keys per lane
+      float sc[kOwn];
+      bool used[kOwn], fit = true;
 #pragma unroll
-      for (int k = 0; k < kTile / 32; ++k) {
-        const int r = lane + 32 * k;
+      for (int k = 0; k < kOwn; ++k) {
+        const int r = kt0 * 16 + lane + 32 * k;
         sc[k] = bf16_lo(lds32(params + (r * NG + vg) * 4));
         used[k] = !masked || r0 + r < a.n_sink || (r0 + r >= see.lo_min && r0 + r < see.hi_max);
         fit = fit && (!used[k] || kv4_in_range(sc[k], f));
@@ -310,7 +313,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
       if (!__all_sync(0xffffffffu, fit)) {
         uint32_t e = 0;
 #pragma unroll
-        for (int k = 0; k < kTile / 32; ++k)
+        for (int k = 0; k < kOwn; ++k)
           if (used[k] && sc[k] <= 3.4e38f) e = max(e, __float_as_uint(sc[k]) >> 23);
         e = __reduce_max_sync(0xffffffffu, e);
         if (e > 0) {  // largest scale in [2^3, 2^4); sums made before move along
@@ -323,18 +326,18 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
 #pragma unroll
               for (int c = 0; c < 4; ++c)
 #pragma unroll
-                for (int mm = 0; mm < MM; ++mm) acc[mm][nt][c] *= move;
+                for (int mm = 0; mm < 4; ++mm) acc[mm][nt][c] *= move;
           }
         }
         fit = true;
 #pragma unroll
-        for (int k = 0; k < kTile / 32; ++k) fit = fit && (!used[k] || kv4_in_range(sc[k], f));
+        for (int k = 0; k < kOwn; ++k) fit = fit && (!used[k] || kv4_in_range(sc[k], f));
         slow = !__all_sync(0xffffffffu, fit);
       }
     }
-    // ---- output: this warp's value dims over all keys of the tile ---------------------
+    // ---- output: this warp's value dims over its keys of the tile ---------------------
 #pragma unroll 1
-    for (int kt = 0; kt < kTile / 16; ++kt) {
+    for (int kt = kt0; kt < kt0 + kTile / 16 / KS; ++kt) {
       const uint32_t c0 = codes + (kt * 16 + key_0) * C::kRow + i * 4 + vg * 32;
       const uint32_t c1 = codes + (kt * 16 + key_1) * C::kRow + i * 4 + vg * 32;
       const uint32_t q0 = params + ((kt * 16 + key_0) * NG + vg) * 4, q1 = params + ((kt * 16 + key_1) * NG + vg) * 4;
@@ -363,9 +366,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
           accm[nt] = fmaf(p0.x, m0, fmaf(p0.y, m1, fmaf(p8.x, m8, fmaf(p8.y, m9, accm[nt]))));
         }
       }
-      uint32_t l0 = __byte_perm(w0, w1, 0x5410), h0 = __byte_perm(w0, w1, 0x7632);
-      uint32_t l8 = __byte_perm(w8, w9, 0x5410), h8 = __byte_perm(w8, w9, 0x7632);
-      if (MM == 2) l0 >>= v_shift, h0 >>= v_shift, l8 >>= v_shift, h8 >>= v_shift;
+      const uint32_t l0 = __byte_perm(w0, w1, 0x5410), h0 = __byte_perm(w0, w1, 0x7632);
+      const uint32_t l8 = __byte_perm(w8, w9, 0x5410), h8 = __byte_perm(w8, w9, 0x7632);
       uint32_t bw[NT][2];
       if (!slow) {
 #pragma unroll
@@ -375,10 +377,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
         }
         mma_values<0, NT>(acc[0], l0, h0, l8, h8, bw);
         mma_values<1, NT>(acc[1], l0, h0, l8, h8, bw);
-        if (MM == 4) {
-          mma_values<2, NT>(acc[MM - 2], l0, h0, l8, h8, bw);
-          mma_values<3, NT>(acc[MM - 1], l0, h0, l8, h8, bw);
-        }
+        mma_values<2, NT>(acc[2], l0, h0, l8, h8, bw);
+        mma_values<3, NT>(acc[3], l0, h0, l8, h8, bw);
       } else {
         float sums[NT][4];
 #pragma unroll
@@ -391,10 +391,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
         }
         mma_values_bf16<0, NT>(acc[0], l0, h0, l8, h8, bw, sums);
         mma_values_bf16<1, NT>(acc[1], l0, h0, l8, h8, bw, sums);
-        if (MM == 4) {
-          mma_values_bf16<2, NT>(acc[MM - 2], l0, h0, l8, h8, bw, sums);
-          mma_values_bf16<3, NT>(acc[MM - 1], l0, h0, l8, h8, bw, sums);
-        }
+        mma_values_bf16<2, NT>(acc[2], l0, h0, l8, h8, bw, sums);
+        mma_values_bf16<3, NT>(acc[3], l0, h0, l8, h8, bw, sums);
       }
     }
     if (tile + kStages < t1) {
@@ -426,36 +424,52 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
   __syncthreads();
   const bool alone = t0 == 0 && piece.step1 == piece.steps;
   float* part = a.part + (size_t)(2 * blockIdx.x + (t0 == 0)) * kRows * (V + 2);
+  const float unit = f == 0.f ? 0.f : 1.f / f;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int mm = 0; mm < 4; ++mm)
+        acc[mm][nt][c] = fmaf(acc[mm][nt][c], unit * value_unit(mm), sp[warp * kRows + nt * 8 + 2 * j + (c & 1)]);
+  if (KS == 2) {  // the stages' memory is free: the second warp of a pair hands over its sums
+    float* to = reinterpret_cast<float*>(smem) + (warp % C::VG) * 32 * 32 + lane;
+#pragma unroll
+    for (int n = 0; n < 32; ++n)
+      if (warp >= C::VG) to[n * 32] = acc[n >> 3][(n >> 2) & 1][n & 3];
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < 32; ++n)
+      if (warp < C::VG) acc[n >> 3][(n >> 2) & 1][n & 3] += to[n * 32];
+  }
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int q = nt * 8 + 2 * j + c;
-      if (q >= nrows) continue;
+      if (q >= nrows || warp >= C::VG) continue;
       float l = 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) l += smx[w * kRows + q];
       const float inv = !alone ? 1.f : (l == 0.f ? 0.f : 1.f / l);
-      const float unit = f == 0.f ? 0.f : 1.f / f;
-      const float m = sp[warp * kRows + q];
-      const int d = vg * 64 + 8 * i + (v_shift >> 2);
+      const int d = vg * 64 + 8 * i;
+      float o[8];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {  // dims d .. d + MM - 1, then the same 4 up
-        float o[MM];
-#pragma unroll
-        for (int mm = 0; mm < MM; ++mm) o[mm] = fmaf(acc[mm][nt][c + 2 * h], unit * value_unit(mm), m) * inv;
-        if (!alone) {
-          float* p = part + q * V + d + 4 * h;
-          if (MM == 4) *reinterpret_cast<float4*>(p) = make_float4(o[0], o[1], o[MM - 2], o[MM - 1]);
-          else *reinterpret_cast<float2*>(p) = make_float2(o[0], o[1]);
-        } else {
-          uint16_t* p = reinterpret_cast<uint16_t*>(a.out) + ((long long)b * R + row0 + q) * V + d + 4 * h;
-          if (MM == 4) *reinterpret_cast<uint2*>(p) = make_uint2(kv4_pack2<TYPE>(o[0], o[1]), kv4_pack2<TYPE>(o[MM - 2], o[MM - 1]));
-          else *reinterpret_cast<uint32_t*>(p) = kv4_pack2<TYPE>(o[0], o[1]);
-        }
+      for (int mm = 0; mm < 4; ++mm) {
+        o[mm] = acc[mm][nt][c] * inv;
+        o[4 + mm] = acc[mm][nt][c + 2] * inv;
       }
-      if (!alone && warp == 0 && i == 0)
-        *reinterpret_cast<float2*>(part + kRows * V + 2 * q) = make_float2(limit[nt][c] == -INFINITY ? -INFINITY : ref[nt][c], l);
+      if (!alone) {
+        float4* p = reinterpret_cast<float4*>(part + q * V + d);
+        p[0] = make_float4(o[0], o[1], o[2], o[3]);
+        p[1] = make_float4(o[4], o[5], o[6], o[7]);
+        if (warp == 0 && i == 0)
+          *reinterpret_cast<float2*>(part + kRows * V + 2 * q) = make_float2(limit[nt][c] == -INFINITY ? -INFINITY : ref[nt][c], l);
+      } else {
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + ((long long)b * R + row0 + q) * V + d) =
+            make_uint4(kv4_pack2<TYPE>(o[0], o[1]), kv4_pack2<TYPE>(o[2], o[3]), kv4_pack2<TYPE>(o[4], o[5]),
+                       kv4_pack2<TYPE>(o[6], o[7]));
+      }
     }
   __syncthreads();  // the next segment refills shared memory
   }
