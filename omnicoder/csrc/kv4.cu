@@ -175,6 +175,8 @@ __device__ __forceinline__ bool kv4_near_border(const float* x, float m, float i
 
 template <int TYPE>
 __global__ void __launch_bounds__(kIoThreads) kv4_write_kernel(const Kv4IO a, const IoGrid g) {
+  wait_for_previous_grid();
+  launch_dependents();
   const int b = blockIdx.y, r_in = g.pieces.of(threadIdx.x), piece = threadIdx.x - r_in * g.pieces.d;
   const Kv4Cache& c = a.cache[blockIdx.z];
   const Kv4Rows& src = a.rows[blockIdx.z];
@@ -263,6 +265,8 @@ __global__ void __launch_bounds__(kIoThreads) kv4_write_kernel(const Kv4IO a, co
 
 template <int TYPE>
 __global__ void __launch_bounds__(kIoThreads) kv4_read_kernel(const Kv4IO a, const IoGrid g) {
+  wait_for_previous_grid();
+  launch_dependents();
   const int b = blockIdx.y, r_in = g.pieces.of(threadIdx.x), piece = threadIdx.x - r_in * g.pieces.d;
   if (r_in >= g.rows_per_pass) return;
   const Kv4Cache& c = a.cache[blockIdx.z];
@@ -349,6 +353,8 @@ constexpr int kRowDims = 32;  // value dims of a lane: V <= 1024
 
 template <int TYPE>
 __global__ void __launch_bounds__(kRowWarps * 32) kv4_row_kernel(const Kv4Attend a) {
+  wait_for_previous_grid();
+  launch_dependents();
   extern __shared__ float sm[];
   float* sq = sm;                              // [W]
   float* so = sq + a.W;                        // [kRowWarps][V]
@@ -443,7 +449,7 @@ void launch_rows(const Kv4Attend& a, cudaStream_t s) {
   auto kern = kv4_row_kernel<TYPE>;
   const int smem = (a.W + kRowWarps * (a.V + 2)) * 4;
   ensure_smem_attr(reinterpret_cast<const void*>(kern), smem);
-  kern<<<dim3((unsigned)(a.Tn * a.H), (unsigned)a.B), kRowWarps * 32, smem, s>>>(a);
+  kv4_launch(kern, dim3((unsigned)(a.Tn * a.H), (unsigned)a.B), kRowWarps * 32, smem, s, a);
 }
 
 }  // namespace
@@ -451,17 +457,17 @@ void launch_rows(const Kv4Attend& a, cudaStream_t s) {
 void kv4_write(const Kv4IO& a, cudaStream_t s) {
   IoGrid g{Kv4Div(1), Kv4Div(1), 0, 0, 0, 0, 0};
   const dim3 grid = io_grid(a, &g);
-  if (a.type == KV4_F32) kv4_write_kernel<KV4_F32><<<grid, kIoThreads, 0, s>>>(a, g);
-  else if (a.type == KV4_F16) kv4_write_kernel<KV4_F16><<<grid, kIoThreads, 0, s>>>(a, g);
-  else kv4_write_kernel<KV4_BF16><<<grid, kIoThreads, 0, s>>>(a, g);
+  if (a.type == KV4_F32) kv4_launch(kv4_write_kernel<KV4_F32>, grid, kIoThreads, 0, s, a, g);
+  else if (a.type == KV4_F16) kv4_launch(kv4_write_kernel<KV4_F16>, grid, kIoThreads, 0, s, a, g);
+  else kv4_launch(kv4_write_kernel<KV4_BF16>, grid, kIoThreads, 0, s, a, g);
 }
 
 void kv4_read(const Kv4IO& a, cudaStream_t s) {
   IoGrid g{Kv4Div(1), Kv4Div(1), 0, 0, 0, 0, 0};
   const dim3 grid = io_grid(a, &g);
-  if (a.type == KV4_F32) kv4_read_kernel<KV4_F32><<<grid, kIoThreads, 0, s>>>(a, g);
-  else if (a.type == KV4_F16) kv4_read_kernel<KV4_F16><<<grid, kIoThreads, 0, s>>>(a, g);
-  else kv4_read_kernel<KV4_BF16><<<grid, kIoThreads, 0, s>>>(a, g);
+  if (a.type == KV4_F32) kv4_launch(kv4_read_kernel<KV4_F32>, grid, kIoThreads, 0, s, a, g);
+  else if (a.type == KV4_F16) kv4_launch(kv4_read_kernel<KV4_F16>, grid, kIoThreads, 0, s, a, g);
+  else kv4_launch(kv4_read_kernel<KV4_BF16>, grid, kIoThreads, 0, s, a, g);
 }
 
 Kv4Plan kv4_plan(const Kv4Attend& a) {

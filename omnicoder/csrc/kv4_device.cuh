@@ -373,9 +373,25 @@ __device__ __forceinline__ Kv4Rows4 kv4_rows(const Kv4Attend& a, const Kv4Line& 
   return r;
 }
 
-// The kernel that joins the pieces may start its blocks early; they wait for this one's end.
+// Every kernel of this family may be set up while its predecessor in the stream still runs: it
+// waits for that one's end, and its memory, before it touches any.
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous_grid() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... Params, typename... Args>
+void kv4_launch(void (*kernel)(Params...), dim3 grid, int threads, int smem, cudaStream_t s, Args... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = s;
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, args...);
+}
 
 // Grid and workspace: slots blocks stay resident, shares of at least min_steps.
 void kv4_line_plan(const Kv4Attend& a, Kv4Plan& p, int slots, int min_steps);

@@ -64,7 +64,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
   float* srs = sqs + C::kRows * NG;                                         // [kRows]: factor of the scores
   const int lane = lane_id(), warp = warp_id(), i = lane >> 2, j = lane & 3;
   const uint32_t ring = smem_u32(smem) + warp * C::kStages * C::kStage;
-  if (line.min_steps > 0) launch_dependents();
+  wait_for_previous_grid();
+  launch_dependents();
   __shared__ Kv4Walk walk;
   int share = 0;
   int2 span = walk.begin<kWarps * 32, kTile>(a, line, &share);
@@ -444,7 +445,7 @@ void launch(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s) {
   auto kern = kv4_heads_kernel<D, NT, TYPE>;
   constexpr int smem = HeadsCfg<D, NT>::kSmem;
   ensure_smem_attr(reinterpret_cast<const void*>(kern), smem);
-  kern<<<p.blocks, kWarps * 32, smem, s>>>(a, kv4_line(a, p));
+  kv4_launch(kern, dim3((unsigned)p.blocks), kWarps * 32, smem, s, a, kv4_line(a, p));
 }
 
 template <int TYPE>

@@ -67,7 +67,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
     for (int k = 0; k < kStages; ++k) mbar_init(&full[k], 1);
     fence_barrier_init();
   }
-  if (line.min_steps > 0) launch_dependents();
+  wait_for_previous_grid();
+  launch_dependents();
   __shared__ Kv4Walk walk;
   int share = 0;
   int2 span = walk.begin<kWarps * 32, kTile>(a, line, &share);
@@ -481,8 +482,8 @@ void launch(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s) {
   auto kern = kv4_latent_kernel<V, TYPE>;
   constexpr int smem = LatentCfg<V>::kSmem;
   ensure_smem_attr(reinterpret_cast<const void*>(kern), smem);
-  kern<<<p.blocks, kWarps * 32, smem, s>>>(a, kv4_line(a, p),
-                                           reinterpret_cast<StatusBlock*>(status_ptr()));
+  kv4_launch(kern, dim3((unsigned)p.blocks), kWarps * 32, smem, s, a, kv4_line(a, p),
+             reinterpret_cast<StatusBlock*>(status_ptr()));
 }
 
 }  // namespace

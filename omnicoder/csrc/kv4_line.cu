@@ -23,6 +23,7 @@ __global__ void __launch_bounds__(kThreads) kv4_combine_kernel(const Kv4Attend a
   const int head = line.rows.of(place), row = place - head * line.rows.d, t = line.group.of(row);
   const int r = row & (rows_per_block - 1), b = head / a.Hk, hk = head - b * a.Hk;
   wait_for_previous_grid();
+  launch_dependents();
   int2 range = make_int2(0, 0);
   if (b < a.B) range = line.meta[b * line.segments.d + hk * line.row_blocks.d + row / rows_per_block];
   const bool join = range.x != range.y;  // otherwise one block held the segment and has written the row
@@ -74,16 +75,8 @@ __global__ void __launch_bounds__(kThreads) kv4_combine_kernel(const Kv4Attend a
 template <int TYPE, int GROUPS>
 void launch(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s) {
   const long long items = (long long)a.B * a.Tn * a.H * (a.V / 4), per = kThreads / GROUPS;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((items + per - 1) / per));
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = s;
-  cudaLaunchAttribute early{};
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &early;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, kv4_combine_kernel<TYPE, GROUPS>, a, kv4_line(a, p), Kv4Div(a.V / 4), 8 * p.row_tiles);
+  kv4_launch(kv4_combine_kernel<TYPE, GROUPS>, dim3((unsigned)((items + per - 1) / per)), kThreads, 0, s, a, kv4_line(a, p),
+             Kv4Div(a.V / 4), 8 * p.row_tiles);
 }
 
 }  // namespace
