@@ -55,7 +55,7 @@ struct Kv4Plan {
   int row_tiles;         // 8-row query tiles per block
   int row_blocks;        // blocks that share a key / value head's query rows
   int blocks;            // grid: blocks that share the key tiles of all of them
-  int min_steps;         // smallest share of a block, in steps of 128 keys; 0: a block per (sequence, head, rows)
+  int restart;           // what a block's start costs it, in steps of 128 keys; 0: a block per (sequence, head, rows)
   size_t floats;         // workspace
 };
 Kv4Plan kv4_plan(const Kv4Attend& a);

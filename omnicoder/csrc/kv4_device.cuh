@@ -213,13 +213,17 @@ __device__ __forceinline__ void kv4_load8(const void* base, long long i, float* 
 
 // ---- work of the blocks ---------------------------------------------------------
 // A segment is (sequence, key / value head, row block): its keys are walked in
-// steps of 128 rows.  Few short segments: a block each.  Otherwise the steps of
-// all segments form one line that the blocks share in equal consecutive pieces,
-// so that uneven lengths and segment counts that do not fill the GPU cost
-// nothing.  A block then holds at most two pieces that it shares with others,
-// the first (of a segment begun by an earlier block) and the last; those go to
-// slots 2 * block and 2 * block + 1 of the workspace, and the block that begins a
-// segment notes its first and last block for the kernel that joins them.
+// steps of 128 rows.  Few steps, or very many segments: a block each.  Otherwise
+// the blocks that stay resident share them in one of two ways, chosen on the
+// device from the lengths:
+//   - every segment in equal parts, a block each;
+//   - the steps of all segments in one line, cut into equal consecutive pieces,
+//     so that uneven lengths and segment counts that do not fill the GPU cost
+//     nothing, but a block that goes on to a second segment starts anew.
+// A block then holds at most two pieces that it shares with others, the first (of
+// a segment begun by an earlier block) and the last; those go to slots 2 * block
+// and 2 * block + 1 of the workspace, and the block that begins a segment notes
+// its first and last block for the kernel that joins them.
 constexpr int kKv4Step = 128;
 
 // n / d for 0 <= n < 2^31 as a multiplication.
@@ -236,8 +240,10 @@ struct Kv4Div {
 struct Kv4Line {
   Kv4Div segments;    // of one sequence: Hk * row_blocks
   Kv4Div row_blocks, group, rows;  // row blocks of a head, heads that share one, query rows of it: Tn * group
-  int min_steps;      // smallest share of a block; 0: a block per segment
+  int restart;        // what a second segment costs a block, in steps; 0: a block per segment
+  int blocks;
   int2* meta;         // [B * segments] first and last block
+  int* begun;         // [blocks] the segment that begins in a block and goes on in others, or -1
 };
 
 constexpr int kKv4MaxLine = 256;   // sequences on a line
@@ -273,14 +279,15 @@ __device__ __forceinline__ void kv4_tiles(const Kv4Attend& a, Kv4Seen u, Kv4Piec
 // The pieces of one block, in turn; every thread of the block calls both functions.
 // Shared memory: for each sequence the steps up to its end, its first tile and its tiles.
 struct Kv4Walk {
-  int end[kKv4MaxLine], first[kKv4MaxLine], tiles[kKv4MaxLine], sums[32];
+  int end[kKv4MaxLine], first[kKv4MaxLine], tiles[kKv4MaxLine], sums[32], most[32];
 
-  // -> first and last step of the block on the line
+  // -> first and last step of the block on the line.  share: steps of a block, or minus the parts
+  // that every segment is cut into
   template <int kThreads, int kTile>
   __device__ __forceinline__ int2 begin(const Kv4Attend& a, const Kv4Line& l, int* share) {
-    if (l.min_steps == 0) return make_int2(0, 1);
+    if (l.restart == 0) return make_int2(0, 1);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    int before = 0;
+    int before = 0, longest = 0;
     for (int b0 = 0; b0 < a.B; b0 += kThreads) {
       Kv4Piece q;
       q.steps = 0;
@@ -291,13 +298,18 @@ struct Kv4Walk {
         const int up = __shfl_up_sync(0xffffffffu, sum, o);
         if (lane >= o) sum += up;
       }
-      if (lane == 31) sums[warp] = sum;
+      const int top = __reduce_max_sync(0xffffffffu, q.steps);
+      if (lane == 31) {
+        sums[warp] = sum;
+        most[warp] = top;
+      }
       __syncthreads();
       int all = before;
 #pragma unroll
       for (int w = 0; w < kThreads / 32; ++w) {
         if (w < warp) sum += sums[w];
         all += sums[w];
+        longest = max(longest, most[w]);
       }
       if (b0 + tid < a.B) {
         end[b0 + tid] = before + sum;
@@ -308,9 +320,15 @@ struct Kv4Walk {
       __syncthreads();
     }
     const int total = before * l.segments.d;
-    *share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, l.min_steps);
-    const int at = blockIdx.x * *share;
-    return make_int2(at, min(total, at + *share));
+    if (threadIdx.x == 0) l.begun[blockIdx.x] = -1;
+    const int blocks = gridDim.x, even = (total + blocks - 1) / blocks, parts = blocks / (a.B * l.segments.d);
+    if (parts > 0 && (longest + parts - 1) / parts <= even + l.restart) {
+      *share = -parts;
+      return make_int2(0, (int)blockIdx.x < a.B * l.segments.d * parts);
+    }
+    *share = even;
+    const int at = blockIdx.x * even;
+    return make_int2(at, min(total, at + even));
   }
 
   // The segment that holds step span.x; moves span.x behind it.  A block per segment: tiles and
@@ -318,10 +336,24 @@ struct Kv4Walk {
   template <int kTile>
   __device__ __forceinline__ Kv4Piece next(const Kv4Attend& a, const Kv4Line& l, int share, int2* span) {
     Kv4Piece p;
-    if (l.min_steps == 0) {
+    if (l.restart == 0) {
       p.b = l.segments.of(blockIdx.x);
       p.segment = blockIdx.x - p.b * l.segments.d;
       p.steps = p.step0 = p.step1 = p.sink_tiles = p.first = p.tiles = 0;
+      span->x = span->y;
+      return p;
+    }
+    p.sink_tiles = (a.n_sink + kTile - 1) / kTile;
+    int last = blockIdx.x;
+    if (share < 0) {
+      const int place = blockIdx.x / -share, part = blockIdx.x + place * share;
+      p.b = l.segments.of(place);
+      p.segment = place - p.b * l.segments.d;
+      p.steps = end[p.b] - (p.b > 0 ? end[p.b - 1] : 0);
+      const int each = (p.steps - share - 1) / -share;
+      p.step0 = min(p.steps, part * each);
+      p.step1 = min(p.steps, p.step0 + each);
+      last += (p.steps - 1) / each;   // of part 0
       span->x = span->y;
     } else {
       int lo = 0, hi = a.B - 1;
@@ -333,16 +365,19 @@ struct Kv4Walk {
       const int start = lo > 0 ? end[lo - 1] : 0;
       p.b = lo;
       p.steps = end[lo] - start;
-      p.first = first[lo];
-      p.tiles = tiles[lo];
-      p.sink_tiles = (a.n_sink + kTile - 1) / kTile;
       p.segment = (span->x - start * l.segments.d) / p.steps;
       const int at = start * l.segments.d + p.segment * p.steps;   // the segment's first step on the line
       p.step0 = span->x - at;
       p.step1 = min(p.steps, span->y - at);
-      if (p.step0 == 0 && threadIdx.x == 0)
-        l.meta[p.b * l.segments.d + p.segment] = make_int2(blockIdx.x, (at + p.steps - 1) / share);
+      last = (at + p.steps - 1) / share;
       span->x = at + p.steps;
+    }
+    p.first = first[p.b];
+    p.tiles = tiles[p.b];
+    if (p.step0 == 0 && threadIdx.x == 0) {
+      const int place = p.b * l.segments.d + p.segment;
+      l.meta[place] = make_int2(blockIdx.x, last);
+      if (last > (int)blockIdx.x) l.begun[blockIdx.x] = place;
     }
     return p;
   }
@@ -366,7 +401,7 @@ __device__ __forceinline__ Kv4Rows4 kv4_rows(const Kv4Attend& a, const Kv4Line& 
   r.hi_max = __reduce_max_sync(0xffffffffu, any ? r.seen.hi : 0);
   r.lo_max = __reduce_max_sync(0xffffffffu, valid ? r.seen.lo : 0);
   r.hi_min = __reduce_min_sync(0xffffffffu, valid ? r.seen.hi : a.L);
-  if (l.min_steps == 0) {
+  if (l.restart == 0) {
     kv4_tiles<kTile>(a, Kv4Seen{r.lo_min, r.hi_max}, p);
     p->step1 = p->steps;
   }
@@ -393,8 +428,8 @@ void kv4_launch(void (*kernel)(Params...), dim3 grid, int threads, int smem, cud
   cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-// Grid and workspace: slots blocks stay resident, shares of at least min_steps.
-void kv4_line_plan(const Kv4Attend& a, Kv4Plan& p, int slots, int min_steps);
+// Grid and workspace: slots blocks stay resident; a block's start costs it about restart steps.
+void kv4_line_plan(const Kv4Attend& a, Kv4Plan& p, int slots, int restart);
 Kv4Line kv4_line(const Kv4Attend& a, const Kv4Plan& p);
 // Joins the pieces: 8 * row_tiles rows of V sums and then (max, sum) pairs per slot.
 void kv4_combine(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s);

@@ -463,13 +463,13 @@ void kv4_heads_plan(const Kv4Attend& a, Kv4Plan& p) {
   p.kernel = 1;
   p.row_tiles = R <= 8 ? 1 : 2;
   p.row_blocks = (R + 8 * p.row_tiles - 1) / (8 * p.row_tiles);
-  kv4_line_plan(a, p, 148 * (p.row_tiles == 1 ? 3 : 2), 1);
+  kv4_line_plan(a, p, 148 * (p.row_tiles == 1 ? 3 : 2), 3);
 }
 
 void kv4_heads_launch(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s) {
   if (a.type == KV4_F16) launch_dims<KV4_F16>(a, p, s);
   else launch_dims<KV4_BF16>(a, p, s);
-  if (p.min_steps > 0) kv4_combine(a, p, s);
+  if (p.restart > 0) kv4_combine(a, p, s);
 }
 
 }  // namespace omni

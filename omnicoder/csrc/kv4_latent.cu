@@ -500,7 +500,7 @@ void kv4_latent_launch(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s) {
     a.V == 512 ? launch<512, KV4_F16>(a, p, s) : launch<256, KV4_F16>(a, p, s);
   else
     a.V == 512 ? launch<512, KV4_BF16>(a, p, s) : launch<256, KV4_BF16>(a, p, s);
-  if (p.min_steps > 0) kv4_combine(a, p, s);
+  if (p.restart > 0) kv4_combine(a, p, s);
 }
 
 }  // namespace omni

@@ -1,6 +1,7 @@
 // How the attention kernels over a 4-bit cache share their keys, and the kernel
 // that joins what they shared.
 #include <algorithm>
+#include <cmath>
 
 #include "kv4_device.cuh"
 
@@ -14,18 +15,34 @@ constexpr int kThreads = 256;
 // piece each and are summed in a fixed order.
 template <int TYPE, int GROUPS>
 __global__ void __launch_bounds__(kThreads) kv4_combine_kernel(const Kv4Attend a, const Kv4Line line, const Kv4Div cols,
-                                                              const int rows_per_block) {
+                                                              const int rows_per_block, const bool by_block) {
   constexpr int kItems = kThreads / GROUPS;
   __shared__ float4 s_sum[kThreads];
   __shared__ float2 s_ml[kThreads];
   const int item = threadIdx.x % kItems, group = threadIdx.x / kItems, at = blockIdx.x * kItems + item;
-  const int place = cols.of(at), col = at - place * cols.d;                      // (sequence, head, row), four dims
-  const int head = line.rows.of(place), row = place - head * line.rows.d, t = line.group.of(row);
-  const int r = row & (rows_per_block - 1), b = head / a.Hk, hk = head - b * a.Hk;
+  const int place0 = cols.of(at), col = at - place0 * cols.d;   // four dims of a row
   wait_for_previous_grid();
   launch_dependents();
+  // by segment: place is (sequence, head, row); by block: (block, row of the segment begun there)
   int2 range = make_int2(0, 0);
-  if (b < a.B) range = line.meta[b * line.segments.d + hk * line.row_blocks.d + row / rows_per_block];
+  int b = 0, hk = 0, row = 0;
+  if (by_block) {
+    const int block = place0 / rows_per_block, segment = block < line.blocks ? line.begun[block] : -1;
+    if (segment >= 0) {
+      b = line.segments.of(segment);
+      const int in = segment - b * line.segments.d;
+      hk = line.row_blocks.of(in);
+      row = (in - hk * line.row_blocks.d) * rows_per_block + place0 % rows_per_block;
+      if (row < line.rows.d) range = line.meta[segment];
+    }
+  } else {
+    const int head = line.rows.of(place0);
+    row = place0 - head * line.rows.d;
+    b = head / a.Hk;
+    hk = head - b * a.Hk;
+    if (b < a.B) range = line.meta[b * line.segments.d + hk * line.row_blocks.d + row / rows_per_block];
+  }
+  const int t = line.group.of(row), r = row & (rows_per_block - 1);
   const bool join = range.x != range.y;  // otherwise one block held the segment and has written the row
   const size_t slot = (size_t)rows_per_block * (a.V + 2);
   float top = -INFINITY, l = 0.f;
@@ -74,42 +91,53 @@ __global__ void __launch_bounds__(kThreads) kv4_combine_kernel(const Kv4Attend a
 
 template <int TYPE, int GROUPS>
 void launch(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s) {
-  const long long items = (long long)a.B * a.Tn * a.H * (a.V / 4), per = kThreads / GROUPS;
+  const long long segments = (long long)a.B * a.Hk * p.row_blocks, rows = 8 * p.row_tiles;
+  const bool by_block = p.blocks < segments;   // at most one shared segment begins in a block
+  const long long items = (by_block ? p.blocks * rows : (long long)a.B * a.Tn * a.H) * (a.V / 4), per = kThreads / GROUPS;
   kv4_launch(kv4_combine_kernel<TYPE, GROUPS>, dim3((unsigned)((items + per - 1) / per)), kThreads, 0, s, a, kv4_line(a, p),
-             Kv4Div(a.V / 4), 8 * p.row_tiles);
+             Kv4Div(a.V / 4), (int)rows, by_block);
 }
 
 }  // namespace
 
 Kv4Line kv4_line(const Kv4Attend& a, const Kv4Plan& p) {
-  const size_t sums = (size_t)p.blocks * 2 * 8 * p.row_tiles * (a.V + 2);
+  const size_t sums = (size_t)p.blocks * 2 * 8 * p.row_tiles * (a.V + 2), segments = (size_t)a.B * a.Hk * p.row_blocks;
   const int group = a.H / a.Hk;
-  return Kv4Line{Kv4Div(a.Hk * p.row_blocks), Kv4Div(p.row_blocks), Kv4Div(group), Kv4Div(a.Tn * group), p.min_steps,
-                 reinterpret_cast<int2*>(a.part + sums)};
+  int2* meta = reinterpret_cast<int2*>(a.part + sums);
+  return Kv4Line{Kv4Div(a.Hk * p.row_blocks), Kv4Div(p.row_blocks), Kv4Div(group), Kv4Div(a.Tn * group), p.restart, p.blocks,
+                 meta, reinterpret_cast<int*>(meta + segments)};
 }
 
-// The host knows the cache's size, not the sequences' lengths.  A block per segment where a full
-// cache (or window) is at most two steps, or where finding a block's place on the line would cost
-// more than uneven lengths: many sequences, many new tokens.
-void kv4_line_plan(const Kv4Attend& a, Kv4Plan& p, int slots, int min_steps) {
+// The host knows the cache's size, not the sequences' lengths, and plans for a full cache (or window).
+// A block per segment costs its steps times the waves of blocks; shared steps cost their share, and
+// about `restart` steps more to find the places and to join the pieces (3 us).  Measured, one query
+// row a sequence, us shared / a block each: 8 heads of 128, 1 sequence of 2, 4, 8 steps 8.4 / 6.2,
+// 8.6 / 8.4, 8.3 / 12.7; 256 sequences of 16 steps 160 / 147; one latent head, 1 sequence of 1, 2, 4
+// steps 11.8 / 9.7, 12.7 / 13.6, 13.2 / 21.4.  Many sequences or new tokens make the places on the
+// line dear to find: a block each.
+void kv4_line_plan(const Kv4Attend& a, Kv4Plan& p, int slots, int restart) {
   const long long rows = a.n_sink + std::min<long long>(a.L - a.sink_rows, a.window > 0 ? (long long)a.window + a.Tn : 1 << 30);
   const long long steps = (rows + kKv4Step - 1) / kKv4Step, segments = (long long)a.B * a.Hk * p.row_blocks;
-  if (steps <= 2 || a.B > kKv4MaxLine || a.Tn > 16 || segments * (steps + 1) > (1 << 30) ||
+  const double waves = (double)segments / slots;
+  const double each = steps * (waves < 4 ? std::ceil(waves) : waves), shared = std::max(1.0, std::ceil(steps * waves)) + restart;
+  if (each <= shared || a.B > kKv4MaxLine || a.Tn > 16 || segments * (steps + 1) > (1 << 30) ||
       (long long)a.B * a.Tn * a.H * a.V > (1 << 30)) {
-    p.min_steps = 0;
+    p.restart = 0;
     p.blocks = (int)segments;
     p.floats = 0;
     return;
   }
-  p.min_steps = min_steps;
-  p.blocks = (int)std::min<long long>(slots, (segments * (steps + 1) + min_steps - 1) / min_steps);
-  p.floats = (size_t)p.blocks * 2 * 8 * p.row_tiles * (a.V + 2) + 2 * (size_t)segments;
+  p.restart = restart;
+  p.blocks = (int)std::min<long long>(slots, segments * (steps + 1));
+  p.floats = (size_t)p.blocks * (2 * 8 * p.row_tiles * (a.V + 2) + 1) + 2 * (size_t)segments;
 }
 
 void kv4_combine(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s) {
-  // a segment has about blocks / segments + 1 pieces
+  // A segment has about blocks / segments + 1 pieces.  Measured, 16 and 2 threads for the pieces of four
+  // dims, us of the whole call: 55 pieces 13.0 / 16.8, 17 pieces 8.8 / 10.9, 5 pieces 8.3 / 8.6 and,
+  // of many rows (32768 times four dims), 9 pieces 19.5 / 14.8, 18 pieces 27.5 / 27.7.
   const long long segments = (long long)a.B * a.Hk * p.row_blocks;
-  const bool many = p.blocks > 6 * segments;
+  const bool many = p.blocks > 6 * segments && (long long)a.B * a.Tn * a.H * (a.V / 4) <= 16384;
   if (a.type == KV4_F16) many ? launch<KV4_F16, 16>(a, p, s) : launch<KV4_F16, 2>(a, p, s);
   else many ? launch<KV4_BF16, 16>(a, p, s) : launch<KV4_BF16, 2>(a, p, s);
 }
