@@ -104,7 +104,8 @@ __device__ __forceinline__ uint32_t nibbles_bf16(uint32_t x) {
 // keys at hand has s f in [2^-8, 2^6], or 0: then x < 2^14 (p < 2^8), its rounding is 2^-11 of it
 // down to 2^-14 and 2^-25 below, 2^-17 of a row's largest weight.  Where the scales of
 // neighbouring keys lie further apart, x is rounded to bf16 instead (slow).
-constexpr float kKv4Low = 0.00390625f, kKv4High = 64.f;
+// Smaller scales raise f only as far as the sums in it leave room for.
+constexpr float kKv4Low = 0.00390625f, kKv4High = 64.f, kKv4Room = 1.2676506e30f;  // 2^100
 
 // f = 0: none yet.  A NaN or an infinity fits any f: it stays one, for the queries that see it.
 __device__ __forceinline__ bool kv4_in_range(float s, float f) {
@@ -384,15 +385,15 @@ struct Kv4Walk {
 };
 
 // What the queries of a block see.  Lane r holds query row r; the other numbers are the warp's.
-struct Kv4Rows4 {
+struct Kv4View {
   Kv4Seen seen;
   int lo_min, hi_max;   // rows that any of them sees
   int lo_max, hi_min;   // rows that all of them see
 };
 
 template <int kTile>
-__device__ __forceinline__ Kv4Rows4 kv4_rows(const Kv4Attend& a, const Kv4Line& l, Kv4Piece* p, int row0, int nrows) {
-  Kv4Rows4 r{Kv4Seen{0, 0}, 0, 0, 0, 0};
+__device__ __forceinline__ Kv4View kv4_rows(const Kv4Attend& a, const Kv4Line& l, Kv4Piece* p, int row0, int nrows) {
+  Kv4View r{Kv4Seen{0, 0}, 0, 0, 0, 0};
   const int lane = lane_id();
   const bool valid = lane < nrows;
   if (valid) r.seen = kv4_seen(a, p->b, l.group.of(row0 + lane));

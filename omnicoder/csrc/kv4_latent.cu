@@ -8,11 +8,17 @@
 // registers, so the eight warps of a block share a tile of 128 keys: each warp
 // scores 16 of them over all groups, then the weights go through shared memory
 // and each warp accumulates one group of the value dims over all 128 (r = 256: over
-// half of them).  A tile is
-// one contiguous piece of memory and arrives by two bulk copies on an mbarrier.
+// half of them).  A tile is one contiguous piece of memory and arrives by two bulk
+// copies on an mbarrier.
 // The sum over groups of m sum(q_g) is a product of its own, keys x groups, with
 // m in bf16 as stored and sum(q_g) split into three bf16 terms: nine
 // multiply-adds per score less.
+//
+// Measured: 64 sequences x 4160 rows of 512 + 64 dims, 16 heads: 73 us, 1.2 TB/s.
+// Bound by tensor (32 %), ALU (38 %) and FMA (15 %) issue together and the three
+// phases' latency: a block walks a tile in about 9k cycles, two blocks per SM
+// overlap to 5k.  Four warps of two key tiles each took 78 us, a second pair of
+// stages does not fit beside a second block.
 #include <algorithm>
 
 #include "kv4_device.cuh"
@@ -78,7 +84,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
   while (span.x < span.y) {
   Kv4Piece piece = walk.next<kTile>(a, line, share, &span);
   const int b = piece.b, row0 = piece.segment * kRows, nrows = min(kRows, R - row0);
-  const Kv4Rows4 see = kv4_rows<kTile>(a, line, &piece, row0, nrows);
+  const Kv4View see = kv4_rows<kTile>(a, line, &piece, row0, nrows);
   const int sink_tiles = piece.sink_tiles, first = piece.first, t0 = piece.step0, t1 = min(piece.tiles, piece.step1);
   auto row_of = [&](int tile) { return (tile < sink_tiles ? tile : first + tile - sink_tiles) * kTile; };
 
@@ -157,7 +163,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
 #pragma unroll
     for (int c = 0; c < 2; ++c) rs[nt][c] = srs[nt * 8 + 2 * j + c];
 
-  // acc: a value tile holds dims MM and 4 + MM of a lane's eight; accm: sums of p m
+  // acc[mm]: value dims mm and 4 + mm of a lane's eight; accm: sums of p m
   float f = 0.f;   // the values' power of two; 0 before any
   float acc[4][NT][4], accm[NT], lsum[NT][2], limit[NT][2], ref[NT][2];
 #pragma unroll
@@ -320,7 +326,14 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
         if (e > 0) {  // largest scale in [2^3, 2^4); sums made before move along
           const float now = __uint_as_float(min(257u - e, 254u) << 23);
           const float move = f == 0.f ? 0.f : now / f;
-          if (f == 0.f || (move >= 8.67e-19f && move <= 1.15e18f)) {
+          float most = 0.f;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int mm = 0; mm < 4; ++mm) most = fmaxf(most, fabsf(acc[mm][nt][c]));
+          if (__all_sync(0xffffffffu, most * move < kKv4Room)) {
             f = now;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -388,7 +401,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
           bw[nt][1] = pack_bf16x2(x[nt][2], x[nt][3]);
           mma_bf16_zero(sums[nt], 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, bw[nt][0], bw[nt][1]);
           // p 8 s: these weights meet n - 8
-          accm[nt] = fmaf(8.f / f, (x[nt][0] + x[nt][1]) + (x[nt][2] + x[nt][3]), accm[nt]);
+          accm[nt] = fmaf(f == 0.f ? 0.f : 8.f / f, (x[nt][0] + x[nt][1]) + (x[nt][2] + x[nt][3]), accm[nt]);
         }
         mma_values_bf16<0, NT>(acc[0], l0, h0, l8, h8, bw, sums);
         mma_values_bf16<1, NT>(acc[1], l0, h0, l8, h8, bw, sums);

@@ -141,10 +141,14 @@ def kv4_write(pos, k, k_codes, k_params, v=None, v_codes=None, v_params=None, ro
     pairs = [(k, k_codes, k_params, "k")] + ([(v, v_codes, v_params, "v")] if v is not None else [])
     for x, c, p, what in pairs:
         _check_cache(c, p, f"kv4_write: {what}")
+        if x.device != c.device:
+            raise ValueError(f"kv4_write: {what} on {x.device}, its cache on {c.device}")
         if x.dim() != 4 or tuple(x.shape[:2]) != tuple(pos.shape) or x.shape[0] != c.shape[0] \
                 or x.shape[2] != c.shape[1] or x.shape[3] != 2 * c.shape[3]:
             raise ValueError(f"kv4_write: {what} {tuple(x.shape)} does not fit positions {tuple(pos.shape)} and codes "
                              f"{tuple(c.shape)}")
+    if v is not None and v_codes.data_ptr() == k_codes.data_ptr() != 0:
+        raise ValueError("kv4_write: k and v need caches of their own")
     rows = pos.long() + row_offset
     for x, c, p, _ in pairs:
         codes, params = quantize_kv4(x, x.shape[3] // p.shape[3])
@@ -182,7 +186,9 @@ def decode_attention_kv4(q, k, v, q_pos, kv_len, *, window=0, scale=None, k_para
                          latent_v_dim=0, sink_rows=0, n_sink=0):
     """Attention of new tokens q [B, Tn, H, W] against a 4-bit cache (k, v codes; v None with
     latent_v_dim = r for an MLA latent, whose value is the first r dims of a row).  Visibility as in
-    omnicoder.ops.decode; a query that sees no row gets zeros.  -> [B, Tn, H, W or r]."""
+    omnicoder.ops.decode; a query that sees no row gets zeros.  Sums are fp32 in units of the largest
+    scale of a head's rows: values up to 2^100, and of rows whose scales differ by more than 2^90 the
+    smaller ones may be lost.  -> [B, Tn, H, W or r]."""
     sc = scale if scale is not None else 1.0 / math.sqrt(q.shape[3])
     if q.is_cuda:                        # checked by the bindings
         return _ext.load().kv4_attend(q, k, k_params, v, v_params, q_pos, kv_len, window, sc, latent_v_dim,

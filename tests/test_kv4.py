@@ -155,6 +155,8 @@ def test_refusals():
         kv4_write(pos, x, c, p[:, :, :16])
     with pytest.raises(ValueError, match="params must be"):
         kv4_write(pos, x, c, None)
+    with pytest.raises(ValueError, match="caches of their own"):
+        kv4_write(pos, x, c, p, x, c, p)
     with pytest.raises(ValueError, match="groups of"):
         kv4_read(pos, *kv4_alloc(2, 4, 32, 128)[:1], torch.zeros(2, 4, 32, 1, 2, dtype=torch.bfloat16))
     with pytest.raises(ValueError, match="dtype"):
@@ -364,6 +366,45 @@ def test_attention_scales_far_apart(H, Hk, W, latent, far):
         out, want = _check_attention(q, kc, kp, vc, vp, q_pos, kv_len, **kw)
         # weights of one size, at most 700: half a step of the output and 2^-8 of eight scales
         assert (out.double() - want).abs().max() <= 2.0 ** -7 * want.abs().max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,Hk,W,latent", [(48, 8, 128, 0), (32, 8, 64, 0), (16, 1, 576, 512), (4, 1, 320, 256)])
+@pytest.mark.parametrize("B,ctx,even", [(61, 1100, False), (64, 1100, True), (260, 400, False), (2, 3000, True)])
+def test_attention_of_many_sequences(H, Hk, W, latent, B, ctx, even):
+    """Batches whose blocks walk several sequences, hold parts of one, or one each."""
+    g = torch.Generator().manual_seed(22)
+    lens = [ctx] * B if even else [0, 1, ctx] + torch.randint(0, ctx + 1, (B - 3,), generator=g).tolist()
+    q, kc, kp, vc, vp, q_pos, kv_len = _attend_case(B, 1, H, Hk, W, latent, ctx, seed=23, lens=lens)
+    _check_attention(q, kc, kp, vc, vp, q_pos, kv_len, latent=latent)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,Hk,W,latent", [(8, 1, 128, 0), (16, 1, 576, 512), (16, 1, 320, 256)])
+@pytest.mark.parametrize("levels", [(40, -5, -50, -95), (-95, -50, -5, 40), (-60, 30, -60, 30), (40, -100, 40, -100), (-100, 40, -100, 40)])
+def test_attention_scales_that_drop_and_rise(H, Hk, W, latent, levels):
+    """Long runs of rows whose values are 2^level, all of one weight: the largest are the result.  260
+    sequences, so that a block walks every run."""
+    q, kc, kp, vc, vp, q_pos, kv_len = _attend_case(260, 1, H, Hk, W, latent, 1024, seed=24, lens=[1024] * 260)
+    g, run = W // kp.shape[3], kc.shape[2] // len(levels)
+    q.zero_()
+    for n, e in enumerate(levels):
+        (vp if vp is not None else kp[:, :, :, :latent // g])[:, :, n * run:(n + 1) * run] *= 2.0 ** e
+    out, want = _check_attention(q, kc, kp, vc, vp, q_pos, kv_len, latent=latent)
+    assert torch.isfinite(out).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,Hk,W,latent", [(8, 1, 128, 0), (16, 1, 576, 512), (16, 1, 320, 256)])
+@pytest.mark.parametrize("s", [0.0, 2.0 ** -130])
+def test_attention_of_constant_groups(H, Hk, W, latent, s):
+    """Scales of zero, or below any that a quantised row has: the minima alone are the result."""
+    q, kc, kp, vc, vp, q_pos, kv_len = _attend_case(2, 2, H, Hk, W, latent, 200, seed=25)
+    kp[..., 0] = s
+    if vp is not None:
+        vp[..., 0] = s
+    out, want = _check_attention(q, kc, kp, vc, vp, q_pos, kv_len, latent=latent)
+    assert torch.isfinite(out).all()
 
 
 @pytest.mark.gpu
