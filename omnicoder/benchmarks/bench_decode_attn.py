@@ -82,7 +82,10 @@ def main(argv=None):
     times.sort()
     ms = times[len(times) // 2]
     rows = (min(a.ctx + Tn, a.window + Tn - 1) if a.window else a.ctx + Tn) + a.mem
-    row_bytes = (2 * a.mha * kv4_row_bytes(DQ) if a.mha else kv4_row_bytes(DQ, DV)) if a.kv == "int4" else (a.mha * (DQ + DV) if a.mha else DQ) * (1 if a.kv == "int8" else 2)
+    if a.kv == "int4":
+        row_bytes = 2 * a.mha * kv4_row_bytes(DQ) if a.mha else kv4_row_bytes(DQ, DV)
+    else:
+        row_bytes = (a.mha * (DQ + DV) if a.mha else DQ) * (1 if a.kv == "int8" else 2)
     row_bytes += (4 * (2 * a.mha if a.mha else 1)) if a.kv == "int8" else 0
     nbytes = B * rows * row_bytes
     print(json.dumps({"kernel": f"decode attention ({'MHA/GQA %d kv heads x %d' % (a.mha, DQ) if a.mha else 'MLA latent'})", "batch": B, "tn": Tn, "heads": H, "ctx": a.ctx,

@@ -32,7 +32,6 @@ struct Kv4IO {
   int B, T, Hk, L, W, group;
   long long row_offset;
   int type;              // Kv4Type of the rows
-  bool wide;             // rows to write from start on 32-byte boundaries (rows read into always do)
 };
 void kv4_write(const Kv4IO& a, cudaStream_t s);
 void kv4_read(const Kv4IO& a, cudaStream_t s);

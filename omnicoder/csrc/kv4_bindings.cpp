@@ -99,8 +99,6 @@ void kv4_write_t(const at::Tensor& pos, const at::Tensor& k, const at::Tensor& k
         reinterpret_cast<uintptr_t>(x.data_ptr()) % 16)
       x = x.clone(at::MemoryFormat::Contiguous);
     keep[i] = x;
-    a.wide = (i == 0 || a.wide) && x.stride(0) % (2 * align) == 0 && x.stride(1) % (2 * align) == 0 &&
-             x.stride(2) % (2 * align) == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 32 == 0;
     a.rows[i] = Kv4Rows{x.data_ptr(), x.stride(0), x.stride(1), x.stride(2)};
   }
   if (a.B == 0 || a.T == 0 || a.Hk == 0) return;

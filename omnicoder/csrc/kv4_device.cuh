@@ -429,6 +429,8 @@ void kv4_launch(void (*kernel)(Params...), dim3 grid, int threads, int smem, cud
   cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// Steps of a segment in a full cache (or window): the host does not know the sequences' lengths.
+long long kv4_plan_steps(const Kv4Attend& a);
 // Grid and workspace: slots blocks stay resident; a block's start costs it about restart steps.
 void kv4_line_plan(const Kv4Attend& a, Kv4Plan& p, int slots, int restart);
 Kv4Line kv4_line(const Kv4Attend& a, const Kv4Plan& p);

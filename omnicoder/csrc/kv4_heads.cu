@@ -9,8 +9,8 @@
 // weights p s (rounded to fp16, the only rounding before the output's) with the
 // codes.  The second sums stay in fp32.
 //
-// A block owns (sequence, key / value head, up to 16 query rows, one split of
-// the keys).  Each of its four warps takes every fourth 32-row tile on its own:
+// A block owns up to 16 query rows of a (sequence, key / value head) and a stretch
+// of its keys, then the next one's (Kv4Line).  Each of its four warps takes every fourth 32-row tile on its own:
 // tiles arrive by cp.async in a ring private to the warp, so that the loop has
 // no block-wide barrier, and the codes go from shared memory to matrix operands
 // in registers.  The 8 query rows (two tiles of 8 for up to 16) are the n side of
@@ -40,7 +40,7 @@ constexpr float kSlack = 8.f;   // log2 units a score may exceed the running max
 template <int D, int NT>
 struct HeadsCfg {
   static constexpr int NG = D / 64;
-  static constexpr int kStages = 3;
+  static constexpr int kStages = 3;   // and three blocks per SM: 149 us, two stages and four blocks 155 us
   static constexpr int kRow = D / 2;
   static constexpr int kCodes = kTile * kRow;
   static constexpr int kParams = kTile * NG * 4;
@@ -473,7 +473,14 @@ void launch_dims(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s) {
 void kv4_heads_plan(const Kv4Attend& a, Kv4Plan& p) {
   const int R = a.Tn * (a.H / a.Hk);
   p.kernel = 1;
-  p.row_tiles = R <= 8 ? 1 : 2;
+  // 8 query rows per block and three blocks per SM, or 16 and two: that reads the codes once for twice the
+  // rows, but a block takes 4.5 us longer to start and to end.  Measured, us 8 / 16 rows (cold): 6 rows of
+  // 64 x 8 heads x 64 steps 155 / 226; 12 rows of 16 x 8 x 32 steps 56 / 48, of 1 x 8 x 64 steps 21.5 / 23.6;
+  // 16 rows of 64 x 4 x 32 steps 93 / 81; heads of 64, 12 rows of 64 x 8 x 32 steps 106 / 93, of 8 x 8 x 8
+  // steps 17.4 / 19.5.  That is 2.2 and 2.0 us per step of a block.
+  const double steps = (double)kv4_plan_steps(a) * a.B * a.Hk;
+  const double one = 2.2 * steps * ((R + 7) / 8) / (148 * 3), two = 2.0 * steps * ((R + 15) / 16) / (148 * 2) + 4.5;
+  p.row_tiles = one <= two ? 1 : 2;
   p.row_blocks = (R + 8 * p.row_tiles - 1) / (8 * p.row_tiles);
   kv4_line_plan(a, p, 148 * (p.row_tiles == 1 ? 3 : 2), 3);
 }

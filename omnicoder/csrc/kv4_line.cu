@@ -108,7 +108,11 @@ Kv4Line kv4_line(const Kv4Attend& a, const Kv4Plan& p) {
                  meta, reinterpret_cast<int*>(meta + segments)};
 }
 
-// The host knows the cache's size, not the sequences' lengths, and plans for a full cache (or window).
+long long kv4_plan_steps(const Kv4Attend& a) {
+  const long long rows = a.n_sink + std::min<long long>(a.L - a.sink_rows, a.window > 0 ? (long long)a.window + a.Tn : 1 << 30);
+  return (rows + kKv4Step - 1) / kKv4Step;
+}
+
 // A block per segment costs its steps times the waves of blocks; shared steps cost their share, and
 // about `restart` steps more to find the places and to join the pieces (3 us).  Measured, one query
 // row a sequence, us shared / a block each: 8 heads of 128, 1 sequence of 2, 4, 8 steps 8.4 / 6.2,
@@ -116,8 +120,7 @@ Kv4Line kv4_line(const Kv4Attend& a, const Kv4Plan& p) {
 // steps 11.8 / 9.7, 12.7 / 13.6, 13.2 / 21.4.  Many sequences or new tokens make the places on the
 // line dear to find: a block each.
 void kv4_line_plan(const Kv4Attend& a, Kv4Plan& p, int slots, int restart) {
-  const long long rows = a.n_sink + std::min<long long>(a.L - a.sink_rows, a.window > 0 ? (long long)a.window + a.Tn : 1 << 30);
-  const long long steps = (rows + kKv4Step - 1) / kKv4Step, segments = (long long)a.B * a.Hk * p.row_blocks;
+  const long long steps = kv4_plan_steps(a), segments = (long long)a.B * a.Hk * p.row_blocks;
   const double waves = (double)segments / slots;
   const double each = steps * (waves < 4 ? std::ceil(waves) : waves), shared = std::max(1.0, std::ceil(steps * waves)) + restart;
   if (each <= shared || a.B > kKv4MaxLine || a.Tn > 16 || segments * (steps + 1) > (1 << 30) ||

@@ -369,18 +369,29 @@ def test_attention_scales_far_apart(H, Hk, W, latent, far):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("H,Hk,W,latent", [(48, 8, 128, 0), (32, 8, 64, 0), (16, 1, 576, 512), (4, 1, 320, 256)])
-@pytest.mark.parametrize("B,ctx,even", [(61, 1100, False), (64, 1100, True), (260, 400, False), (2, 3000, True)])
-def test_attention_of_many_sequences(H, Hk, W, latent, B, ctx, even):
-    """Batches whose blocks walk several sequences, hold parts of one, or one each."""
+@pytest.mark.parametrize("H,Hk,W,latent", [(48, 8, 128, 0), (32, 8, 64, 0), (48, 4, 128, 0), (64, 4, 64, 0), (16, 1, 576, 512),
+                                           (4, 1, 320, 256)])
+@pytest.mark.parametrize("B,ctx,even,kw", [(61, 1100, False, {}), (64, 1100, True, {}), (260, 400, False, {}), (2, 3000, True, {}),
+                                           (64, 1100, False, {"window": 700, "sink_rows": 40, "n_sink": 37})])
+def test_attention_of_many_sequences(H, Hk, W, latent, B, ctx, even, kw):
+    """Batches whose blocks walk several sequences, hold parts of one, or one each; then the same bits
+    over NaN in every row that a sequence does not see."""
     g = torch.Generator().manual_seed(22)
     lens = [ctx] * B if even else [0, 1, ctx] + torch.randint(0, ctx + 1, (B - 3,), generator=g).tolist()
-    q, kc, kp, vc, vp, q_pos, kv_len = _attend_case(B, 1, H, Hk, W, latent, ctx, seed=23, lens=lens)
-    _check_attention(q, kc, kp, vc, vp, q_pos, kv_len, latent=latent)
+    sink = kw.get("sink_rows", 0)
+    q, kc, kp, vc, vp, q_pos, kv_len = _attend_case(B, 1, H, Hk, W, latent, ctx, seed=23, lens=lens, sink=sink)
+    want, _ = _check_attention(q, kc, kp, vc, vp, q_pos, kv_len, latent=latent, **kw)
+    row = torch.arange(kc.shape[2], device="cuda")[None]
+    unseen = (row >= kw.get("n_sink", 0)) & ((row < sink) | (row - sink >= kv_len[:, None]))
+    for p in (kp, vp):
+        if p is not None:
+            p.masked_fill_(unseen[:, None, :, None, None], float("nan"))
+    got = decode_attention(q, kc, vc, q_pos, kv_len, k_scale=kp, v_scale=vp, latent_v_dim=latent, **kw)
+    assert torch.equal(got, want)
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("H,Hk,W,latent", [(8, 1, 128, 0), (16, 1, 576, 512), (16, 1, 320, 256)])
+@pytest.mark.parametrize("H,Hk,W,latent", [(8, 1, 128, 0), (16, 1, 128, 0), (16, 1, 576, 512), (16, 1, 320, 256)])
 @pytest.mark.parametrize("levels", [(40, -5, -50, -95), (-95, -50, -5, 40), (-60, 30, -60, 30), (40, -100, 40, -100), (-100, 40, -100, 40)])
 def test_attention_scales_that_drop_and_rise(H, Hk, W, latent, levels):
     """Long runs of rows whose values are 2^level, all of one weight: the largest are the result.  260
