@@ -37,21 +37,22 @@ __device__ __forceinline__ void store32(void* p, const uint32_t* w) {
                : "memory");
 }
 
+// Words of sixteen values, and the values.
 template <int TYPE>
-__device__ __forceinline__ void load_piece(const void* base, long long i, float* x, uint32_t* bits) {
-  constexpr int kWords = TYPE == KV4_F32 ? 16 : 8;
+__device__ __forceinline__ void load_words(const void* base, long long i, uint32_t* w) {
   const uint8_t* p = reinterpret_cast<const uint8_t*>(base) + i * (TYPE == KV4_F32 ? 4 : 2);
-  uint32_t w[kWords];
 #pragma unroll
-  for (int k = 0; k < kWords / 8; ++k) load32(p + 32 * k, w + 8 * k);
+  for (int k = 0; k < (TYPE == KV4_F32 ? 2 : 1); ++k) load32(p + 32 * k, w + 8 * k);
+}
+template <int TYPE>
+__device__ __forceinline__ void words_to_floats(const uint32_t* w, float* x) {
 #pragma unroll
-  for (int k = 0; k < kWords; ++k) {
+  for (int k = 0; k < (TYPE == KV4_F32 ? 16 : 8); ++k) {
     if (TYPE == KV4_F32) {
       x[k] = __uint_as_float(w[k]);
     } else if (TYPE == KV4_BF16) {
       x[2 * k] = bf16_lo(w[k]);
       x[2 * k + 1] = bf16_hi(w[k]);
-      bits[k] = w[k];
     } else {
       const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
       x[2 * k] = f.x;
@@ -81,13 +82,14 @@ __device__ __forceinline__ void store1(void* base, long long i, float x) {
 }
 
 // ---------------------------------------------------------------------------
-// Append and read back.  A thread owns sixteen dims of kPasses rows; the threads of
-// a group of g dims are neighbours in a warp, and a block's rows run over the
-// tokens of one head and then the next, so that a warp writes whole sectors of
-// the codes.  Measured: 8 x 8192 rows of 576 bf16 values written in 29 us and read
-// back in 20 us (3.5 TB/s together); the write is bound by its instructions (issue
-// 78 %: 350 per 16 values), the read by them and by memory.  Single tokens of 64
-// sequences: 3 us each, the launch.
+// Append and read back.  A thread owns sixteen dims (writing groups of 32 and 64:
+// 32 dims) of up to kPasses rows; the threads of a group of g dims are neighbours in
+// a warp, and a block's rows run over the tokens of one head and then the next, so
+// that a warp writes whole sectors of the codes.  Measured: 8 x 8192 rows of 576
+// bf16 values written in 24 us (4.1 TB/s) and read back in 18.5 us (5.2 TB/s); the
+// write is bound by its instructions, the read by memory.  Single tokens of 64
+// sequences: 2.5 and 1.5 us.  Writing 16 dims per thread took 29 us: 312 instead of
+// 215 instructions per 16 values, for addresses, minimum and maximum.
 // ---------------------------------------------------------------------------
 constexpr int kIoThreads = 256;
 constexpr int kPasses = 4;
@@ -123,96 +125,140 @@ __device__ __forceinline__ uint32_t* io_params(const Kv4Cache& c, const IoGrid& 
 // Round (x - m) / s, .. < 15.5, decided as if the quotient were exact: d + e = x - m exactly,
 // r = d - n s exactly for n next to it (n s has at most 12 significant bits), and r + e is compared
 // with half a step; ties to even.
-__device__ __forceinline__ uint32_t kv4_codes8_exact(const float* x, float m, float s, float inv) {
-  uint32_t code = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float d = x[i] - m, back = d - x[i], half = 0.5f * s;
-    const float e = (x[i] - (d - back)) - (m + back);
-    float n = rintf(d * inv);
-    const float r = fmaf(-n, s, d);
-    const bool odd = ((int)n & 1) != 0;
-    if (r > half || (r == half && (e > 0.f || (e == 0.f && odd)))) n += 1.f;
-    else if (r < -half || (r == -half && (e < 0.f || (e == 0.f && odd)))) n -= 1.f;
-    code |= (uint32_t)fminf(fmaxf(n, 0.f), 15.f) << (4 * i);
-  }
-  return code;
+__device__ __forceinline__ uint32_t kv4_code_exact(float x, float m, float s, float inv) {
+  const float d = x - m, back = d - x, half = 0.5f * s;
+  const float e = (x - (d - back)) - (m + back);
+  float n = rintf(d * inv);
+  const float r = fmaf(-n, s, d);
+  const bool odd = ((int)n & 1) != 0;
+  if (r > half || (r == half && (e > 0.f || (e == 0.f && odd)))) n += 1.f;
+  else if (r < -half || (r == -half && (e < 0.f || (e == 0.f && odd)))) n -= 1.f;
+  return (uint32_t)fminf(fmaxf(n, 0.f), 15.f);
 }
 
-// Eight codes from q', the quotient (x - m) / s with one residual correction (Markstein, 1990):
+// Two fp32 numbers in one instruction.
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+  uint64_t x;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a), "f"(b));
+  return x;
+}
+__device__ __forceinline__ float2 split2(uint64_t x) {
+  float2 v;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(x));
+  return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t x;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(x) : "l"(a), "l"(b));
+  return x;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t x;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(x) : "l"(a), "l"(b));
+  return x;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t x;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(x) : "l"(a), "l"(b), "l"(c));
+  return x;
+}
+
+// Sixteen codes from q', the quotient (x - m) / s with one residual correction (Markstein, 1990):
 // within 2^-20 of it, and exactly k + 1/2 where the quotient is that and x - m is exact.  Adding
 // 2^23 rounds it, ties to even.  That decides as an exact quotient would
-//   - for bf16 rows whose values are 0 or at least 2^-16 of the range R: x, m and s are then
+//   - for a bf16 value that is 0 or at least 2^-16 of the range R, where m is too: x, m and s are then
 //     multiples of 2^-24 R, x - m is exact, and a quotient that is not halfway between two codes is
 //     2^-24 R / s > 2^-21 or more away, half a unit of the quotient's last place;
-//   - for any row where no quotient lies within 10^-4 of halfway (kv4_near_border).
-// Codes join by multiply-adds on the sums' bits.
+//   - for any value whose quotient is not within 2^-16 of halfway (kv4_near_border, whose quotient
+//     lacks the correction: within 2^-18).
+// Other values are rounded again (kv4_code_exact).
+// The two words of codes go side by side, dims i and i + 8; four codes join as a number below 2^16.
 template <int TYPE>
-__device__ __forceinline__ uint32_t kv4_codes8(const float* x, float m, float s, float inv) {
-  uint32_t acc = 0;
+__device__ __forceinline__ uint64_t kv4_codes16(const float* x, float m, float s, float inv) {
+  const uint64_t m2 = pair2(-m, -m), s2 = pair2(-s, -s), inv2 = pair2(inv, inv), sixteen = pair2(16.f, 16.f);
+  const uint64_t up = pair2(8388608.f, 8388608.f), down = pair2(-8388608.f, -8388608.f);
+  uint64_t half[2];
 #pragma unroll
-  for (int i = 7; i >= 0; --i) {
-    const float d = x[i] - m, q = d * inv;
-    float q1 = fmaf(fmaf(-q, s, d), inv, q);
-    if (TYPE != KV4_BF16) q1 = fminf(fmaxf(q1, 0.f), 15.f);  // the minimum was rounded to bf16
-    acc = acc * 16u + __float_as_uint(q1 + 8388608.f);
+  for (int h = 0; h < 2; ++h) {
+    uint64_t acc = 0;
+#pragma unroll
+    for (int i = 4 * h + 3; i >= 4 * h; --i) {
+      const uint64_t d = add2(pair2(x[i], x[i + 8]), m2), q = mul2(d, inv2);
+      uint64_t q1 = fma2(fma2(q, s2, d), inv2, q);
+      if (TYPE != KV4_BF16) {  // the minimum was rounded to bf16
+        const float2 v = split2(q1);
+        q1 = pair2(fminf(fmaxf(v.x, 0.f), 15.f), fminf(fmaxf(v.y, 0.f), 15.f));
+      }
+      const uint64_t n = add2(add2(q1, up), down);
+      acc = i == 4 * h + 3 ? n : fma2(acc, sixteen, n);
+    }
+    half[h] = add2(acc, up);
   }
-  return acc - 0xfb000000u;  // the sum of 0x4b000000 * 16^i, the bits of 2^23, modulo 2^32
+  const float2 lo = split2(half[0]), hi = split2(half[1]);
+  const uint32_t w0 = __byte_perm(__float_as_uint(lo.x), __float_as_uint(hi.x), 0x5410);
+  const uint32_t w1 = __byte_perm(__float_as_uint(lo.y), __float_as_uint(hi.y), 0x5410);
+  return (uint64_t)w0 | ((uint64_t)w1 << 32);
 }
 
-__device__ __forceinline__ bool kv4_near_border(const float* x, float m, float inv) {
-  float far = 0.f;
-#pragma unroll
-  for (int i = 0; i < kPiece; ++i) {
-    const float t = fminf(fmaxf((x[i] - m) * inv, 0.f), 15.f);
-    far = fmaxf(far, fabsf(t - ((t + 8388608.f) - 8388608.f)));
-  }
-  return far > 0.4999f;
+// Is the quotient within 2^-16 of halfway between two codes?
+__device__ __forceinline__ bool kv4_near_border(float x, float m, float inv) {
+  const float t = fminf(fmaxf((x - m) * inv, 0.f), 15.f);
+  return fabsf(t - ((t + 8388608.f) - 8388608.f)) > 0.4999847412109375f;
 }
 
-template <int TYPE>
+template <int TYPE, int PIECES>
 __global__ void __launch_bounds__(kIoThreads) kv4_write_kernel(const Kv4IO a, const IoGrid g) {
   wait_for_previous_grid();
   launch_dependents();
+  constexpr int kWords = TYPE == KV4_F32 ? 16 : 8;   // of a piece
   const int b = blockIdx.y, r_in = g.pieces.of(threadIdx.x), piece = threadIdx.x - r_in * g.pieces.d;
   const Kv4Cache& c = a.cache[blockIdx.z];
   const Kv4Rows& src = a.rows[blockIdx.z];
-  const int lanes = 1 << g.lanes_shift;  // 1, 2 or 4 neighbouring threads hold a group
+  const int lanes = 1 << g.lanes_shift;  // 1 or 2 neighbouring threads hold a group
   const int first = blockIdx.x * (g.rows_per_pass * g.passes) + r_in;
   const bool idle = r_in >= g.rows_per_pass;
 #pragma unroll 1
   for (int k = 0; k < g.passes; ++k) {
     const int r = first + k * g.rows_per_pass;
-    float x[kPiece];
-    uint32_t bits[8];
+    uint32_t w[PIECES * kWords];
     const IoRow row = io_row(a, g, min(r, g.total - 1));   // threads behind the last row repeat it and write nothing
-    load_piece<TYPE>(src.x, b * src.x_b + row.t * src.x_t + row.h * src.x_h + piece * kPiece, x, bits);
-    float lo, hi, probe;  // probe: NaN behind a NaN or an infinity
-    if (TYPE == KV4_BF16) {
-      const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(bits);
-      const __nv_bfloat162 zero = __floats2bfloat162_rn(0.f, 0.f);
-      __nv_bfloat162 l = v[0], h = v[0], p = __hmul2(v[0], zero);
+    const long long at = b * src.x_b + row.t * src.x_t + row.h * src.x_h + piece * (PIECES * kPiece);
 #pragma unroll
-      for (int i = 1; i < 8; ++i) {
+    for (int n = 0; n < PIECES; ++n) load_words<TYPE>(src.x, at + n * kPiece, w + n * kWords);
+    float lo, hi, probe, least = 0.f;  // probe: NaN behind a NaN or an infinity; least |x|
+    if (TYPE == KV4_BF16) {
+      const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(w);
+      const __nv_bfloat162 zero = __floats2bfloat162_rn(0.f, 0.f);
+      __nv_bfloat162 l = v[0], h = v[0], p = __hmul2(v[0], zero), q = __habs2(v[0]);
+#pragma unroll
+      for (int i = 1; i < PIECES * kWords; ++i) {
         l = __hmin2(l, v[i]);
         h = __hmax2(h, v[i]);
         p = __hfma2(v[i], zero, p);
+        q = __hmin2(q, __habs2(v[i]));
       }
       lo = fminf(__low2float(l), __high2float(l));
       hi = fmaxf(__low2float(h), __high2float(h));
       probe = __low2float(p) + __high2float(p);
+      least = fminf(__low2float(q), __high2float(q));
     } else {
-      lo = hi = x[0];
+      lo = INFINITY;
+      hi = -INFINITY;
       probe = 0.f;
 #pragma unroll
-      for (int i = 0; i < kPiece; ++i) {
-        lo = fminf(lo, x[i]);
-        hi = fmaxf(hi, x[i]);
-        probe = fmaf(x[i], 0.f, probe);
+      for (int n = 0; n < PIECES; ++n) {
+        float x[kPiece];
+        words_to_floats<TYPE>(w + n * kWords, x);
+#pragma unroll
+        for (int i = 0; i < kPiece; ++i) {
+          lo = fminf(lo, x[i]);
+          hi = fmaxf(hi, x[i]);
+          probe = fmaf(x[i], 0.f, probe);
+        }
       }
     }
 #pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
+    for (int o = 1; o < PIECES; o <<= 1) {  // groups of 16 are a thread's own
       const float l2 = __shfl_xor_sync(0xffffffffu, lo, o), h2 = __shfl_xor_sync(0xffffffffu, hi, o);
       const float p2 = __shfl_xor_sync(0xffffffffu, probe, o);
       if (o < lanes) {
@@ -232,27 +278,43 @@ __global__ void __launch_bounds__(kIoThreads) kv4_write_kernel(const Kv4IO a, co
       s = 0.f;
       sb = __float2bfloat16_rn(0.f);
     }
-    uint64_t code = 0;
+    uint64_t code[PIECES];
+#pragma unroll
+    for (int n = 0; n < PIECES; ++n) code[n] = 0;
     if (!bad && s > 0.f) {
       float inv;  // within 2^-23: candidates and residual corrections need no more
       asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
-      bool check = TYPE != KV4_BF16 || s < 1e-27f;
-      if (TYPE == KV4_BF16) {
-        // the smallest |x| - 1 as bits; 0 becomes the largest
-        uint32_t least = 0xffffffffu;
+      // the values to look at: all, or bf16 ones below 2^-16 of the range
+      const float small = range * 1.52587890625e-5f;
+      const float limit = TYPE != KV4_BF16 || s < 1e-27f || (m != 0.f && fabsf(m) < small) ? INFINITY : small;
+      uint32_t again = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) least = __viaddmin_u16x2(bits[i] & 0x7fff7fffu, 0xffffffffu, least);
-        const float smallest = __uint_as_float((min(least & 0xffffu, least >> 16) + 1u) << 16);
-        const float limit = range * 1.52587890625e-5f;
-        check = check || smallest < limit || (m != 0.f && fabsf(m) < limit);
+      for (int n = 0; n < PIECES; ++n) {
+        float x[kPiece];
+        words_to_floats<TYPE>(w + n * kWords, x);
+        if (TYPE != KV4_BF16 || least < limit) {
+#pragma unroll
+          for (int i = 0; i < kPiece; ++i)
+            if (fabsf(x[i]) < limit && kv4_near_border(x[i], m, inv)) again |= 1u << (n * kPiece + i);
+        }
+        code[n] = kv4_codes16<TYPE>(x, m, s, inv);
       }
-      if (check && (s < 1e-27f || kv4_near_border(x, m, inv)))
-        code = (uint64_t)kv4_codes8_exact(x, m, s, inv) | ((uint64_t)kv4_codes8_exact(x + 8, m, s, inv) << 32);
-      else
-        code = (uint64_t)kv4_codes8<TYPE>(x, m, s, inv) | ((uint64_t)kv4_codes8<TYPE>(x + 8, m, s, inv) << 32);
+      if (s < 1e-27f) again = 0xffffffffu >> (32 - PIECES * kPiece);
+      while (again != 0) {  // few values of few threads: read again
+        const int i = __ffs(again) - 1, shift = 4 * (i & 15);
+        again &= again - 1;
+        const uint64_t exact = (uint64_t)kv4_code_exact(kv4_load1<TYPE>(src.x, at + i), m, s, inv) << shift;
+        const uint64_t keep = ~(15ull << shift);
+        if (PIECES == 1 || i < kPiece) code[0] = (code[0] & keep) | exact;
+        else code[PIECES - 1] = (code[PIECES - 1] & keep) | exact;
+      }
     }
     if (row.row < 0 || idle || r >= g.total) continue;
-    *reinterpret_cast<uint64_t*>(io_codes(a, c, row, piece)) = code;
+    uint8_t* to = io_codes(a, c, row, piece * PIECES);
+    if (PIECES == 2)
+      *reinterpret_cast<ulonglong2*>(to) = make_ulonglong2(code[0], code[PIECES - 1]);
+    else
+      *reinterpret_cast<uint64_t*>(to) = code[0];
     if ((piece & (lanes - 1)) == 0) {
       const uint32_t word = (uint32_t)__bfloat16_as_ushort(sb) | ((uint32_t)__bfloat16_as_ushort(mb) << 16);
       *io_params(c, g, row, piece) = bad ? 0x7fc07fc0u : word;
@@ -327,15 +389,15 @@ __global__ void __launch_bounds__(kIoThreads) kv4_read_kernel(const Kv4IO a, con
 }
 
 // Enough blocks first, then several rows per thread.  Measured, 1, 2 and up to 4 rows, us written /
-// read back (cold): 8 x 8192 rows of 576 in bf16 41 / 29, 37 / 27, 37 / 25; 3 x 4001 x 8 heads of 128
-// 19 / 14, 19 / 14, 19 / 12; a token of 64 sequences the same.
-dim3 io_grid(const Kv4IO& a, IoGrid* g) {
-  g->pieces = Kv4Div(a.W / kPiece);
+// read back: 8 x 8192 rows of 576 in bf16 27.6 / 23.4, 25.8 / 19.8, 26.0 / 18.5, in fp32 74 / 35, 61 / 31,
+// 54 / 31; 3 x 4001 x 8 heads of 128 and a token of 64 sequences within 4 %.
+dim3 io_grid(const Kv4IO& a, int dims, IoGrid* g) {
+  g->pieces = Kv4Div(a.W / dims);
   g->tokens = Kv4Div(a.T);
   g->rows_per_pass = kIoThreads / g->pieces.d;
   g->total = a.T * a.Hk;
   g->groups = a.W / a.group;
-  g->lanes_shift = a.group == 64 ? 2 : a.group == 32 ? 1 : 0;
+  g->lanes_shift = a.group == 4 * dims ? 2 : a.group == 2 * dims ? 1 : 0;
   const long long blocks1 = (g->total + g->rows_per_pass - 1) / g->rows_per_pass;
   g->passes = (int)std::min<long long>(kPasses, std::max<long long>(1, blocks1 * a.B * a.count / (148 * 4)));
   const long long per_block = (long long)g->rows_per_pass * g->passes;
@@ -455,15 +517,17 @@ void launch_rows(const Kv4Attend& a, cudaStream_t s) {
 
 void kv4_write(const Kv4IO& a, cudaStream_t s) {
   IoGrid g{Kv4Div(1), Kv4Div(1), 0, 0, 0, 0, 0};
-  const dim3 grid = io_grid(a, &g);
-  if (a.type == KV4_F32) kv4_launch(kv4_write_kernel<KV4_F32>, grid, kIoThreads, 0, s, a, g);
-  else if (a.type == KV4_F16) kv4_launch(kv4_write_kernel<KV4_F16>, grid, kIoThreads, 0, s, a, g);
-  else kv4_launch(kv4_write_kernel<KV4_BF16>, grid, kIoThreads, 0, s, a, g);
+  const bool two = a.group >= 32;
+  const dim3 grid = io_grid(a, two ? 32 : 16, &g);
+  auto go = [&](auto one_piece, auto two_pieces) { kv4_launch(two ? two_pieces : one_piece, grid, kIoThreads, 0, s, a, g); };
+  if (a.type == KV4_F32) go(kv4_write_kernel<KV4_F32, 1>, kv4_write_kernel<KV4_F32, 2>);
+  else if (a.type == KV4_F16) go(kv4_write_kernel<KV4_F16, 1>, kv4_write_kernel<KV4_F16, 2>);
+  else go(kv4_write_kernel<KV4_BF16, 1>, kv4_write_kernel<KV4_BF16, 2>);
 }
 
 void kv4_read(const Kv4IO& a, cudaStream_t s) {
   IoGrid g{Kv4Div(1), Kv4Div(1), 0, 0, 0, 0, 0};
-  const dim3 grid = io_grid(a, &g);
+  const dim3 grid = io_grid(a, kPiece, &g);
   if (a.type == KV4_F32) kv4_launch(kv4_read_kernel<KV4_F32>, grid, kIoThreads, 0, s, a, g);
   else if (a.type == KV4_F16) kv4_launch(kv4_read_kernel<KV4_F16>, grid, kIoThreads, 0, s, a, g);
   else kv4_launch(kv4_read_kernel<KV4_BF16>, grid, kIoThreads, 0, s, a, g);
