@@ -102,28 +102,40 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
     for (int k = 0; k < kStages; ++k)
       if (t0 + k < t1) issue(t0 + k, (used + k) % kStages);
 
-  // ---- queries: normalised fp16, laid out as the operands of the scores; a lane takes
-  // the eight dims of a code word -------------------------------------------------------------------
-  for (int r = warp; r < kRows; r += kWarps) {
-    constexpr int kWords = W / 8, kPer = (kWords + 31) / 32;
-    float x[kPer][8] = {}, amax = 0.f, un;
+  // ---- queries: normalised fp16, laid out as the operands of the scores; a warp holds two rows,
+  // a lane takes the eight dims of a code word ------------------------------------------------------
+  {
+    constexpr int kWords = W / 8, kPer = (2 * kWords + 31) / 32;
+    static_assert(kRows == 2 * kWarps && kWords % 8 == 0, "two rows a warp, groups within eight lanes");
+    const int r0 = 2 * warp;
+    float x[kPer][8] = {}, amax[2] = {}, sc[2], un[2];
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-      const int w = lane + 32 * e;
-      if (r < nrows && w < kWords) kv4_load8<TYPE>(a.q, ((long long)b * R + row0 + r) * W + w * 8, x[e]);
+      const int at = lane + 32 * e, second = at >= kWords, r = r0 + second, w = at - second * kWords;
+      if (w < kWords && r < nrows) kv4_load8<TYPE>(a.q, ((long long)b * R + row0 + r) * W + w * 8, x[e]);
     }
 #pragma unroll
-    for (int e = 0; e < kPer; ++e)
+    for (int e = 0; e < kPer; ++e) {
+      const bool second = lane + 32 * e >= kWords;
+      float top = 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(x[e][k]));
-    const float sc = q_normaliser(warp_max(amax), &un);
+      for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(x[e][k]));
+      if (second) amax[1] = fmaxf(amax[1], top);
+      else amax[0] = fmaxf(amax[0], top);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      sc[h] = q_normaliser(warp_max(amax[h]), &un[h]);
+      if (lane == h) srs[r0 + h] = un[h] * (a.scale * (kKv4Log2e * kKv4Codes));
+    }
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-      const int w = lane + 32 * e, g = w >> 3;
+      const int at = lane + 32 * e, second = at >= kWords, r = r0 + second, w = at - second * kWords, g = w >> 3;
       float sum = 0.f;
       if (w < kWords) {
+        const float by = second ? sc[1] : sc[0];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[e][k] *= sc;
+        for (int k = 0; k < 8; ++k) x[e][k] *= by;
         uint2 q[2];
         sum = query_pairs(x[e], q);
 #pragma unroll
@@ -132,10 +144,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
       }
 #pragma unroll
       for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if ((lane & 7) == 0 && g < 16) sqs[r * 16 + g] = w < kWords ? sum * (1.f / kKv4Codes) : 0.f;
+      if ((lane & 7) == 0 && w < kWords) sqs[r * 16 + g] = sum * (1.f / kKv4Codes);
     }
-    if (lane >= kPer * 4 && lane < 16) sqs[r * 16 + lane] = 0.f;
-    if (lane == 0) srs[r] = un * (a.scale * (kKv4Log2e * kKv4Codes));
+    if ((lane & 15) >= NG) sqs[(r0 + (lane >> 4)) * 16 + (lane & 15)] = 0.f;
   }
   if (warp == 0 && lane < kRows) {
     slo[lane] = see.seen.lo;
