@@ -124,21 +124,24 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
   }
 
   // ---- queries: normalised fp16 rows, group sums, score factors; a lane takes the eight
-  // dims of a code word ---------------------------------------------------------------------------
-  for (int r = warp; r < C::kRows; r += kWarps) {
-    constexpr int kWords = D / 8;
-    float x[8] = {}, amax = 0.f, sum = 0.f, un;
-    if (r < nrows && lane < kWords) kv4_load8<TYPE>(a.q, head_of(r) * D + lane * 8, x);
+  // dims of a code word, a warp two or four rows ----------------------------------------------------
+  constexpr int kWords = D / 8, kAtOnce = 32 / kWords;
+  for (int r = warp * kAtOnce + lane / kWords; r < C::kRows; r += kWarps * kAtOnce) {
+    const int w = lane % kWords;
+    float x[8] = {}, amax = 0.f, un;
+    if (r < nrows) kv4_load8<TYPE>(a.q, head_of(r) * D + w * 8, x);
 #pragma unroll
     for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
-    const float sc = q_normaliser(warp_max(amax), &un);
+#pragma unroll
+    for (int o = 1; o < kWords; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    const float sc = q_normaliser(amax, &un);
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] *= sc;
-    if (lane < kWords) sum = query_pairs(x, sq + (r * kWords + lane) * 2);
+    float sum = query_pairs(x, sq + (r * kWords + w) * 2);
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane < kWords && (lane & 7) == 0) sqs[r * NG + (lane >> 3)] = sum * (1.f / kKv4Codes);
-    if (lane == 0) srs[r] = un * (a.scale * (kKv4Log2e * kKv4Codes));
+    if ((w & 7) == 0) sqs[r * NG + (w >> 3)] = sum * (1.f / kKv4Codes);
+    if (w == 0) srs[r] = un * (a.scale * (kKv4Log2e * kKv4Codes));
   }
   __syncthreads();
   // operand of the scores: lane (i, j) holds query row i against the 16 dims that it reads of each group
