@@ -218,7 +218,7 @@ __device__ __forceinline__ void kv4_load8(const void* base, long long i, float* 
 // the blocks that stay resident share them in one of two ways, chosen on the
 // device from the lengths:
 //   - every segment in equal parts, a block each;
-//   - the steps of all segments in one line, cut into equal consecutive pieces,
+//   - the steps of all segments in one line, cut into consecutive pieces equal to one step,
 //     so that uneven lengths and segment counts that do not fill the GPU cost
 //     nothing, but a block that goes on to a second segment starts anew.
 // A block then holds at most two pieces that it shares with others, the first (of
@@ -282,8 +282,8 @@ __device__ __forceinline__ void kv4_tiles(const Kv4Attend& a, Kv4Seen u, Kv4Piec
 struct Kv4Walk {
   int end[kKv4MaxLine], first[kKv4MaxLine], tiles[kKv4MaxLine], sums[32], most[32];
 
-  // -> first and last step of the block on the line.  share: steps of a block, or minus the parts
-  // that every segment is cut into
+  // -> first and last step of the block on the line.  share: steps of a block (or one more), or minus
+  // the parts that every segment is cut into
   template <int kThreads, int kTile>
   __device__ __forceinline__ int2 begin(const Kv4Attend& a, const Kv4Line& l, int* share) {
     if (l.restart == 0) return make_int2(0, 1);
@@ -322,14 +322,14 @@ struct Kv4Walk {
     }
     const int total = before * l.segments.d;
     if (threadIdx.x == 0) l.begun[blockIdx.x] = -1;
-    const int blocks = gridDim.x, even = (total + blocks - 1) / blocks, parts = blocks / (a.B * l.segments.d);
-    if (parts > 0 && (longest + parts - 1) / parts <= even + l.restart) {
+    const int blocks = gridDim.x, at = blockIdx.x, each = total / blocks, parts = blocks / (a.B * l.segments.d);
+    if (parts > 0 && (longest + parts - 1) / parts <= each + l.restart) {
       *share = -parts;
-      return make_int2(0, (int)blockIdx.x < a.B * l.segments.d * parts);
+      return make_int2(0, at < a.B * l.segments.d * parts);
     }
-    *share = even;
-    const int at = blockIdx.x * even;
-    return make_int2(at, min(total, at + even));
+    *share = each;
+    const int more = total - each * blocks;   // blocks of one step more come first
+    return make_int2(at * each + min(at, more), (at + 1) * each + min(at + 1, more));
   }
 
   // The segment that holds step span.x; moves span.x behind it.  A block per segment: tiles and
@@ -370,8 +370,12 @@ struct Kv4Walk {
       const int at = start * l.segments.d + p.segment * p.steps;   // the segment's first step on the line
       p.step0 = span->x - at;
       p.step1 = min(p.steps, span->y - at);
-      last = (at + p.steps - 1) / share;
       span->x = at + p.steps;
+      if (p.step0 == 0 && p.step1 < p.steps && threadIdx.x == 0) {   // the block of the segment's last step
+        const int step = at + p.steps - 1, more = end[a.B - 1] * l.segments.d - share * (int)gridDim.x;
+        const int cut = more * (share + 1);
+        last = step < cut ? step / (share + 1) : more + (step - cut) / share;
+      }
     }
     p.first = first[p.b];
     p.tiles = tiles[p.b];

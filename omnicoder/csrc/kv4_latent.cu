@@ -53,8 +53,8 @@ struct LatentCfg {
   static constexpr int kSmem = kMisc + kRows * (16 + 1 + kWarps + 1) * 4 + kRows * 2 * 4 + kStages * 8;
 };
 
-template <int V, int TYPE>
-__global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Attend a, const Kv4Line line, StatusBlock* st) {
+template <int V, int TYPE, int PER_SM>
+__global__ void __launch_bounds__(kWarps * 32, PER_SM) kv4_latent_kernel(const Kv4Attend a, const Kv4Line line, StatusBlock* st) {
   using C = LatentCfg<V>;
   constexpr int W = C::W, NG = C::NG, KS = C::KS;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -84,6 +84,14 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
   while (span.x < span.y) {
   Kv4Piece piece = walk.next<kTile>(a, line, share, &span);
   const int b = piece.b, row0 = piece.segment * kRows, nrows = min(kRows, R - row0);
+  // query rows, two per warp, a lane eight dims (a code word); asked for before anything waits
+  constexpr int kWords = W / 8, kPer = (2 * kWords + 31) / 32;
+  float x[kPer][8] = {};
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    const int at = lane + 32 * e, second = at >= kWords, r = 2 * warp + second, w = at - second * kWords;
+    if (w < kWords && r < nrows) kv4_load8<TYPE>(a.q, ((long long)b * R + row0 + r) * W + w * 8, x[e]);
+  }
   const Kv4View see = kv4_rows<kTile>(a, line, &piece, row0, nrows);
   const int sink_tiles = piece.sink_tiles, first = piece.first, t0 = piece.step0, t1 = min(piece.tiles, piece.step1);
   auto row_of = [&](int tile) { return (tile < sink_tiles ? tile : first + tile - sink_tiles) * kTile; };
@@ -102,18 +110,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
     for (int k = 0; k < kStages; ++k)
       if (t0 + k < t1) issue(t0 + k, (used + k) % kStages);
 
-  // ---- queries: normalised fp16, laid out as the operands of the scores; a warp holds two rows,
-  // a lane takes the eight dims of a code word ------------------------------------------------------
+  // ---- queries: normalised fp16, laid out as the operands of the scores ---------------------------
   {
-    constexpr int kWords = W / 8, kPer = (2 * kWords + 31) / 32;
     static_assert(kRows == 2 * kWarps && kWords % 8 == 0, "two rows a warp, groups within eight lanes");
     const int r0 = 2 * warp;
-    float x[kPer][8] = {}, amax[2] = {}, sc[2], un[2];
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      const int at = lane + 32 * e, second = at >= kWords, r = r0 + second, w = at - second * kWords;
-      if (w < kWords && r < nrows) kv4_load8<TYPE>(a.q, ((long long)b * R + row0 + r) * W + w * 8, x[e]);
-    }
+    float amax[2] = {}, sc[2], un[2];
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
       const bool second = lane + 32 * e >= kWords;
@@ -219,7 +220,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
 #pragma unroll
       for (int k = 0; k < 3; ++k) mma_bf16(s[nt], m[0], m[1], m[2], m[3], qm[k][nt][0], qm[k][nt][1]);
     }
-#pragma unroll 3
+#pragma unroll(PER_SM == 1 ? NG : 3)
     for (int g = 0; g < NG; ++g) {
       const uint2 wa = lds64(k_at + g * 32), wb = lds64(k_at + 8 * C::kRow + g * 32);
       const float sa = bf16_lo(lds32(p_at + g * 4)), sb = bf16_lo(lds32(p_at + (8 * NG + g) * 4));
@@ -361,7 +362,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
       }
     }
     // ---- output: this warp's value dims over its keys of the tile ---------------------
-#pragma unroll 1
+#pragma unroll(PER_SM == 1 ? 4 : 1)
     for (int kt = kt0; kt < kt0 + kTile / 16 / KS; ++kt) {
       const uint32_t c0 = codes + (kt * 16 + key_0) * C::kRow + i * 4 + vg * 32;
       const uint32_t c1 = codes + (kt * 16 + key_1) * C::kRow + i * 4 + vg * 32;
@@ -501,13 +502,21 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_latent_kernel(const Kv4Att
   (void)ok;
 }
 
-template <int V, int TYPE>
-void launch(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s) {
-  auto kern = kv4_latent_kernel<V, TYPE>;
+template <int V, int TYPE, int PER_SM>
+void launch_per_sm(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s) {
+  auto kern = kv4_latent_kernel<V, TYPE, PER_SM>;
   constexpr int smem = LatentCfg<V>::kSmem;
   ensure_smem_attr(reinterpret_cast<const void*>(kern), smem);
   kv4_launch(kern, dim3((unsigned)p.blocks), kWarps * 32, smem, s, a, kv4_line(a, p),
              reinterpret_cast<StatusBlock*>(status_ptr()));
+}
+
+// No more blocks than SMs: twice the registers, loops unrolled.  Measured, us one / two blocks per SM:
+// 1 sequence of 128, 256, 8192 rows of 576 8.1 / 9.1, 11.8 / 13.2, 13.1 / 13.9; 16 of 1024 14.9 / 14.4,
+// rows of 320 12.0 / 14.4.
+template <int V, int TYPE>
+void launch(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s) {
+  p.blocks <= 148 ? launch_per_sm<V, TYPE, 1>(a, p, s) : launch_per_sm<V, TYPE, 2>(a, p, s);
 }
 
 }  // namespace
@@ -516,7 +525,10 @@ void kv4_latent_plan(const Kv4Attend& a, Kv4Plan& p) {
   p.kernel = 2;
   p.row_tiles = NT;
   p.row_blocks = (a.Tn * a.H + kRows - 1) / kRows;
-  kv4_line_plan(a, p, 148 * 2, 1);
+  // One block per SM of up to two steps, or two blocks that share it.  Measured, us: 4 x 64 steps 17.3 /
+  // 18.2, rows of 320 13.4 / 14.1; 16 x 33 steps 26.3 / 27.2, rows of 320 18.9 / 18.6; 64 x 33 71 / 64.
+  const long long steps = kv4_plan_steps(a) * a.B * p.row_blocks;
+  kv4_line_plan(a, p, steps <= 148 * 2 ? 148 : 148 * 2, 1);
 }
 
 void kv4_latent_launch(const Kv4Attend& a, const Kv4Plan& p, cudaStream_t s) {
