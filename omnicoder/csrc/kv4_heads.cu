@@ -21,10 +21,10 @@
 // The running maximum moves only when a score exceeds it by 2^8, which keeps
 // the shuffles and the rescaling out of most tiles.
 //
-// Measured: 64 sequences x 8192 keys, 48 query heads on 8 of 128: 147 us, 4.1 TB/s
+// Measured: 64 sequences x 8192 keys, 48 query heads on 8 of 128: 146 us, 4.1 TB/s
 // (63 % of the measured copy bandwidth).  Bound by the instruction mix: ALU 51 %,
 // tensor 23 %, FMA 17 %, LSU 21 % of their cycles, which overlap little; 314
-// instructions per 16 keys.  One sequence of 8192 keys: 12.8 us, of 130 keys: 6 us.
+// instructions per 16 keys.  One sequence of 8192 keys: 11.7 us, of 130 keys: 5.1 us.
 #include <algorithm>
 
 #include "kv4_device.cuh"
