@@ -461,6 +461,40 @@ def test_attention_strides_streams_and_graphs(H, Hk, W, latent):
 
 
 @pytest.mark.gpu
+def test_calls_at_once():
+    """Appends, read-backs and attention of two caches on two streams, interleaved without waiting: the
+    bits of each alone."""
+    def chain(c, out):
+        q, kc, kp, vc, vp, q_pos, kv_len, latent, k, v = c
+        for pos in range(3):
+            at = kv_len.long()[:, None] - 1 - pos
+            kv4_write(at, k, kc, kp, v, vc, vp)
+            got = kv4_read(at, kc, kp, vc, vp)
+            out += list(got) if isinstance(got, tuple) else [got]
+            out.append(decode_attention(q, kc, vc, q_pos, kv_len, k_scale=kp, v_scale=vp, latent_v_dim=latent))
+
+    cases = []
+    for H, Hk, W, latent, seed in ((48, 8, 128, 0, 41), (16, 1, 576, 512, 42)):
+        c = _attend_case(9, 1, H, Hk, W, latent, 1500, seed=seed)
+        k = _rows((9, 1, Hk, W), seed + 5).cuda()
+        cases.append((*c, latent, k, None if latent else k.flip(0).contiguous()))
+    for c in cases:
+        chain(c, [])                         # every row in place
+    want = [[], []]
+    for c, o in zip(cases, want):
+        chain(c, o)
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in cases], [[], []]
+    for _ in range(8):
+        for s, c, o in zip(streams, cases, got):
+            with torch.cuda.stream(s):
+                chain(c, o)
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert len(g) == 8 * len(w) and all(torch.equal(x, w[i % len(w)]) for i, x in enumerate(g))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("W,latent", [(128, 0), (320, 256)])
 def test_offsets_beyond_32_bits(W, latent):
     """Codes of more than 2^31 bytes (and 2^32 for the wider row): the last rows are written, read and
@@ -670,3 +704,14 @@ def test_generate_on_gpu(kind, attn):
     ids = torch.randint(0, 512, (2, 200), generator=torch.Generator().manual_seed(5)).cuda()
     out = generate(m, ids, 12, temperature=0.0, kvq="int4")
     assert out.shape == (2, 212) and torch.equal(out[:, :200], ids)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,attn", GPU_KINDS)
+def test_speculative_decoding_on_gpu(kind, attn):
+    """Several new tokens per step, and rejected ones that the next step writes over."""
+    from omnicoder.inference.generate import generate
+    m, draft = (_model(kind, "cuda", torch.bfloat16, **attn) for _ in range(2))
+    ids = torch.randint(0, 512, (2, 100), generator=torch.Generator().manual_seed(6)).cuda()
+    out, st = generate(m, ids, 10, temperature=0.0, kvq="int4", draft_model=draft, speculative_draft_len=3, return_stats=True)
+    assert out.shape == (2, 110) and torch.equal(out[:, :100], ids)
