@@ -1,6 +1,7 @@
 // Tensor-level bindings of the 4-bit key / value cache kernels: every shape,
 // type, stride and device is checked here; the kernels assume them.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -11,6 +12,11 @@ namespace omni {
 namespace {
 
 using OptTensor = c10::optional<at::Tensor>;
+
+// at::empty without the dispatcher: 0.25 us less of the 4 to 6 that a call takes on the host.
+at::Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const at::Device& dev) {
+  return at::detail::empty_cuda(sizes, type, dev, c10::nullopt);
+}
 
 cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
@@ -116,7 +122,7 @@ std::vector<at::Tensor> kv4_read_t(const at::Tensor& pos, const at::Tensor& kc, 
   a.type = kv4_type(dtype, what);
   std::vector<at::Tensor> out;
   for (int i = 0; i < a.count; ++i) {
-    out.push_back(at::empty({a.B, a.T, a.Hk, a.W}, kc.options().dtype(dtype)));
+    out.push_back(empty({a.B, a.T, a.Hk, a.W}, dtype, kc.device()));
     a.rows[i] = Kv4Rows{out[i].data_ptr(), out[i].stride(0), out[i].stride(1), out[i].stride(2)};
   }
   if (a.B == 0 || a.T == 0 || a.Hk == 0) return out;
@@ -171,14 +177,14 @@ at::Tensor kv4_attend_t(const at::Tensor& q_in, const at::Tensor& kc, const at::
   a.scale = (float)scale;
   a.sink_rows = (int)sink_rows;
   a.n_sink = (int)n_sink;
-  auto out = at::empty({a.B, a.Tn, a.H, a.V}, q.options());
+  auto out = empty({a.B, a.Tn, a.H, a.V}, q.scalar_type(), kc.device());
   if (out.numel() == 0) return out;
   if (a.L == 0) return out.zero_();
   a.out = out.data_ptr();
   const Kv4Plan plan = kv4_plan(a);
   at::Tensor ws;
   if (plan.floats > 0) {
-    ws = at::empty({(int64_t)plan.floats}, q.options().dtype(at::kFloat));
+    ws = empty({(int64_t)plan.floats}, at::kFloat, kc.device());
     a.part = ws.data_ptr<float>();
   }
   kv4_attend(a, plan, stream());
