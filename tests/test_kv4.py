@@ -391,6 +391,17 @@ def test_attention_of_many_sequences(H, Hk, W, latent, B, ctx, even, kw):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,Hk,W,latent,B", [(48, 8, 128, 0, 12), (32, 8, 64, 0, 12), (16, 1, 576, 512, 100), (16, 1, 320, 256, 100)])
+@pytest.mark.parametrize("long", [0, 5, -1])
+def test_attention_of_one_long_sequence_among_short_ones(H, Hk, W, latent, B, long):
+    """Fewer steps than blocks, most of them one sequence's."""
+    lens = [1 + i % 3 for i in range(B)]
+    lens[long] = 3900
+    q, kc, kp, vc, vp, q_pos, kv_len = _attend_case(B, 1, H, Hk, W, latent, 4000, seed=26, lens=lens)
+    _check_attention(q, kc, kp, vc, vp, q_pos, kv_len, latent=latent)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("H,Hk,W,latent", [(8, 1, 128, 0), (16, 1, 128, 0), (16, 1, 576, 512), (16, 1, 320, 256)])
 @pytest.mark.parametrize("levels", [(40, -5, -50, -95), (-95, -50, -5, 40), (-60, 30, -60, 30), (40, -100, 40, -100), (-100, 40, -100, 40)])
 def test_attention_scales_that_drop_and_rise(H, Hk, W, latent, levels):
