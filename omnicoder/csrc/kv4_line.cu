@@ -113,16 +113,17 @@ long long kv4_plan_steps(const Kv4Attend& a) {
   return (rows + kKv4Step - 1) / kKv4Step;
 }
 
-// A block per segment costs its steps times the waves of blocks; shared steps cost their share, and
-// about `restart` steps more to find the places and to join the pieces (3 us).  Measured, one query
-// row a sequence, us shared / a block each: 8 heads of 128, 1 sequence of 2, 4, 8 steps 8.4 / 6.2,
-// 8.6 / 8.4, 8.3 / 12.7; 256 sequences of 16 steps 160 / 147; one latent head, 1 sequence of 1, 2, 4
-// steps 11.8 / 9.7, 12.7 / 13.6, 13.2 / 21.4.  Many sequences or new tokens make the places on the
-// line dear to find: a block each.
+// A block per segment costs the steps of the SM with the most of them, the blocks of an SM sharing its
+// pipes; shared steps cost their share, and about `restart` steps more to find the places and to join the
+// pieces.  Measured, one query row a sequence, us shared / a block each: 8 heads of 128, 1 sequence of 2,
+// 4, 8 steps 6.7 / 4.9, 7.3 / 7.2, 7.3 / 11.5, 64 of 8 steps 30.9 / 27.5, 256 of 16 150 / 141; one latent
+// head, 1 sequence of 1, 2, 4 steps 10.2 / 7.9, 11.2 / 11.6, 11.8 / 18.5, 64 of 8 25 / 34, 256 of 16
+// 112 / 105, of up to 16 88 / 103.  Many sequences or new tokens make the places on the line dear to
+// find: a block each.
 void kv4_line_plan(const Kv4Attend& a, Kv4Plan& p, int slots, int restart) {
   const long long steps = kv4_plan_steps(a), segments = (long long)a.B * a.Hk * p.row_blocks;
-  const double waves = (double)segments / slots;
-  const double each = steps * (waves < 4 ? std::ceil(waves) : waves), shared = std::max(1.0, std::ceil(steps * waves)) + restart;
+  const double each = steps * std::max(1.0, (segments + 147) / 148 * 148.0 / slots);
+  const double shared = std::max(1.0, std::ceil((double)steps * segments / slots)) + restart;
   if (each <= shared || a.B > kKv4MaxLine || a.Tn > 16 || segments * (steps + 1) > (1 << 30) ||
       (long long)a.B * a.Tn * a.H * a.V > (1 << 30)) {
     p.restart = 0;

@@ -372,6 +372,7 @@ def test_attention_scales_far_apart(H, Hk, W, latent, far):
 @pytest.mark.parametrize("H,Hk,W,latent", [(48, 8, 128, 0), (32, 8, 64, 0), (48, 4, 128, 0), (64, 4, 64, 0), (16, 1, 576, 512),
                                            (4, 1, 320, 256)])
 @pytest.mark.parametrize("B,ctx,even,kw", [(61, 1100, False, {}), (64, 1100, True, {}), (260, 400, False, {}), (2, 3000, True, {}),
+                                           (61, 3000, False, {}),
                                            (64, 1100, False, {"window": 700, "sink_rows": 40, "n_sink": 37})])
 def test_attention_of_many_sequences(H, Hk, W, latent, B, ctx, even, kw):
     """Batches whose blocks walk several sequences, hold parts of one, or one each; then the same bits
@@ -403,7 +404,8 @@ def test_attention_of_one_long_sequence_among_short_ones(H, Hk, W, latent, B, lo
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("H,Hk,W,latent", [(8, 1, 128, 0), (16, 1, 128, 0), (16, 1, 576, 512), (16, 1, 320, 256)])
-@pytest.mark.parametrize("levels", [(40, -5, -50, -95), (-95, -50, -5, 40), (-60, 30, -60, 30), (40, -100, 40, -100), (-100, 40, -100, 40)])
+@pytest.mark.parametrize("levels", [(40, -5, -50, -95), (-95, -50, -5, 40), (-60, 30, -60, 30), (40, -100, 40, -100),
+                                    (-100, 40, -100, 40)])
 def test_attention_scales_that_drop_and_rise(H, Hk, W, latent, levels):
     """Long runs of rows whose values are 2^level, all of one weight: the largest are the result.  260
     sequences, so that a block walks every run."""
