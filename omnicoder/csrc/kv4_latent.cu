@@ -463,6 +463,9 @@ __global__ void __launch_bounds__(kWarps * 32, PER_SM) kv4_latent_kernel(const K
 #pragma unroll
     for (int n = 0; n < 32; ++n)
       if (warp >= C::VG) to[n * 32] = acc[n >> 3][(n >> 2) & 1][n & 3];
+    // ordinary stores to bytes that the next segment's bulk copies (another proxy) write: a barrier
+    // alone does not order the two
+    fence_proxy_async_smem();
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < 32; ++n)

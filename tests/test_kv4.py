@@ -403,6 +403,23 @@ def test_attention_of_one_long_sequence_among_short_ones(H, Hk, W, latent, B, lo
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,W,latent", [(16, 320, 256), (16, 576, 512)])
+@pytest.mark.parametrize("B,Tn", [(8, 4), (61, 1), (40, 6)])
+def test_latent_blocks_that_walk_several_segments(H, W, latent, B, Tn):
+    """Ragged drafted tokens: a block refills the stages in which its warps have just handed over their
+    sums.  The same bits in every call, and no wait that ran out."""
+    from omnicoder.ops import _ext
+    g = torch.Generator().manual_seed(51)
+    lens = torch.randint(Tn, 2100, (B,), generator=g).tolist()
+    q, kc, kp, _, _, q_pos, kv_len = _attend_case(B, Tn, H, 1, W, latent, 2100, seed=52, lens=lens)
+    first, _ = _check_attention(q, kc, kp, None, None, q_pos, kv_len, latent=latent)
+    kw = dict(k_scale=kp, latent_v_dim=latent)
+    outs = [decode_attention(q, kc, None, q_pos, kv_len, **kw) for _ in range(40)]
+    assert all(torch.equal(o, first) for o in outs)
+    _ext.check_status()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("H,Hk,W,latent", [(8, 1, 128, 0), (16, 1, 128, 0), (16, 1, 576, 512), (16, 1, 320, 256)])
 @pytest.mark.parametrize("levels", [(40, -5, -50, -95), (-95, -50, -5, 40), (-60, 30, -60, 30), (40, -100, 40, -100),
                                     (-100, 40, -100, 40)])
