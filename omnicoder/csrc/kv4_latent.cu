@@ -79,7 +79,9 @@ __global__ void __launch_bounds__(kWarps * 32, PER_SM) kv4_latent_kernel(const K
   int share = 0;
   int2 span = walk.begin<kWarps * 32, kTile>(a, line, &share);
   int used = 0;     // tiles that went through the stages
-  bool ok = true;
+  // Behind a wait that ran out (uniform over the block): nothing is copied or read any more, and this
+  // piece and the block's later ones become NaN; their places are noted all the same.
+  bool dead = false;
 
   while (span.x < span.y) {
   Kv4Piece piece = walk.next<kTile>(a, line, share, &span);
@@ -93,7 +95,8 @@ __global__ void __launch_bounds__(kWarps * 32, PER_SM) kv4_latent_kernel(const K
     if (w < kWords && r < nrows) kv4_load8<TYPE>(a.q, ((long long)b * R + row0 + r) * W + w * 8, x[e]);
   }
   const Kv4View see = kv4_rows<kTile>(a, line, &piece, row0, nrows);
-  const int sink_tiles = piece.sink_tiles, first = piece.first, t0 = piece.step0, t1 = min(piece.tiles, piece.step1);
+  const int sink_tiles = piece.sink_tiles, first = piece.first, t0 = piece.step0;
+  const int t1 = dead ? t0 : min(piece.tiles, piece.step1);
   auto row_of = [&](int tile) { return (tile < sink_tiles ? tile : first + tile - sink_tiles) * kTile; };
 
   const uint8_t* kc = a.k.codes + b * a.k.c_b;
@@ -185,7 +188,7 @@ __global__ void __launch_bounds__(kWarps * 32, PER_SM) kv4_latent_kernel(const K
 #pragma unroll
       for (int c = 0; c < 4; ++c) acc[mm][nt][c] = 0.f;
     accm[nt] = 0.f;
-    lsum[nt][0] = lsum[nt][1] = 0.f;
+    lsum[nt][0] = lsum[nt][1] = dead ? __int_as_float(0x7fffffff) : 0.f;
     limit[nt][0] = limit[nt][1] = -INFINITY;
     ref[nt][0] = ref[nt][1] = 0.f;
   }
@@ -197,9 +200,13 @@ __global__ void __launch_bounds__(kWarps * 32, PER_SM) kv4_latent_kernel(const K
   const int vg = warp % C::VG, kt0 = warp / C::VG * (kTile / 16 / KS);
   const int key_0 = (2 * j) ^ ((j >> 1) & 1), key_1 = (2 * j + 1) ^ ((j >> 1) & 1);
 
+  auto landed = [&](int tile, int code) {
+    const int n = used + tile - t0;
+    return mbar_wait(&full[n % kStages], (n / kStages) & 1, st, code);
+  };
   for (int tile = t0; tile < t1; ++tile) {
     const int stage = (used + tile - t0) % kStages;
-    ok = mbar_wait(&full[stage], ((used + tile - t0) / kStages) & 1, st, STATUS_TIMEOUT_TMA_FULL) && ok;
+    const bool late = !landed(tile, STATUS_TIMEOUT_TMA_FULL);
     const uint32_t codes = smem_u32(smem + stage * C::kStage), params = codes + C::kCodes;
     const int r0 = row_of(tile);
 
@@ -267,7 +274,7 @@ __global__ void __launch_bounds__(kWarps * 32, PER_SM) kv4_latent_kernel(const K
         above |= top[nt][c] > limit[nt][c];
       }
     // also the barrier behind the previous tile's reads of the weights
-    if (__syncthreads_or(above)) {
+    if (__syncthreads_or(above || late)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -277,7 +284,13 @@ __global__ void __launch_bounds__(kWarps * 32, PER_SM) kv4_latent_kernel(const K
           for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
           if (i == 0) smx[warp * kRows + nt * 8 + 2 * j + c] = x;
         }
-      __syncthreads();
+      if (__syncthreads_or(late)) {
+        dead = true;
+        for (int k = tile; k < min(tile + kStages, t1); ++k) landed(k, STATUS_TIMEOUT_DRAIN);  // copies in flight
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) lsum[nt][0] = lsum[nt][1] = __int_as_float(0x7fffffff);
+        break;
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -502,7 +515,6 @@ __global__ void __launch_bounds__(kWarps * 32, PER_SM) kv4_latent_kernel(const K
     }
   __syncthreads();  // the next segment refills shared memory
   }
-  (void)ok;
 }
 
 template <int V, int TYPE, int PER_SM>
