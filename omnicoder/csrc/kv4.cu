@@ -26,9 +26,11 @@ constexpr float kMinScale = 7.52316384526264e-37f;  // 2^-120
 // ---------------------------------------------------------------------------
 constexpr int kPiece = 16;
 
+// Ordinary loads: the read-only path is for memory that nobody writes while the kernel lives, and this one
+// is alive before its predecessor has written the rows.
 __device__ __forceinline__ void load32(const void* p, uint32_t* w) {
-  *reinterpret_cast<uint4*>(w) = __ldg(reinterpret_cast<const uint4*>(p));
-  *reinterpret_cast<uint4*>(w + 4) = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+  *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(p);
+  *reinterpret_cast<uint4*>(w + 4) = *(reinterpret_cast<const uint4*>(p) + 1);
 }
 // Rows to read into are allocated by the call and start on 32-byte boundaries.
 __device__ __forceinline__ void store32(void* p, const uint32_t* w) {

@@ -572,6 +572,31 @@ def test_gpu_refusals():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_writes_of_rows_that_were_just_made(dtype):
+    """A write is set up while the kernel before it still makes its rows: read-backs of one cache into
+    the next, and rows written over in place, without a pause."""
+    src = [kv4_alloc(2, 2, 512, 64, device="cuda") for _ in range(4)]
+    pos = torch.arange(512, device="cuda").expand(2, -1).contiguous()
+    for i, (c, p) in enumerate(src):
+        kv4_write(pos, _rows((2, 512, 2, 64), 60 + i).cuda(), c, p)
+    want = [quantize_kv4(kv4_read(pos, c, p, dtype=dtype).cpu(), 64) for c, p in src]
+    to = [kv4_alloc(2, 2, 512, 64, device="cuda") for _ in range(64)]
+    for i, (c, p) in enumerate(to):
+        kv4_write(pos, kv4_read(pos, *src[i % 4], dtype=dtype), c, p)
+    for i, (c, p) in enumerate(to):
+        assert torch.equal(c.cpu(), want[i % 4][0].transpose(1, 2)) and torch.equal(p.cpu(), want[i % 4][1].transpose(1, 2))
+    x = torch.empty(2, 512, 2, 64, dtype=dtype, device="cuda")
+    made = [_rows((2, 512, 2, 64), 70 + i, dtype).cuda() for i in range(4)]
+    want = [quantize_kv4(m.cpu(), 64) for m in made]
+    for i, (c, p) in enumerate(to):
+        x.copy_(made[i % 4])
+        kv4_write(pos, x, c, p)
+    for i, (c, p) in enumerate(to):
+        assert torch.equal(c.cpu(), want[i % 4][0].transpose(1, 2)) and torch.equal(p.cpu(), want[i % 4][1].transpose(1, 2))
+
+
+@pytest.mark.gpu
 def test_write_takes_views():
     """Keys and values as slices of a fused projection, without a copy or with one where they do not
     start on 16-byte boundaries."""
