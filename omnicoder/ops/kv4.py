@@ -83,7 +83,15 @@ def quantize_kv4(x: torch.Tensor, group: int):
     s = ((g.amax(-1).float() - m.float()) * (1.0 / 15.0)).to(torch.bfloat16)
     bad = ~(torch.isfinite(g).all(-1) & torch.isfinite(m) & torch.isfinite(s))
     s = torch.where(s.float() < _MIN_SCALE, torch.zeros_like(s), s)
-    n = torch.round((g - m.double()[..., None]) / s.double()[..., None]).clamp(0, 15)
+    md, sd = m.double()[..., None], s.double()[..., None]
+    d = g - md                           # d + e = x - m exactly: an x far below m is not lost
+    back = d - g
+    e = (g - (d - back)) - (md + back)
+    n = torch.round(d / sd)
+    r, half, odd = d - n * sd, 0.5 * sd, n % 2 != 0
+    n = n + ((r > half) | ((r == half) & ((e > 0) | ((e == 0) & odd)))).double()
+    n = n - ((r < -half) | ((r == -half) & ((e < 0) | ((e == 0) & odd)))).double()
+    n = n.clamp(0, 15)
     n = torch.where((bad | (s == 0))[..., None], torch.zeros_like(n), n).to(torch.uint8)
     n = n.reshape(*x.shape[:-1], x.shape[-1] // 2, 2)
     p = torch.stack([s, m], -1)

@@ -101,6 +101,35 @@ def test_hard_rows(device, dtype):
 
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_values_far_below_a_border(device, dtype):
+    """x - m is half a step away from a code but for an x that no 64-bit difference keeps: rounded as
+    the exact quotient, taken in fractions.  Borders k + 1/2 with k even and odd, s = 2^p."""
+    from fractions import Fraction
+    top = 12 if dtype == torch.float16 else 100
+    rows = []
+    for p in (0, -3, top):                             # m = -(k + 1/2) s, max = m + 15 s, both exact in bf16
+        for k in range(0, 15):
+            s = 2.0 ** p
+            r = torch.zeros(64, dtype=torch.float64)
+            r[0], r[1] = -(k + 0.5) * s, (14.5 - k) * s
+            small = [2.0 ** -24] if dtype == torch.float16 else [2.0 ** e for e in (-20, -52, -60, -100, -126)]
+            for i, t in enumerate(small):
+                r[2 + 2 * i], r[3 + 2 * i] = t, -t
+            rows.append(r)
+    x = torch.stack(rows).to(dtype)[None, :, None, :].contiguous()
+    T = x.shape[1]
+    codes, params = kv4_alloc(1, 1, T, 64, device=device)
+    pos = torch.arange(T, device=device)[None]
+    kv4_write(pos, x.to(device), codes, params)
+    n = torch.stack([codes & 15, codes >> 4], -1).reshape(-1, 64)[:T].cpu()
+    for t in range(T):
+        s, m = (Fraction(float(params[0, 0, t, 0, i])) for i in range(2))
+        want = [min(15, max(0, round((Fraction(float(v)) - m) / s))) for v in x[0, t, 0]]      # ties to even
+        assert n[t].tolist() == want, t
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("B,T,Hk,W,latent", [(3, 5, 4, 128, 0), (2, 1, 1, 576, 512), (1, 33, 2, 64, 0), (2, 7, 1, 176, 128),
                                              (2, 3, 3, 32, 0), (1, 2, 1, 192, 160)])
 def test_write_and_read(device, dtype, B, T, Hk, W, latent):
