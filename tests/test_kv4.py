@@ -128,6 +128,64 @@ def test_values_far_below_a_border(device, dtype):
         assert n[t].tolist() == want, t
 
 
+def _border_rows(n, dtype, seed):
+    """[1, n, 1, 64] groups whose values lie on borders between codes or a few units of the last place
+    beside them, next to the sizes at which the kernel decides in another way: minima of every size
+    from 2^-20 of the range to 2^6 times it, values around 2^-16 of the range, scales down to 2^-100."""
+    g = torch.Generator().manual_seed(seed)
+    lo_e = (-3, 3) if dtype == torch.float16 else (-100, 100)
+    size = 2.0 ** torch.randint(lo_e[0], lo_e[1] + 1, (n, 1), generator=g).double()
+    R = (1 + torch.rand(n, 1, generator=g).double()) * size
+    least = R * torch.randn(n, 1, generator=g).double().sign() * 2.0 ** torch.randint(-20, 7, (n, 1), generator=g).double()
+    least = torch.where(torch.rand(n, 1, generator=g) < 0.5, -R * torch.rand(n, 1, generator=g).double(), least)
+    least = torch.where(torch.rand(n, 1, generator=g) < 0.1, torch.zeros_like(least), least)
+    x = torch.zeros(n, 64, dtype=torch.float64)
+    x[:, 0], x[:, 1] = least[:, 0], least[:, 0] + R[:, 0]
+    x = x.to(dtype)
+    lo = x[:, :2].amin(-1).float()
+    m = lo.to(torch.bfloat16).double()[:, None]
+    s = ((x[:, :2].amax(-1).float() - m[:, 0].float()) * (1.0 / 15.0)).to(torch.bfloat16).double()[:, None]
+    k = torch.randint(0, 15, (n, 62), generator=g).double()
+    at = (m + (k + 0.5) * s).to(dtype)
+    word = torch.int32 if dtype == torch.float32 else torch.int16
+    near = (at.view(word) + torch.randint(-3, 4, (n, 62), generator=g).to(word)).view(dtype)
+    tiny = (R * 2.0 ** -torch.randint(14, 40, (n, 62), generator=g).double() *
+            torch.randn(n, 62, generator=g).double().sign()).to(dtype)
+    pick = torch.where(torch.rand(n, 62, generator=g) < 0.15, tiny, near)
+    hi = x[:, :2].amax(-1, keepdim=True)
+    ok = torch.isfinite(pick) & (pick >= lo[:, None].to(dtype)) & (pick <= hi)       # the range stays
+    x[:, 2:] = torch.where(ok, pick, x[:, :1].expand(-1, 62))
+    return x[None, :, None, :].contiguous()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_plain_codes_next_to_borders(dtype):
+    """The plain form against fractions."""
+    from fractions import Fraction
+    x = _border_rows(150, dtype, 80)
+    codes, params = quantize_kv4(x, 64)
+    n = torch.stack([codes & 15, codes >> 4], -1).reshape(-1, 64)
+    for t in range(x.shape[1]):
+        s, m = (Fraction(float(params[0, t, 0, 0, i])) for i in range(2))
+        want = [min(15, max(0, round((Fraction(float(v)) - m) / s))) for v in x[0, t, 0]]
+        assert n[t].tolist() == want, t
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("seed", [81, 82, 83])
+def test_codes_next_to_borders(dtype, seed):
+    """The kernel against the plain form: a million values, most of them within three units of the last
+    place of a border."""
+    x = _border_rows(1 << 14, dtype, seed)
+    T = x.shape[1]
+    codes, params = kv4_alloc(1, 1, T, 64, device="cuda")
+    kv4_write(torch.arange(T, device="cuda")[None], x.cuda(), codes, params)
+    want_c, want_p = quantize_kv4(x, 64)
+    assert torch.equal(params[0, 0].cpu(), want_p[0, :, 0])
+    assert torch.equal(codes[0, 0].cpu(), want_c[0, :, 0])
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("B,T,Hk,W,latent", [(3, 5, 4, 128, 0), (2, 1, 1, 576, 512), (1, 33, 2, 64, 0), (2, 7, 1, 176, 128),
