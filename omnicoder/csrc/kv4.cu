@@ -269,7 +269,9 @@ __global__ void __launch_bounds__(kIoThreads) kv4_write_kernel(const Kv4IO a, co
         probe += p2;
       }
     }
-    // m is exact for bf16 rows; the scale is taken from the rounded minimum
+    // m is exact for bf16 rows; the scale is taken from the rounded minimum, as a product with
+    // fp32(1 / 15): where the quotient by 15 would lie halfway between two bf16 numbers (0.05 % of random
+    // bf16 ranges) that decides which of the two is stored.  The codes refer to the stored one.
     const bf16 mb = __float2bfloat16_rn(lo);
     const float m = __bfloat162float(mb);
     const float range = hi - m;

@@ -9,7 +9,8 @@ and stands for x = n * s + m, n = 0 .. 15.  A row of a head is contiguous, and s
 head (head-major, unlike the bf16 / int8 cache): the attention kernels copy whole key tiles.  With
 groups of 64 a value takes 4.5 bits; an int8 cache of 128-wide heads takes 8.25.
 
-Quantisation of a group: m = bf16(min x), s = bf16((max x - m) * (1 / 15)) with the product in fp32, and
+Quantisation of a group: m = bf16(min x), s = bf16((max x - m) * (1 / 15)) with the product in fp32 (torch
+on a GPU divides by 15 so, on a CPU it does not: quotients halfway between two bf16 numbers differ), and
 n = clamp(round((x - m) / s), 0, 15), where the rounding (ties to even) is decided as if (x - m) / s
 were exact.  s below 2^-120 is stored as 0 (then every n is 0 and the group reads back as m).  A group
 that holds a NaN or an infinity, or whose range overflows fp32, reads back as NaN; other groups of

@@ -128,6 +128,25 @@ def test_values_far_below_a_border(device, dtype):
         assert n[t].tolist() == want, t
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_scale_is_the_product_with_a_fifteenth(device, dtype):
+    """Ranges of 15 times an odd 9-bit number: the quotient by 15 lies halfway between two bf16 scales, the
+    product with fp32(1 / 15) beside it.  The format takes the product."""
+    q = torch.arange(257, 512, 2)
+    R = 15 * q                                          # <= 7665: hi = its upper bits, lo = -(the rest)
+    hi = R // 32 * 32
+    x = torch.zeros(1, len(q), 1, 64)
+    x[0, :, 0, 0], x[0, :, 0, 1] = hi.float(), (hi - R).float()
+    codes, params = kv4_alloc(1, 1, len(q), 64, device=device)
+    kv4_write(torch.arange(len(q), device=device)[None], x.to(dtype).to(device), codes, params)
+    fifteenth = torch.tensor(1.0 / 15.0).double()       # fp32(1 / 15); the product of 13 and 24 bits is exact in 64
+    want = (R.double() * fifteenth).float().to(torch.bfloat16)
+    even = torch.where(q % 4 == 1, q - 1, q + 1).to(torch.bfloat16)
+    assert torch.equal(params[0, 0, :len(q), 0, 0].cpu(), want)
+    assert (want != even).sum() > 40                    # the quotient would round these to the other side
+
+
 def _border_rows(n, dtype, seed):
     """[1, n, 1, 64] groups whose values lie on borders between codes or a few units of the last place
     beside them, next to the sizes at which the kernel decides in another way: minima of every size
