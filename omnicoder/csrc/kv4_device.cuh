@@ -183,6 +183,26 @@ __device__ __forceinline__ float q_normaliser(float amax, float* unscale) {
   return __uint_as_float((268u - e) << 23);     // 2^(14 - (e - 127))
 }
 
+// Factor of a row's raw scores: the row's unscale, the softmax scale, log2 e and kKv4Codes.  That can
+// leave fp32 where the scores do not (|q| scale from 2^117 on, small keys), so rows are prepared without
+// kKv4Codes, and where one of a block's is kKv4Huge or more, all are multiplied in two steps: here by
+// kKv4Codes / kKv4Lift and, in the loop's branch for tiles that some row does not see whole, by kKv4Lift.
+constexpr float kKv4Huge = 1.2676506e30f, kKv4Lift = 4294967296.f;  // 2^100, 2^32
+template <int N>
+__device__ __forceinline__ bool kv4_score_factors(float (*rs)[2]) {  // this lane's; the warp holds every row
+  bool huge = false;
+#pragma unroll
+  for (int n = 0; n < N; ++n) huge = huge || fabsf(rs[n][0]) >= kKv4Huge || fabsf(rs[n][1]) >= kKv4Huge;
+  huge = __any_sync(0xffffffffu, huge);
+  const float by = huge ? kKv4Codes / kKv4Lift : kKv4Codes;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    rs[n][0] *= by;
+    rs[n][1] *= by;
+  }
+  return huge;
+}
+
 // Eight dims of a normalised query, the partners of a code word: operands of two k steps (nibbles
 // 0 and 4 with 1 and 5, 2 and 6 with 3 and 7; the second pair of each counts 16-fold); -> their sum
 // (what fp16 rounds off is below 2^-39 of the row's largest).

@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if ((w & 7) == 0) sqs[r * NG + (w >> 3)] = sum * (1.f / kKv4Codes);
-    if (w == 0) srs[r] = un * (a.scale * (kKv4Log2e * kKv4Codes));
+    if (w == 0) srs[r] = un * (a.scale * kKv4Log2e);
   }
   __syncthreads();
   // operand of the scores: lane (i, j) holds query row i against the 16 dims that it reads of each group
@@ -161,6 +161,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
       rs[nt][c] = srs[nt * 8 + 2 * j + c];
     }
   }
+  const bool huge = kv4_score_factors<NT>(rs);
 
   float f[NG];                     // the values' power of two; 0 before any
 #pragma unroll
@@ -198,7 +199,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
     if (next < t1) issue(next, stage == 0 ? C::kStages - 1 : stage - 1);
     kv4_cp_commit();
     const int r0 = row_of(tile);
-    const bool masked = !(r0 + kTile <= a.n_sink || (r0 >= see.lo_max && r0 + kTile <= see.hi_min));
+    const bool masked = huge || !(r0 + kTile <= a.n_sink || (r0 >= see.lo_max && r0 + kTile <= see.hi_min));
     uint32_t st = ring + stage * C::kStage, sp = st + 2 * C::kCodes + i * NG * 4;
     // ---- do the scales of the tile's values fit their power of two?  Lane: key r0 + lane ----
     bool slow[NG];
@@ -287,6 +288,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
           for (int c = 0; c < 2; ++c) {
             const int lo = __shfl_sync(0xffffffffu, see.seen.lo, nt * 8 + 2 * j + c);
             const int hi = __shfl_sync(0xffffffffu, see.seen.hi, nt * 8 + 2 * j + c);
+            if (huge) {
+              s[nt][c] *= kKv4Lift;
+              s[nt][c + 2] *= kKv4Lift;
+            }
             if (!(r < a.n_sink || (r >= lo && r < hi))) s[nt][c] = -INFINITY;
             if (!(r + 8 < a.n_sink || (r + 8 >= lo && r + 8 < hi))) s[nt][c + 2] = -INFINITY;
           }

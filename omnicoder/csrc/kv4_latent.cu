@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kWarps * 32, PER_SM) kv4_latent_kernel(const K
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       sc[h] = q_normaliser(warp_max(amax[h]), &un[h]);
-      if (lane == h) srs[r0 + h] = un[h] * (a.scale * (kKv4Log2e * kKv4Codes));
+      if (lane == h) srs[r0 + h] = un[h] * (a.scale * kKv4Log2e);
     }
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
@@ -177,6 +177,7 @@ __global__ void __launch_bounds__(kWarps * 32, PER_SM) kv4_latent_kernel(const K
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int c = 0; c < 2; ++c) rs[nt][c] = srs[nt * 8 + 2 * j + c];
+  const bool huge = kv4_score_factors<NT>(rs);
 
   // acc[mm]: value dims mm and 4 + mm of a lane's eight; accm: sums of p m
   float f = 0.f;   // the values' power of two; 0 before any
@@ -250,7 +251,7 @@ __global__ void __launch_bounds__(kWarps * 32, PER_SM) kv4_latent_kernel(const K
 #pragma unroll
         for (int c = 0; c < 4; ++c) s[nt][c] = fmaf(d[nt][c], c < 2 ? sa : sb, s[nt][c]);
     }
-    const bool masked = !(r0 + kTile <= a.n_sink || (r0 >= see.lo_max && r0 + kTile <= see.hi_min));
+    const bool masked = huge || !(r0 + kTile <= a.n_sink || (r0 >= see.lo_max && r0 + kTile <= see.hi_min));
     bool above = false;
     float top[NT][2];
 #pragma unroll
@@ -263,6 +264,7 @@ __global__ void __launch_bounds__(kWarps * 32, PER_SM) kv4_latent_kernel(const K
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const int r = r0 + warp * 16 + key_i + (c >> 1) * 8, q = nt * 8 + 2 * j + (c & 1);
+          if (huge) s[nt][c] *= kKv4Lift;
           if (!(r < a.n_sink || (r >= slo[q] && r < shi[q]))) s[nt][c] = -INFINITY;
         }
     }

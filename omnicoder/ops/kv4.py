@@ -195,9 +195,9 @@ def decode_attention_kv4(q, k, v, q_pos, kv_len, *, window=0, scale=None, k_para
                          latent_v_dim=0, sink_rows=0, n_sink=0):
     """Attention of new tokens q [B, Tn, H, W] against a 4-bit cache (k, v codes; v None with
     latent_v_dim = r for an MLA latent, whose value is the first r dims of a row).  Visibility as in
-    omnicoder.ops.decode; a query that sees no row gets zeros.  Sums are fp32 in units of the largest
-    scale of a head's rows: values up to 2^100, and of rows whose scales differ by more than 2^90 the
-    smaller ones may be lost.  -> [B, Tn, H, W or r]."""
+    omnicoder.ops.decode; a query that sees no row gets zeros.  |q| scale and scores up to 2^127.  Sums
+    are fp32 in units of the largest scale of a head's rows: values up to 2^100, and of rows whose
+    scales differ by more than 2^90 the smaller ones may be lost.  -> [B, Tn, H, W or r]."""
     sc = scale if scale is not None else 1.0 / math.sqrt(q.shape[3])
     if q.is_cuda:                        # checked by the bindings
         return _ext.load().kv4_attend(q, k, k_params, v, v_params, q_pos, kv_len, window, sc, latent_v_dim,

@@ -429,6 +429,26 @@ def test_attention_nan_of_one_group(H, Hk, W, latent):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,Hk,W,latent", HEADS)
+@pytest.mark.parametrize("window", [0, 40])
+def test_attention_of_huge_queries(H, Hk, W, latent, window):
+    """Queries of 2^122 against keys of 2^-118 beside queries of usual size and of zeros: the scores are
+    of usual size, but no single fp32 factor takes a normalised query's product to them."""
+    q, kc, kp, vc, vp, q_pos, kv_len = _attend_case(3, 2, H, Hk, W, latent, 400, seed=31, lens=[400, 1, 257])
+    g = W // kp.shape[3]
+    if latent:                               # small keys in the dims that are not the value
+        q[..., :latent] = 0
+        kp[:, :, :, latent // g:] *= 2.0 ** -118
+    else:
+        kp *= 2.0 ** -118
+    q *= 2.0 ** 122
+    q[1, 0] *= 2.0 ** -140
+    q[2, 1, ::2] = 0
+    out, _ = _check_attention(q, kc, kp, vc, vp, q_pos, kv_len, latent=latent, window=window, scale=W ** -0.5)
+    assert torch.isfinite(out).all() and (out != 0).any()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("H,Hk,W,latent", [(8, 8, 128, 0), (16, 1, 576, 512), (4, 4, 32, 0)])
 def test_attention_extreme_values(H, Hk, W, latent):
     """Scores far apart, large and tiny queries, scales of very different size, one head of zeros."""
