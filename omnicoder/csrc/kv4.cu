@@ -446,6 +446,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv4_row_kernel(const Kv4Attend
     const int r0 = (tile < piece.sink_tiles ? tile : piece.first + tile - piece.sink_tiles) * 32;
     const int r = r0 + lane;
     const bool vis = r < a.n_sink || (r >= seen.lo && r < seen.hi);
+    const uint32_t seen_rows = __ballot_sync(0xffffffffu, vis);
     float s = -INFINITY;
     if (vis) {
       s = 0.f;
@@ -470,7 +471,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv4_row_kernel(const Kv4Attend
     for (int i = 0; i < kRowDims; ++i) o[i] *= alpha;
     for (int k = 0; k < 32; ++k) {
       const float pk = __shfl_sync(0xffffffffu, p, k);
-      if (pk == 0.f) continue;  // unseen rows, whatever they hold
+      if (!(seen_rows >> k & 1)) continue;  // whatever they hold
       const long long rk = r0 + k;
 #pragma unroll
       for (int i = 0; i < kRowDims; ++i) {

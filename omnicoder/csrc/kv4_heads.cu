@@ -281,6 +281,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 4; ++c) s[nt][c] *= rs[nt][c & 1];
+      uint32_t hidden = 0;   // bit 4 nt + c: the row does not see the key
       if (masked) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -292,8 +293,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
               s[nt][c] *= kKv4Lift;
               s[nt][c + 2] *= kKv4Lift;
             }
-            if (!(r < a.n_sink || (r >= lo && r < hi))) s[nt][c] = -INFINITY;
-            if (!(r + 8 < a.n_sink || (r + 8 >= lo && r + 8 < hi))) s[nt][c + 2] = -INFINITY;
+            if (!(r < a.n_sink || (r >= lo && r < hi))) {
+              s[nt][c] = -INFINITY;
+              hidden |= 1u << (4 * nt + c);
+            }
+            if (!(r + 8 < a.n_sink || (r + 8 >= lo && r + 8 < hi))) {
+              s[nt][c + 2] = -INFINITY;
+              hidden |= 4u << (4 * nt + c);
+            }
           }
       }
 #pragma unroll
@@ -351,10 +358,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv4_heads_kernel
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) x[nt][c] = s[nt][c] * (c < 2 ? fa : fb);
-          if (masked) {  // a key that a row does not see may hold anything
+          if (masked) {  // a key that a row does not see may hold anything; one that it sees counts, whatever its weight
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              if (s[nt][c] == 0.f) x[nt][c] = 0.f;
+              if (hidden >> (4 * nt + c) & 1) x[nt][c] = 0.f;
               else accm[g][nt][c & 1] = fmaf(s[nt][c], c < 2 ? ma : mb, accm[g][nt][c & 1]);
             }
           } else {

@@ -448,6 +448,27 @@ def test_attention_of_huge_queries(H, Hk, W, latent, window):
     assert torch.isfinite(out).all() and (out != 0).any()
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("H,Hk,W", [(48, 8, 128), (8, 8, 128), (16, 2, 64), (4, 4, 32), (12, 2, 96)])
+@pytest.mark.parametrize("row", [5, 70, 149])
+def test_attention_nan_of_no_weight(device, H, Hk, W, row):
+    """A NaN in a row that a query sees counts, however small the row's weight: in a tile that every
+    query sees whole and in one that ends inside the sequence."""
+    q, kc, kp, vc, vp, q_pos, kv_len = _attend_case(2, 2, H, Hk, W, 0, 200, seed=32, device=device, lens=[150, 60])
+    kw = dict(scale=0.5, window=148)         # row 5 is seen by both queries of sequence 0
+    q.zero_()
+    q[..., 0] = 2.0
+    kp[..., 0], kp[..., 1] = 0, 0            # scores 0, and -400 for the row
+    kp[:, :, row, :, 1] = -400.0
+    clean = decode_attention(q, kc, vc, q_pos, kv_len, k_scale=kp, v_scale=vp, **kw)
+    assert torch.isfinite(clean).all()
+    vp[0, :, row, 0] = float("nan")
+    out = decode_attention(q, kc, vc, q_pos, kv_len, k_scale=kp, v_scale=vp, **kw)
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    bad[0, (1 if row == 149 else 0):, :, :W // vp.shape[3]] = True
+    assert torch.equal(torch.isnan(out), bad) and torch.equal(out[~bad], clean[~bad])
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("H,Hk,W,latent", [(8, 8, 128, 0), (16, 1, 576, 512), (4, 4, 32, 0)])
 def test_attention_extreme_values(H, Hk, W, latent):
