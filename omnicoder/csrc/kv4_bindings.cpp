@@ -92,8 +92,9 @@ void kv4_write_t(const at::Tensor& pos, const at::Tensor& k, const at::Tensor& k
   Kv4IO a{};
   at::Tensor p = pos.contiguous(), keep[2];
   fill_io(a, p, kc, kp, vc, vp, row_offset, what);
-  TORCH_CHECK(a.count == 1 || a.cache[0].codes != a.cache[1].codes || a.cache[0].codes == nullptr, what,
-              ": k and v need caches of their own");
+  TORCH_CHECK(a.count == 1 || a.cache[0].codes == nullptr ||
+                  (a.cache[0].codes != a.cache[1].codes && a.cache[0].params != a.cache[1].params),
+              what, ": k and v need caches of their own");
   a.type = kv4_type(k.scalar_type(), what);
   for (int i = 0; i < a.count; ++i) {
     at::Tensor x = i == 0 ? k : *v;

@@ -156,7 +156,7 @@ def kv4_write(pos, k, k_codes, k_params, v=None, v_codes=None, v_params=None, ro
                 or x.shape[2] != c.shape[1] or x.shape[3] != 2 * c.shape[3]:
             raise ValueError(f"kv4_write: {what} {tuple(x.shape)} does not fit positions {tuple(pos.shape)} and codes "
                              f"{tuple(c.shape)}")
-    if v is not None and v_codes.data_ptr() == k_codes.data_ptr() != 0:
+    if v is not None and (v_codes.data_ptr() == k_codes.data_ptr() != 0 or v_params.data_ptr() == k_params.data_ptr() != 0):
         raise ValueError("kv4_write: k and v need caches of their own")
     rows = pos.long() + row_offset
     for x, c, p, _ in pairs:

@@ -280,6 +280,20 @@ def test_refusals():
             decode_attention(*args, k_scale=p, v_scale=p, **kw)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_one_tensor_for_keys_and_values_is_refused(device):
+    """Codes or parameters that k and v would both write; heads of one allocation are fine."""
+    (kc, kp), (vc, vp) = (kv4_alloc(1, 2, 32, 64, device=device) for _ in range(2))
+    pos, x = torch.zeros(1, 1, dtype=torch.long, device=device), torch.ones(1, 1, 2, 64, device=device)
+    for pair in ((kc, vp), (vc, kp), (kc, kp)):
+        with pytest.raises((ValueError, RuntimeError), match="caches of their own"):
+            kv4_write(pos, x, kc, kp, x, *pair)
+    assert (kc == 0).all() and (kp == 0).all()
+    c, p = kv4_alloc(1, 4, 32, 64, device=device)
+    kv4_write(pos, x, c[:, :2], p[:, :2], 2 * x, c[:, 2:], p[:, 2:])
+    assert p[0, :, 0, 0, 1].tolist() == [1, 1, 2, 2]
+
+
 # ----------------------------------------------------------------------------------------------
 # attention
 # ----------------------------------------------------------------------------------------------
