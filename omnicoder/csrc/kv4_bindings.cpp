@@ -47,9 +47,9 @@ Kv4Cache cache_of(const at::Tensor& c, const at::Tensor& p, const at::Device& de
               what, ": the rows of a head must be contiguous");
   Kv4Cache o{reinterpret_cast<uint8_t*>(c.data_ptr()), reinterpret_cast<uint8_t*>(p.data_ptr()), c.stride(0),
              c.stride(1), 2 * p.stride(0), 2 * p.stride(1)};
-  TORCH_CHECK((reinterpret_cast<uintptr_t>(o.codes) | reinterpret_cast<uintptr_t>(o.params) | (uintptr_t)o.c_b |
-               (uintptr_t)o.c_h | (uintptr_t)o.p_b | (uintptr_t)o.p_h) % 16 == 0,
-              what, ": heads and sequences must start on 16-byte boundaries");
+  const uintptr_t places = reinterpret_cast<uintptr_t>(o.codes) | reinterpret_cast<uintptr_t>(o.params) |
+                           (uintptr_t)o.c_b | (uintptr_t)o.c_h | (uintptr_t)o.p_b | (uintptr_t)o.p_h;
+  TORCH_CHECK(c.numel() == 0 || places % 16 == 0, what, ": heads and sequences must start on 16-byte boundaries");
   return o;
 }
 

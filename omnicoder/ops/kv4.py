@@ -112,11 +112,13 @@ def decode_attention_kv4_torch(q, k, v, q_pos, kv_len, *, window=0, scale=None, 
     """Dense masked softmax over the dequantised cache; rows that see nothing give zeros."""
     B, Tn, H, W = q.shape
     sc = scale if scale is not None else 1.0 / math.sqrt(W)
-    Hk, L = k.shape[1], k.shape[2]
+    Hk, L, G = k.shape[1], k.shape[2], H // k.shape[1]
+    if L == 0 or q.numel() == 0:
+        return q.new_zeros(B, Tn, H, latent_v_dim or W)
     ct = torch.float64 if q.dtype == torch.float64 else torch.float32
     kf = dequantize_kv4(k, k_params, ct)
     vf = kf[..., :latent_v_dim] if latent_v_dim else dequantize_kv4(v, v_params, ct)
-    qf = q.to(ct).reshape(B, Tn, Hk, H // Hk, W).permute(0, 2, 1, 3, 4)                  # [B, Hk, Tn, G, W]
+    qf = q.to(ct).reshape(B, Tn, Hk, G, W).permute(0, 2, 1, 3, 4)                        # [B, Hk, Tn, G, W]
     s = torch.matmul(qf.reshape(B, Hk, -1, W), kf.transpose(-1, -2)) * sc               # [B, Hk, Tn * G, L]
     rows = torch.arange(L, device=q.device)
     p, t = rows - sink_rows, q_pos.long()[:, :, None]
@@ -124,7 +126,7 @@ def decode_attention_kv4_torch(q, k, v, q_pos, kv_len, *, window=0, scale=None, 
     if window > 0:
         seen = seen & (p > t - window)
     seen = seen | (rows < n_sink)                                                        # [B, Tn, L]
-    seen = seen[:, None, :, None].expand(B, Hk, Tn, H // Hk, L).reshape(s.shape)
+    seen = seen[:, None, :, None].expand(B, Hk, Tn, G, L).reshape(s.shape)
     s = s.masked_fill(~seen, float("-inf"))
     top = s.amax(-1, keepdim=True)
     e = torch.exp(s - torch.where(top == float("-inf"), torch.zeros_like(top), top))
@@ -133,7 +135,7 @@ def decode_attention_kv4_torch(q, k, v, q_pos, kv_len, *, window=0, scale=None, 
     o = torch.matmul(w, torch.where(finite, vf, torch.zeros_like(vf)))
     if not bool(finite.all()):                     # a NaN counts for the queries that see its row
         o = o.masked_fill(torch.matmul(seen.to(ct), (~finite).to(ct)) > 0, float("nan"))
-    return o.reshape(B, Hk, Tn, H // Hk, -1).permute(0, 2, 1, 3, 4).reshape(B, Tn, H, -1).to(q.dtype)
+    return o.reshape(B, Hk, Tn, G, -1).permute(0, 2, 1, 3, 4).reshape(B, Tn, H, -1).to(q.dtype)
 
 
 # ----------------------------------------------------------------------------------------------
@@ -184,6 +186,9 @@ def kv4_read(pos, k_codes, k_params, v_codes=None, v_params=None, row_offset: in
     out = []
     for c, p, _ in pairs:
         ok = (rows >= 0) & (rows < c.shape[2])
+        if c.shape[2] == 0:
+            out.append(torch.zeros(*pos.shape, c.shape[1], 2 * c.shape[3], dtype=dtype, device=c.device))
+            continue
         safe = torch.where(ok, rows, torch.zeros_like(rows))
         b = torch.arange(rows.shape[0], device=rows.device)[:, None].expand_as(rows)
         x = dequantize_kv4(c[b, :, safe], p[b, :, safe], dtype)
@@ -203,7 +208,8 @@ def decode_attention_kv4(q, k, v, q_pos, kv_len, *, window=0, scale=None, k_para
         return _ext.load().kv4_attend(q, k, k_params, v, v_params, q_pos, kv_len, window, sc, latent_v_dim,
                                       sink_rows, n_sink)
     _check_cache(k, k_params, "decode_attention: k")
-    if q.dim() != 4 or q.shape[0] != k.shape[0] or q.shape[3] != 2 * k.shape[3] or q.shape[2] % max(1, k.shape[1]):
+    if q.dim() != 4 or q.shape[0] != k.shape[0] or q.shape[3] != 2 * k.shape[3] or k.shape[1] == 0 \
+            or q.shape[2] % k.shape[1]:
         raise ValueError(f"decode_attention: q {tuple(q.shape)} against codes {tuple(k.shape)}")
     if latent_v_dim:
         if v is not None or k.shape[1] != 1 or not 0 < latent_v_dim <= q.shape[3] \

@@ -281,6 +281,27 @@ def test_refusals():
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("latent", [0, 64])
+@pytest.mark.parametrize("B,rows,T", [(2, 0, 3), (0, 32, 3), (2, 32, 0), (0, 0, 0)])
+def test_empty_calls(device, latent, B, rows, T):
+    """A cache without rows reads as zeros and is attended as one that no query sees; no sequences, no
+    tokens: nothing."""
+    W, Hk = (128, 1) if latent else (64, 2)
+    (kc, kp), (vc, vp) = (kv4_alloc(B, Hk, rows, W, latent, device) for _ in range(2))
+    pos = torch.zeros(B, T, dtype=torch.long, device=device) + torch.arange(T, device=device)
+    x = torch.ones(B, T, Hk, W, device=device)
+    kv = (None, None, None) if latent else (x, vc, vp)
+    kv4_write(pos, x, kc, kp, *kv)
+    got = kv4_read(pos, kc, kp, *kv[1:])
+    for y in (got if isinstance(got, tuple) else (got,)):
+        assert y.shape == (B, T, Hk, W) and (y == (1 if rows else 0)).all()
+    q = torch.ones(B, T, 4, W, dtype=torch.bfloat16, device=device)
+    n = torch.full((B,), T, dtype=torch.int32, device=device)
+    o = decode_attention(q, kc, kv[1], pos, n, k_scale=kp, v_scale=kv[2], latent_v_dim=latent)
+    assert o.shape == (B, T, 4, latent or W) and (o == (1 if rows else 0)).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_one_tensor_for_keys_and_values_is_refused(device):
     """Codes or parameters that k and v would both write; heads of one allocation are fine."""
     (kc, kp), (vc, vp) = (kv4_alloc(1, 2, 32, 64, device=device) for _ in range(2))
