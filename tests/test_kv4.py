@@ -523,6 +523,52 @@ def test_attention_extreme_values(H, Hk, W, latent):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,Hk,W,latent", [(8, 8, 128, 0), (48, 8, 128, 0), (16, 2, 64, 0), (64, 4, 128, 0), (16, 1, 576, 512),
+                                           (16, 1, 320, 256), (4, 4, 32, 0)])
+@pytest.mark.parametrize("lens", [[130], [1], [40, 3, 0, 700, 128, 33, 1]])
+@pytest.mark.parametrize("Tn", [1, 4])
+def test_attention_in_a_cache_far_longer_than_the_text(H, Hk, W, latent, lens, Tn):
+    """The host plans for the allocated rows, the device finds a few of them used."""
+    case = _attend_case(len(lens), Tn, H, Hk, W, latent, 8192, seed=33, lens=lens)
+    _check_attention(*case, latent=latent)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,Hk,W,latent", [(48, 8, 128, 0), (64, 4, 128, 0), (32, 8, 64, 0), (16, 1, 576, 512), (16, 1, 320, 256)])
+def test_attention_rounds_weights_to_eleven_bits(H, Hk, W, latent):
+    """Values of usual sizes meet weights p s in fp16.  A weight's rounding is off by at most 2^-11 w s n, and
+    the roundings are independent: the mean square error is at most sum_t (2^-11 w s n)^2 and that of the
+    output's own rounding, 2^-11 |o| in fp16.  The scores are single products here (2^-20 of a weight:
+    a few fp32 roundings of scores up to 4 and the exponential's).  bf16 weights, 2^-8 w s |n - 8|, are
+    worse than that; so the oracle with such weights has to be."""
+    B, ctx = 64, 40
+    lens = [2 + i % 39 for i in range(B)]
+    q, kc, kp, vc, vp, q_pos, kv_len = _attend_case(B, 1, H, Hk, W, latent, ctx, seed=34, lens=lens, dtype=torch.float16)
+    g, L = W // kp.shape[3], kc.shape[2]
+    level = torch.randint(-128, 129, (L,), generator=torch.Generator().manual_seed(35)).cuda() / 32
+    q.zero_()
+    q[..., latent] = 2.0                                     # one dim against groups of one value: score = level
+    kp[:, :, :, latent // g:, 0], kp[:, :, :, latent // g:, 1] = 0, level.to(torch.bfloat16)[None, None, :, None]
+    out = decode_attention(q, kc, vc, q_pos, kv_len, k_scale=kp, v_scale=vp, latent_v_dim=latent, scale=0.5).double()
+    sc, sp = (kc, kp) if latent else (vc, vp)
+    V = latent or W
+    w = torch.softmax(level.double() + torch.where(torch.arange(L, device="cuda") < kv_len[:, None], 0.0, -math.inf), -1)
+    s = sp[..., 0].double().repeat_interleave(g, -1)[..., :V]
+    n = torch.stack([sc & 15, sc >> 4], -1).reshape(*sc.shape[:3], -1)[..., :V].double()
+    v = dequantize_kv4(sc, sp, torch.float64)[..., :V]
+    at = lambda x: torch.einsum("bl,bhld->bhd", w, x).repeat_interleave(H // Hk, 1)[:, None]
+    sq = lambda x: torch.einsum("bl,bhld->bhd", w ** 2, x ** 2).repeat_interleave(H // Hk, 1)[:, None]
+    want = at(v)
+    square = sq(2.0 ** -11 * s * n) + (2.0 ** -11 * want) ** 2 + (2.0 ** -19 * at(v.abs())) ** 2
+    err = (out - want).abs()
+    assert (err <= 2.0 ** -11 * (at(s * n) + want.abs()) * 1.001 + 2.0 ** -19 * at(v.abs())).all()
+    assert float((err ** 2).mean()) <= float(square.mean())
+    ws = w[:, None, :, None] * s
+    coarse = ((ws.to(torch.bfloat16).double() - ws) * (n - 8)).sum(2)
+    assert float((coarse ** 2).mean()) > 1.5 * float(square.mean())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("H,Hk,W,latent", [(8, 8, 128, 0), (48, 8, 128, 0), (4, 2, 64, 0), (16, 1, 576, 512), (16, 1, 320, 256)])
 @pytest.mark.parametrize("far", [2.0 ** 9, 2.0 ** 40])
 def test_attention_scales_far_apart(H, Hk, W, latent, far):
@@ -952,3 +998,70 @@ def test_speculative_decoding_on_gpu(kind, attn):
     ids = torch.randint(0, 512, (2, 100), generator=torch.Generator().manual_seed(6)).cuda()
     out, st = generate(m, ids, 10, temperature=0.0, kvq="int4", draft_model=draft, speculative_draft_len=3, return_stats=True)
     assert out.shape == (2, 110) and torch.equal(out[:, :100], ids)
+
+
+def _one_layer(kind, seed=0, window=0, mem=0, **attn):
+    """The entries of its cache depend on the embeddings alone, and its logits on the attention more than
+    on anything else (another context changes them by as much as they are)."""
+    from omnicoder.config import AttentionConfig, ModelConfig, MoEConfig
+    from omnicoder.models.lm import build_model
+    cfg = ModelConfig(name="kv4", vocab_size=512, d_model=256, n_layers=1, n_heads=4, ffn_dim=256, tie_embeddings=False,
+                      max_seq_len=512, attn=AttentionConfig(kind=kind, window=window, mem_slots=mem, **attn),
+                      moe=MoEConfig(n_experts=0))
+    return build_model(cfg, device="cuda", dtype=torch.bfloat16, seed=seed).eval().prepare_inference()
+
+
+def _check_tokens(m, out, S, first):
+    """Every generated token is the largest logit, but for twice what the two caches' logits may differ by,
+    of a cache that holds rounded entries and is given the same tokens: the entries in bf16, the
+    attention's output, the projection, the layer's end and its norm, each off by 2^-8 at most, are 2 % of the
+    largest logit.  first: prompt tokens of the first call."""
+    import types
+
+    from omnicoder.inference.kv_cache import KVCache
+    B, T = out.shape
+    c = _rounded_cache(m.cfg, B, T + 8, "cuda")
+    g = kv4_group(c.k[0].shape[-1], m.cfg.attn.kv_lora_rank if c.mla else 0)
+
+    def compress(self, window):
+        n = KVCache.compress_memory(self, window)
+        for t in [t for lst in (self.k, self.v) for t in lst if t is not None]:
+            t[:, :self.sink] = dequantize_kv4(*quantize_kv4(t[:, :self.sink], g), dtype=t.dtype)
+        return n
+
+    c.compress_memory = types.MethodType(compress, c)
+    with torch.no_grad():
+        logits = [m.forward_cached(out[:, :first], c, prefill=True, last_only=True)]
+        if m.cfg.attn.window and c.sink:
+            assert c.compress_memory(m.cfg.attn.window) == c.sink
+        logits += [m.forward_cached(out[:, i:i + 1], c) for i in range(first, T - 1)]
+    y = torch.cat(logits, 1)[:, S - first:]                  # of the tokens out[:, S:]
+    got = y.gather(-1, out[:, S:, None]).squeeze(-1)
+    assert (got >= y.amax(-1) - 2 * 2e-2 * y.abs().amax()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,attn", GPU_KINDS)
+@pytest.mark.parametrize("window,mem", [(0, 0), (96, 8)])
+def test_generated_tokens_on_gpu(kind, attn, window, mem):
+    """Greedy tokens of an int4 cache, captured steps, with a window and memory rows."""
+    from omnicoder.inference.generate import generate
+    m = _one_layer(kind, window=window, mem=mem, **attn)
+    ids = torch.randint(0, 512, (2, 200), generator=torch.Generator().manual_seed(7)).cuda()
+    out = generate(m, ids, 12, temperature=0.0, kvq="int4")
+    assert out.shape == (2, 212) and torch.equal(out[:, :200], ids)
+    _check_tokens(m, out, 200, 200)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,attn", GPU_KINDS)
+def test_rejected_drafts_on_gpu(kind, attn):
+    """A draft model of other weights: most of its tokens are rejected, and the rows that they took in the
+    cache are written over."""
+    from omnicoder.inference.generate import generate
+    m, draft = _one_layer(kind, **attn), _one_layer(kind, seed=1, **attn)
+    ids = torch.randint(0, 512, (2, 100), generator=torch.Generator().manual_seed(8)).cuda()
+    out, st = generate(m, ids, 12, temperature=0.0, kvq="int4", draft_model=draft, speculative_draft_len=3, return_stats=True)
+    assert out.shape == (2, 112) and torch.equal(out[:, :100], ids)
+    assert st.proposed_draft_tokens - st.accepted_draft_tokens >= 6
+    _check_tokens(m, out, 100, 99)
