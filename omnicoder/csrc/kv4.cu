@@ -538,8 +538,12 @@ void kv4_read(const Kv4IO& a, cudaStream_t s) {
   else kv4_launch(kv4_read_kernel<KV4_BF16>, grid, kIoThreads, 0, s, a, g);
 }
 
-// The tensor-core kernels take the rows that the models' caches have; any other goes to one block per
-// query row.  Measured, us tensor / row kernel (cold): 1 sequence of 32 rows, 2 heads of 64 9.1 / 47; 8 x 130
+// The tensor-core kernels take heads of 64 and 128 dims and latents of 512 + 64 and 256 + 64 (the dense,
+// draft, long-context and 24-layer presets); any other width goes to one block per query row, with a
+// sequence's keys in one block: heads of 32 (tiny_moe) and latents of 160 + 64 and 128 + 48 (the mobile
+// presets).  There the int8 cache's kernel, which splits them, can be faster; us int4 / int8, 4096 rows, 8
+// query heads: 8 heads of 32, 1 sequence 498 / 221, 16 535 / 3317; latent of 128 + 48, 1 sequence 722 / 73, 16
+// 754 / 415; latent of 160 + 64 775 (int8 does not take it).  Measured, us tensor / row kernel (cold): 1 sequence of 32 rows, 2 heads of 64 9.1 / 47; 8 x 130
 // rows, 8 heads of 128 11 / 66; 1 x 130 latent rows, 16 heads 20 / 100; 64 x 8192, 48 on 8 heads of 128
 // 147 / 19979.
 Kv4Plan kv4_plan(const Kv4Attend& a) {

@@ -48,14 +48,15 @@ __device__ __forceinline__ Kv4Seen kv4_seen(const Kv4Attend& a, int b, int t) {
 
 // ---- tensor-core tiles on registers ---------------------------------------------
 // Codes become matrix operands in registers, straight from the 4-bit tile in
-// shared memory; tcgen05 operands would have to be written back to shared or
-// tensor memory as wider tiles first, for a product of 8 or 16 columns that the
-// memory-bound kernel does not wait for.
+// shared memory.  tcgen05 operands would have to be written back to shared or
+// tensor memory first: as 16-bit tiles four times the bytes of the codes; as 8-bit
+// ones (a nibble in a byte is the e4m3 number n 2^-9) twice, with the queries and the
+// weights each split into two or three such numbers.  Neither was built.
 //
 // The two low nibbles of a 16-bit half, masked out, are the fp16 subnormals n 2^-24
 // and 16 n 2^-24, which the fp16 product takes exactly: two codes per AND.  (The
-// 8-bit float product, for which a nibble in a byte would be a number as it is, is
-// no instruction of its own here: 29 cycles against 8 for the fp16 one.)
+// 8-bit float product of this family, mma.sync, is emulated here: 29 cycles against 8
+// for the fp16 one.)
 __device__ __forceinline__ void mma_f16(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
   asm volatile(
@@ -168,7 +169,8 @@ __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
 }
 
 // Query rows enter the fp16 product with codes as q 2^e, the largest |q| of the
-// row in [2^14, 2^15): bf16 and fp16 values keep every bit down to 2^-39 of it.
+// row in [2^14, 2^15).  What fp16 rounds off is at most 2^-39 of it in even dims and, as odd
+// ones are stored a sixteenth as large (query_pairs), 2^-35 in odd ones.
 // `unscale` is 2^-e; the codes' 2^-24 is undone separately (kKv4Codes).
 constexpr float kKv4Codes = 16777216.f;
 __device__ __forceinline__ float q_normaliser(float amax, float* unscale) {
@@ -198,8 +200,8 @@ __device__ __forceinline__ bool kv4_score_factors(float (*rs)[2]) {  // this lan
 }
 
 // Eight dims of a normalised query, the partners of a code word: operands of two k steps (nibbles
-// 0 and 4 with 1 and 5, 2 and 6 with 3 and 7; the second pair of each counts 16-fold); -> their sum
-// (what fp16 rounds off is below 2^-39 of the row's largest).
+// 0 and 4 with 1 and 5, 2 and 6 with 3 and 7; the second pair of each counts 16-fold); -> their sum,
+// of the dims before that rounding: the minima meet the query as it is.
 __device__ __forceinline__ float query_pairs(const float* x, uint2* out) {
   float sum = 0.f;
 #pragma unroll

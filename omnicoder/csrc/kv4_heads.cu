@@ -6,7 +6,7 @@
 //   score_t = sum_g s_tg (q_g . n_tg) + m_tg sum(q_g)
 //   o_d     = sum_t (p_t s_tg) n_td + sum_t p_t m_tg
 // so that the tensor cores multiply integers: the query with the codes, and the
-// weights p s (rounded to fp16, the only rounding before the output's) with the
+// weights p s (rounded to fp16, or to bf16 where scales lie far apart) with the
 // codes.  The second sums stay in fp32.
 //
 // A block owns up to 16 query rows of a (sequence, key / value head) and a stretch
@@ -21,7 +21,7 @@
 // The running maximum moves only when a score exceeds it by 2^8, which keeps
 // the shuffles and the rescaling out of most tiles.
 //
-// Measured: 64 sequences x 8192 keys, 48 query heads on 8 of 128: 146 us, 4.1 TB/s
+// Measured: 64 sequences x 8192 keys, 48 query heads on 8 of 128: 142 - 147 us, 4.1 TB/s
 // (63 % of the measured copy bandwidth).  Bound by the instruction mix: ALU 51 %,
 // tensor 23 %, FMA 17 %, LSU 21 % of their cycles, which overlap little; 314
 // instructions per 16 keys.  One sequence of 8192 keys: 11.7 us, of 130 keys: 5.1 us.

@@ -14,11 +14,11 @@
 // m in bf16 as stored and sum(q_g) split into three bf16 terms: nine
 // multiply-adds per score less.
 //
-// Measured: 64 sequences x 4160 rows of 512 + 64 dims, 16 heads: 67 us, 1.3 TB/s.
+// Measured: 64 sequences x 4160 rows of 512 + 64 dims, 16 heads: 70 us, 1.3 TB/s.
 // Bound by tensor (33 %), ALU (41 %) and FMA (17 %) issue together and the three
 // phases' latency, which two blocks per SM do not hide; a third does not fit in
-// shared memory.  Four warps of two key tiles each took 78 us.  One sequence of 8192
-// rows: 13.2 us.
+// shared memory.  Their 128 registers spill 56 and 40 bytes (256 value dims: 8 and 8).
+// Four warps of two key tiles each took 78 us.  One sequence of 8192 rows: 13.7 us.
 #include <algorithm>
 
 #include "kv4_device.cuh"

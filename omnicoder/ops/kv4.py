@@ -7,7 +7,7 @@ A cache of one layer's keys (values have their own; an MLA latent is both):
 
 and stands for x = n * s + m, n = 0 .. 15.  A row of a head is contiguous, and so are the rows of a
 head (head-major, unlike the bf16 / int8 cache): the attention kernels copy whole key tiles.  With
-groups of 64 a value takes 4.5 bits; an int8 cache of 128-wide heads takes 8.25.
+groups of 64 a value takes 4.5 bits (32: 5, 16: 6); an int8 cache of 128-wide heads takes 8.25.
 
 Quantisation of a group: m = bf16(min x), s = bf16((max x - m) * (1 / 15)) with the product in fp32 (torch
 on a GPU divides by 15 so, on a CPU it does not: quotients halfway between two bf16 numbers differ), and
@@ -23,7 +23,8 @@ Position p of a sequence lives in row row_offset + p.  `kv4_write` skips positio
 outside the cache, `kv4_read` returns zeros for them.  The positions that one `kv4_write` call gives
 for a sequence have to differ: two tokens written to one row at once leave a mixture.
 
-CUDA: hand-written kernels (omnicoder/csrc/kv4*.cu; a call that does not fit raises RuntimeError);
+CUDA: hand-written kernels (omnicoder/csrc/kv4*.cu; a call that does not fit raises RuntimeError; a
+kernel whose copy never came gives NaN and omnicoder.ops._ext.check_status() raises);
 CPU: the plain forms below (the oracle; ValueError).
 """
 from __future__ import annotations
