@@ -29,9 +29,20 @@ void* status_ptr() {
   cudaGetDevice(&dev);
   std::lock_guard<std::mutex> lk(g_status_mu);
   if (g_status[dev] == nullptr) {
+    // The first call may stand inside a graph capture: the block is no part of the graph, and is cleared on
+    // a stream of its own before anyone has its address.
     void* p = nullptr;
-    C10_CUDA_CHECK(cudaMalloc(&p, 16));
-    C10_CUDA_CHECK(cudaMemset(p, 0, 16));
+    cudaStream_t own = nullptr;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    C10_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+    cudaError_t err = cudaMalloc(&p, 16);
+    if (err == cudaSuccess) err = cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking);
+    if (err == cudaSuccess) err = cudaMemsetAsync(p, 0, 16, own);
+    if (err == cudaSuccess) err = cudaStreamSynchronize(own);
+    if (own != nullptr) cudaStreamDestroy(own);
+    if (err != cudaSuccess && p != nullptr) cudaFree(p);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    C10_CUDA_CHECK(err);
     g_status[dev] = p;
   }
   return g_status[dev];

@@ -718,6 +718,63 @@ def test_attention_strides_streams_and_graphs(H, Hk, W, latent):
             assert torch.equal(o, want)
 
 
+_FIRST_CALL = """
+import torch
+from omnicoder.ops.decode import decode_attention
+from omnicoder.ops.kv4 import kv4_alloc, kv4_write
+H, Hk, W, latent = {shape}
+caches = [kv4_alloc(2, Hk, 512, W, latent, "cuda") for _ in range(2)]
+(kc, kp), (vc, vp) = caches if not latent else (caches[0], (None, None))
+x = torch.randn(2, 512, Hk, W, device="cuda")
+pos = torch.arange(512, device="cuda").expand(2, -1).contiguous()
+q = torch.randn(2, 1, H, W, device="cuda").to(torch.bfloat16)
+kv_len = torch.tensor([500, 20], dtype=torch.int32, device="cuda")
+q_pos = kv_len.long()[:, None] - 1
+
+def call():
+    kv4_write(pos, x, kc, kp, None if latent else x, vc, vp)
+    return decode_attention(q, kc, vc, q_pos, kv_len, k_scale=kp, v_scale=vp, latent_v_dim=latent)
+
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = call()
+g.replay()
+torch.cuda.synchronize()
+got = out.clone()
+assert got.abs().max() > 0 and torch.equal(got, call())
+print("captured first")
+"""
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(8, 8, 128, 0), (16, 1, 576, 512), (4, 4, 32, 0)])
+def test_the_first_call_of_a_process_is_captured(shape):
+    import subprocess
+    import sys
+    from pathlib import Path
+    r = subprocess.run([sys.executable, "-c", _FIRST_CALL.format(shape=shape)], cwd=Path(__file__).parents[1],
+                       capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0 and "captured first" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,Hk,W,latent", HEADS)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_attention_of_one_bad_query(H, Hk, W, latent, bad):
+    """A NaN or an infinity in one query row: that row is NaN, the others are as exact as ever.  (Not their
+    bits: the running maximum of a block's rows moves when one row's has grown by 2^8, so a row that no
+    longer calls for it changes where its neighbours' weights are rounded.)"""
+    q, kc, kp, vc, vp, q_pos, kv_len = _attend_case(2, 2, H, Hk, W, latent, 300, seed=36)
+    kw = dict(window=0, sink_rows=0, n_sink=0, scale=W ** -0.5)
+    q_bad = q.clone()
+    q_bad[1, 0, 0, 5] = bad
+    out = decode_attention(q_bad, kc, vc, q_pos, kv_len, k_scale=kp, v_scale=vp, latent_v_dim=latent, **kw)
+    assert torch.isnan(out[1, 0, 0]).all()
+    want, worst, _ = _bound(q, kc, kp, vc, vp, q_pos, kv_len, latent, out, kw)
+    out[1, 0, 0] = want[1, 0, 0].to(out.dtype)
+    assert ((out.double() - want).abs() <= worst).all()
+
+
 @pytest.mark.gpu
 def test_calls_at_once():
     """Appends, read-backs and attention of two caches on two streams, interleaved without waiting: the
